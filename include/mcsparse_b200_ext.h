@@ -240,6 +240,116 @@ mcsparseStatus_t mcsparseB200SpMVNoAlloc(mcsparseHandle_t handle, mcsparseOperat
                                          mcsparseDnVecDescr_t vecY, macaDataType computeType,
                                          mcsparseSpMVAlg_t alg);
 
+/* ------------------------------------------------------------------------------------------------------------
+ * Products with matrices that are never stored: rows of a table by token ids, and attention on a banded pattern.
+ * The reference has no counterpart; a caller of mcsparseSpMM would have to write such a matrix down as CSR.
+ * ------------------------------------------------------------------------------------------------------------ */
+
+/*
+ * mcsparseB200EmbeddingLookup: Y = alpha * S * E with S the count x rows matrix whose row t holds a single 1 in column
+ * indices[t] - idxBase. indices: device array of MCSPARSE_INDEX_32I or _64I. matE: rows x width, matY: count x width,
+ * both MCSPARSE_ORDER_ROW with any leading dimension >= width. Each is MACA_R_32F, MACA_R_16F or MACA_R_16BF; they share
+ * a type, or one of them is MACA_R_32F. alpha is a float (host or device memory, by the handle's pointer mode); products
+ * are formed in fp32 and rounded once. An index outside the table gives a row of zeros (padding). Strided batches are
+ * not supported. Asynchronous, no buffer, no allocation; E and Y must not overlap.
+ */
+mcsparseStatus_t mcsparseB200EmbeddingLookup(mcsparseHandle_t handle, const void* alpha, int64_t count,
+                                             const void* indices, mcsparseIndexType_t indexType,
+                                             mcsparseIndexBase_t idxBase, mcsparseDnMatDescr_t matE,
+                                             mcsparseDnMatDescr_t matY);
+
+/*
+ * mcsparseB200EmbeddingGradient: dE = alpha * S^T * dY + beta * dE for the same S. The tokens are sorted by index (stable),
+ * the rows of dY with one index are summed in fp32 in an order that depends on the indices and sizes alone, so equal
+ * inputs give equal bits. Types as in the lookup (matDY in the place of matY). beta == 0: dE is not read, rows without a
+ * token become zero. beta == 1: rows without a token are neither read nor written. Indices outside the table contribute
+ * nothing. externalBuffer: mcsparseB200EmbeddingGradient_bufferSize bytes, free again when the call's work is done;
+ * nothing in it outlives the call.
+ */
+mcsparseStatus_t mcsparseB200EmbeddingGradient_bufferSize(mcsparseHandle_t handle, int64_t count,
+                                                          mcsparseIndexType_t indexType, mcsparseDnMatDescr_t matDY,
+                                                          mcsparseDnMatDescr_t matDE, size_t* bufferSize);
+mcsparseStatus_t mcsparseB200EmbeddingGradient(mcsparseHandle_t handle, const void* alpha, int64_t count,
+                                               const void* indices, mcsparseIndexType_t indexType,
+                                               mcsparseIndexBase_t idxBase, mcsparseDnMatDescr_t matDY, const void* beta,
+                                               mcsparseDnMatDescr_t matDE, void* externalBuffer);
+
+/*
+ * Windowed attention. A sequence has Lq queries and Lk keys; query i stands at position p = Lk - Lq + i and sees key j iff
+ * j <= p and (j > p - window or j < sinks). O = P V with P the row softmax of scale * Q K^T over the seen keys; a query
+ * that sees no key gives a row of zeros and lse = -inf. Query head h reads key head h / (qHeads / kvHeads).
+ *
+ * The descriptor holds the pattern and the heads: window >= 1 (as large as the sequence: plain causal attention),
+ * sinks >= 0, qHeads a multiple of kvHeads, 1 <= headDim <= 128, valueType MACA_R_16BF, MACA_R_16F or MACA_R_32F.
+ */
+struct mcsparseB200WindowDescr;
+typedef struct mcsparseB200WindowDescr* mcsparseB200WindowDescr_t;
+mcsparseStatus_t mcsparseB200CreateWindow(mcsparseB200WindowDescr_t* descr, int64_t window, int64_t sinks, int qHeads,
+                                          int kvHeads, int headDim, float scale, macaDataType valueType);
+mcsparseStatus_t mcsparseB200DestroyWindow(mcsparseB200WindowDescr_t descr);
+
+/* One tensor of tokens x heads x headDim in device memory: element (t, h, d) = values[t * tokenStride + h * headStride + d].
+ * Strides in elements. Inputs may overlap themselves (a stride of 0 broadcasts); outputs may not. */
+typedef struct mcsparseB200Heads {
+    void* values;
+    int64_t tokenStride;
+    int64_t headStride;
+} mcsparseB200Heads_t;
+
+/*
+ * mcsparseB200WindowAttention: forward over a ragged batch. Sequence b holds queries [qOffsets[b], qOffsets[b + 1]) and keys
+ * [kOffsets[b], kOffsets[b + 1]) (device arrays of batch + 1 ascending int32; both NULL with batch == 1: one sequence of all
+ * tokens). totalQ / totalK: rows of the tensors; rows in no sequence are left as they were. lse: qHeads x totalQ floats
+ * (natural logarithm of the softmax sums), may be NULL. A result does not depend on keys and values that no query of its
+ * sequence sees; a value that is not finite in a key that some query sees may reach the sequence's other queries.
+ * fp32 scores, softmax statistics and sums; 16-bit inputs: the softmax weights are rounded to the inputs' type for the
+ * product with V, and O is rounded once. Asynchronous, no buffer, no allocation.
+ */
+mcsparseStatus_t mcsparseB200WindowAttention(mcsparseHandle_t handle, mcsparseB200WindowDescr_t descr, int64_t batch,
+                                             const int32_t* qOffsets, const int32_t* kOffsets, int64_t totalQ,
+                                             int64_t totalK, const mcsparseB200Heads_t* q, const mcsparseB200Heads_t* k,
+                                             const mcsparseB200Heads_t* v, const mcsparseB200Heads_t* o, float* lse);
+
+/*
+ * mcsparseB200WindowAttentionBackward: gradients of the same product. o and lse: what the forward call wrote; dO: the gradient
+ * of O; dQ, dK, dV are written (rows in no sequence are left as they were; keys that no query sees get zeros; shared key
+ * heads get the sum over their query heads). No atomics: equal inputs give equal bits. A dO that is not finite may reach
+ * every gradient of its sequence. externalBuffer: the bytes that _bufferSize reports, free again when the call's work is done.
+ */
+mcsparseStatus_t mcsparseB200WindowAttentionBackward_bufferSize(mcsparseHandle_t handle, mcsparseB200WindowDescr_t descr,
+                                                                int64_t batch, int64_t totalQ, int64_t totalK,
+                                                                size_t* bufferSize);
+mcsparseStatus_t mcsparseB200WindowAttentionBackward(
+    mcsparseHandle_t handle, mcsparseB200WindowDescr_t descr, int64_t batch, const int32_t* qOffsets,
+    const int32_t* kOffsets, int64_t totalQ, int64_t totalK, const mcsparseB200Heads_t* q, const mcsparseB200Heads_t* k,
+    const mcsparseB200Heads_t* v, const mcsparseB200Heads_t* o, const float* lse, const mcsparseB200Heads_t* dO,
+    const mcsparseB200Heads_t* dQ, const mcsparseB200Heads_t* dK, const mcsparseB200Heads_t* dV, void* externalBuffer);
+
+/*
+ * mcsparseB200WindowAttentionDecode: one query per sequence, the newest token of lengths[b] tokens in a cache.
+ * A cache holds numPages pages of pageSize tokens: token j of sequence b is token j % pageSize of page
+ * pageTable[b * maxPages + j / pageSize] (device int32; NULL: page b holds all of sequence b, and maxPages is 1), its element
+ * (h, d) at values[page * pageStride + token * tokenStride + h * headStride + d]. lengths: device int32; a length is taken
+ * as at most maxPages * pageSize, 0 (or less) gives zeros and lse = -inf. Tokens of a page number outside [0, numPages) are
+ * not seen; pages that lie wholly outside the window and the sinks are not read, their numbers neither.
+ * q, o: batch x qHeads x headDim (a token per sequence). lse: batch x qHeads floats, may be NULL.
+ */
+typedef struct mcsparseB200Cache {
+    void* values;
+    int64_t pageStride;
+    int64_t tokenStride;
+    int64_t headStride;
+} mcsparseB200Cache_t;
+mcsparseStatus_t mcsparseB200WindowAttentionDecode_bufferSize(mcsparseHandle_t handle, mcsparseB200WindowDescr_t descr,
+                                                              int64_t batch, int64_t maxPages, int64_t pageSize,
+                                                              size_t* bufferSize);
+mcsparseStatus_t mcsparseB200WindowAttentionDecode(mcsparseHandle_t handle, mcsparseB200WindowDescr_t descr, int64_t batch,
+                                                   const int32_t* lengths, const mcsparseB200Heads_t* q,
+                                                   const mcsparseB200Cache_t* kCache, const mcsparseB200Cache_t* vCache,
+                                                   int64_t numPages, int64_t pageSize, const int32_t* pageTable,
+                                                   int64_t maxPages, const mcsparseB200Heads_t* o, float* lse,
+                                                   void* externalBuffer);
+
 #ifdef __cplusplus
 }
 #endif

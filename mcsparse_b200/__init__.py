@@ -27,9 +27,23 @@ from .host import (  # noqa: F401
     spmv_buffer_size,
     spmv_preprocess,
 )
+from .operators import (  # noqa: F401
+    Window,
+    embedding_gradient,
+    embedding_gradient_buffer_size,
+    embedding_lookup,
+    window_attention,
+    window_attention_backward,
+    window_attention_backward_buffer_size,
+    window_attention_decode,
+    window_attention_decode_buffer_size,
+)
 
 __all__ = [
     "capi", "lib", "load_library", "check", "McsparseError", "Handle", "CsrMatrix", "CscMatrix", "DnVec", "DnMat",
     "HostSpmvPipeline",
     "spmv", "spmv_buffer_size", "spmv_preprocess", "spmm", "spmm_buffer_size", "spmm_preprocess",
+    "embedding_lookup", "embedding_gradient", "embedding_gradient_buffer_size", "Window", "window_attention",
+    "window_attention_backward", "window_attention_backward_buffer_size", "window_attention_decode",
+    "window_attention_decode_buffer_size",
 ]

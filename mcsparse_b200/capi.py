@@ -58,6 +58,19 @@ _CSRMV = [_vp, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]
 _CSRMVEX = [_vp, _i, _i, _i, _i, _i, _vp, _i, _vp, _vp, _i, _vp, _vp, _vp, _i, _vp, _i, _vp, _i, _i]
 _CSRMM2 = [_vp, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _i]
 _CSRMM = [_vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _i]
+
+
+class Heads(C.Structure):
+    """mcsparseB200Heads_t: a tokens x heads x head-dim tensor, strides in elements."""
+    _fields_ = [("values", _vp), ("tokenStride", _i64), ("headStride", _i64)]
+
+
+class Cache(C.Structure):
+    """mcsparseB200Cache_t: pages of tokens x heads x head-dim, strides in elements."""
+    _fields_ = [("values", _vp), ("pageStride", _i64), ("tokenStride", _i64), ("headStride", _i64)]
+
+
+_ph, _pc = C.POINTER(Heads), C.POINTER(Cache)
 PROTOTYPES = {
     "mcsparseCreate": (_i, [_pvp]),
     "mcsparseDestroy": (_i, [_vp]),
@@ -147,6 +160,17 @@ PROTOTYPES = {
     "mcsparseB200SpMVTransposedView": (_i, [_vp, _i, _vp, _pi64, _pvp, _pvp, _pvp]),
     "mcsparseB200ShardRowBounds": (_i, [_vp, _i64, _i64, _i, _vp, _i, _pi64]),
     "mcsparseB200ShardLocalRowOffsets": (_i, [_vp, _vp, _i64, _i64, _i, _vp]),
+    "mcsparseB200EmbeddingLookup": (_i, [_vp, _vp, _i64, _vp, _i, _i, _vp, _vp]),
+    "mcsparseB200EmbeddingGradient_bufferSize": (_i, [_vp, _i64, _i, _vp, _vp, _psz]),
+    "mcsparseB200EmbeddingGradient": (_i, [_vp, _vp, _i64, _vp, _i, _i, _vp, _vp, _vp, _vp]),
+    "mcsparseB200CreateWindow": (_i, [_pvp, _i64, _i64, _i, _i, _i, C.c_float, _i]),
+    "mcsparseB200DestroyWindow": (_i, [_vp]),
+    "mcsparseB200WindowAttention": (_i, [_vp, _vp, _i64, _vp, _vp, _i64, _i64, _ph, _ph, _ph, _ph, _vp]),
+    "mcsparseB200WindowAttentionBackward_bufferSize": (_i, [_vp, _vp, _i64, _i64, _i64, _psz]),
+    "mcsparseB200WindowAttentionBackward": (_i, [_vp, _vp, _i64, _vp, _vp, _i64, _i64, _ph, _ph, _ph, _ph, _vp,
+                                                 _ph, _ph, _ph, _ph, _vp]),
+    "mcsparseB200WindowAttentionDecode_bufferSize": (_i, [_vp, _vp, _i64, _i64, _i64, _psz]),
+    "mcsparseB200WindowAttentionDecode": (_i, [_vp, _vp, _i64, _vp, _ph, _pc, _pc, _i64, _i64, _vp, _i64, _ph, _vp, _vp]),
 }
 
 

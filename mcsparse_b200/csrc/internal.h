@@ -136,6 +136,13 @@ struct mcsparseDnMatDescr {
     int64_t batchCount = 1, batchStride = 0;
 };
 
+struct mcsparseB200WindowDescr {
+    int64_t window = 1, sinks = 0;
+    int q_heads = 1, kv_heads = 1, head_dim = 1;
+    float scale = 1.0f;
+    macaDataType valueType = MACA_R_16BF;
+};
+
 namespace mcsp_b200 {
 
 // alpha / beta as the kernels receive them: a host value, or a device address to read.
@@ -331,6 +338,11 @@ cudaError_t transpose_structure(cudaStream_t s, int64_t m, int64_t n, int64_t nn
 template <typename I>
 cudaError_t coo_sort_structure(cudaStream_t s, int64_t key_range, int64_t nnz, int base, const I* key_idx,
                                const I* other_idx, const TransposePlan& plan, void* buf);
+// The same sort alone: 0-based keys in [0, key_range] sorted with their positions (keys[final_slot()], perm[final_slot()]),
+// and the first place of every key in [0, key_range) at off_ptr (key_range + 1 entries; the last one is where the keys
+// equal to key_range start). The plan is transpose_plan(any, key_range + 1, count, any).
+cudaError_t sort_keys(cudaStream_t s, int64_t key_range, int64_t count, const int32_t* keys, const TransposePlan& plan,
+                      void* buf);
 // Array-of-pairs COO indices (row0, col0, row1, col1, ...; 8-byte aligned) -> two arrays.
 cudaError_t split_index_pairs(cudaStream_t s, int64_t nnz, const int32_t* pairs, int32_t* rows, int32_t* cols);
 // *host_flag = 1 if idx[0 .. count) is not ascending (one kernel, a 4-byte copy, a stream synchronisation).
@@ -349,5 +361,61 @@ cudaError_t shard_row_bounds(cudaStream_t s, int64_t m, int64_t nnz, int base, c
                              int num_shards, int64_t* bounds_host);
 cudaError_t shard_local_row_offsets(cudaStream_t s, const int32_t* row_ptr, int64_t first_row, int64_t num_rows,
                                     int base, int32_t* local);
+
+// Rows of a table by token ids and the table's gradient (checked arguments).
+struct EmbeddingArgs {
+    int64_t count = 0, rows = 0, width = 0;
+    const void* ids = nullptr;
+    bool wide_ids = false;
+    int base = 0;
+    void* table = nullptr;  // E, or dE
+    int64_t ld_table = 0;
+    macaDataType table_type = MACA_R_32F;
+    void* tokens = nullptr;  // Y, or dY
+    int64_t ld_tokens = 0;
+    macaDataType token_type = MACA_R_32F;
+    ScalarArg<float> alpha{1.0f, nullptr}, beta{0.0f, nullptr};
+};
+cudaError_t embedding_lookup(cudaStream_t s, const EmbeddingArgs& a);
+size_t embedding_gradient_bytes(int64_t count, int64_t rows, int64_t width);
+cudaError_t embedding_gradient(cudaStream_t s, const EmbeddingArgs& a, void* buffer);
+
+// Attention on a pattern of a window and first tokens (checked arguments; extents below 2^31).
+struct AttentionTensor {
+    void* p = nullptr;
+    int64_t token = 0, head = 0;  // strides in elements
+};
+struct AttentionArgs {
+    int batch = 0, total_q = 0, total_k = 0;
+    const int* q_offsets = nullptr;  // null: one sequence of all tokens
+    const int* k_offsets = nullptr;
+    int window = 1, sinks = 0;
+    int q_heads = 1, kv_heads = 1, dim = 1;
+    float scale = 1.0f;
+    macaDataType type = MACA_R_16BF;
+    int sm_count = 148;
+    WaitCfg wait;
+    AttentionTensor q, k, v, o, d_o, dq, dk, dv;
+    float* lse = nullptr;
+};
+struct DecodeArgs {
+    int batch = 0;
+    const int* lengths = nullptr;
+    const int* page_table = nullptr;  // null: page b holds sequence b
+    int64_t num_pages = 0, max_pages = 0, page_size = 1;
+    int64_t k_page = 0, v_page = 0;  // page strides in elements
+    int window = 1, sinks = 0;
+    int q_heads = 1, kv_heads = 1, dim = 1;
+    float scale = 1.0f;
+    macaDataType type = MACA_R_16BF;
+    int sm_count = 148;
+    AttentionTensor q, k, v, o;
+    float* lse = nullptr;
+};
+cudaError_t window_attention(cudaStream_t s, const AttentionArgs& a);
+size_t window_attention_backward_bytes(const AttentionArgs& a);
+cudaError_t window_attention_backward(cudaStream_t s, const AttentionArgs& a, void* buffer);
+size_t window_attention_decode_bytes(const DecodeArgs& a);
+cudaError_t window_attention_decode(cudaStream_t s, const DecodeArgs& a, void* buffer);
 
 }  // namespace mcsp_b200

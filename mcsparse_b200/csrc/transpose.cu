@@ -357,6 +357,14 @@ cudaError_t coo_sort_structure(cudaStream_t s, int64_t key_range, int64_t nnz, i
     return e;
 }
 
+cudaError_t sort_keys(cudaStream_t s, int64_t key_range, int64_t count, const int32_t* keys, const TransposePlan& p, void* buf) {
+    char* b = static_cast<char*>(buf);
+    const cudaError_t e = radix_sort_positions(s, count, 0, keys, p, buf);
+    if (e != cudaSuccess) return e;
+    return coo_row_offsets(s, key_range, count, 0, reinterpret_cast<const int*>(b + p.off_keys[p.final_slot()]),
+                           reinterpret_cast<int32_t*>(b + p.off_ptr));
+}
+
 __device__ int g_unsorted_flag;  // result word of indices_unsorted (one check at a time per process)
 static std::mutex g_unsorted_lock;  // one lock for every index type: the instantiations share the word above
 

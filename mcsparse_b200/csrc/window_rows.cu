@@ -1,0 +1,243 @@
+// Windowed attention, one warp per row: the form for every type, head size, stride and alignment. A warp holds its row in
+// registers (lane l: dimensions l, l + 32, l + 64, l + 96) and visits the keys (or queries) of its pattern one by one with a
+// running maximum and sum. Masked keys are never read. Bound by instruction issue (a shuffle reduction per pair).
+#include "window_common.h"
+
+namespace mcsp_b200 {
+namespace {
+
+using namespace window;
+
+constexpr int kSlots = 4;  // dimensions per lane
+constexpr int kWarps = 8;  // warps per block
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+    return v;
+}
+
+template <typename T>
+__device__ __forceinline__ void load_row(const T* p, int dim, int lane, float* out) {
+#pragma unroll
+    for (int i = 0; i < kSlots; ++i) out[i] = lane + 32 * i < dim ? to_float(p[lane + 32 * i]) : 0.0f;
+}
+template <typename T>
+__device__ __forceinline__ void store_row(T* p, int dim, int lane, const float* in) {
+#pragma unroll
+    for (int i = 0; i < kSlots; ++i)
+        if (lane + 32 * i < dim) p[lane + 32 * i] = from_float<T>(in[i]);
+}
+__device__ __forceinline__ float dot(const float* a, const float* b) {
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kSlots; ++i) s = fmaf(a[i], b[i], s);
+    return warp_sum(s);
+}
+
+template <typename T>
+__device__ __forceinline__ T* row_of(const AttentionTensor& t, int64_t token, int head) {
+    return static_cast<T*>(t.p) + token * t.token + head * t.head;
+}
+
+// Running softmax of one row.
+struct Softmax {
+    float m = -INFINITY, l = 0.0f, o[kSlots] = {};
+    __device__ __forceinline__ void add(float s, const float* v) {
+        const float top = fmaxf(m, s);
+        if (m != -INFINITY || s != -INFINITY) {  // (a score of -inf in a row that has seen nothing else adds nothing)
+            const float keep = expf(m - top), w = expf(s - top);
+            l = l * keep + w;
+#pragma unroll
+            for (int i = 0; i < kSlots; ++i) o[i] = o[i] * keep + w * v[i];
+            m = top;
+        }
+    }
+};
+
+template <typename T>
+__global__ void __launch_bounds__(32 * kWarps) window_rows_kernel(AttentionArgs a, Ragged r) {
+    const int64_t w = blockIdx.x * (int64_t)kWarps + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (w >= (int64_t)a.total_q * a.q_heads) return;
+    const int t = (int)(w / a.q_heads), h = (int)(w % a.q_heads), hk = h / (a.q_heads / a.kv_heads);
+    const int b = sequence_at(r.q_offsets, r.batch, r.total_q, t);
+    if (b < 0) return;
+    const Sequence sq = sequence_of(r, b);
+    const int p = sq.lk - sq.lq + (t - sq.q0);
+    float q[kSlots], k[kSlots], v[kSlots];
+    load_row(row_of<const T>(a.q, t, h), a.dim, lane, q);
+    Softmax sm;
+    const int low = max(p - a.window + 1, 0);
+    const int first = min(low, a.sinks);
+    for (int n = 0; n < first + (p - low + 1); ++n) {
+        const int j = n < first ? n : low + (n - first);
+        load_row(row_of<const T>(a.k, sq.k0 + j, hk), a.dim, lane, k);
+        load_row(row_of<const T>(a.v, sq.k0 + j, hk), a.dim, lane, v);
+        sm.add(dot(q, k) * a.scale, v);
+    }
+    const float inv = sm.l == 0.0f ? 0.0f : 1.0f / sm.l;
+#pragma unroll
+    for (int i = 0; i < kSlots; ++i) sm.o[i] *= inv;
+    store_row(row_of<T>(a.o, t, h), a.dim, lane, sm.o);
+    if (a.lse != nullptr && lane == 0) a.lse[(int64_t)h * a.total_q + t] = sm.l == 0.0f ? -INFINITY : sm.m + logf(sm.l);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(32 * kWarps) window_rows_dq_kernel(AttentionArgs a, Ragged r) {
+    const int64_t w = blockIdx.x * (int64_t)kWarps + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (w >= (int64_t)a.total_q * a.q_heads) return;
+    const int t = (int)(w / a.q_heads), h = (int)(w % a.q_heads), hk = h / (a.q_heads / a.kv_heads);
+    const int b = sequence_at(r.q_offsets, r.batch, r.total_q, t);
+    if (b < 0) return;
+    const Sequence sq = sequence_of(r, b);
+    const int p = sq.lk - sq.lq + (t - sq.q0);
+    float q[kSlots], k[kSlots], v[kSlots], go[kSlots], o[kSlots], dq[kSlots] = {};
+    load_row(row_of<const T>(a.q, t, h), a.dim, lane, q);
+    load_row(row_of<const T>(a.d_o, t, h), a.dim, lane, go);
+    load_row(row_of<const T>(a.o, t, h), a.dim, lane, o);
+    const float delta = dot(go, o), lse = a.lse[(int64_t)h * a.total_q + t];
+    const int low = max(p - a.window + 1, 0);
+    const int first = min(low, a.sinks);
+    for (int n = 0; n < first + (p - low + 1); ++n) {
+        const int j = n < first ? n : low + (n - first);
+        load_row(row_of<const T>(a.k, sq.k0 + j, hk), a.dim, lane, k);
+        load_row(row_of<const T>(a.v, sq.k0 + j, hk), a.dim, lane, v);
+        const float ds = expf(dot(q, k) * a.scale - lse) * (dot(go, v) - delta) * a.scale;
+#pragma unroll
+        for (int i = 0; i < kSlots; ++i) dq[i] = fmaf(ds, k[i], dq[i]);
+    }
+    store_row(row_of<T>(a.dq, t, h), a.dim, lane, dq);
+}
+
+// One warp per key row; the queries that see it, over all query heads that share it.
+template <typename T>
+__global__ void __launch_bounds__(32 * kWarps) window_rows_dkv_kernel(AttentionArgs a, Ragged r) {
+    const int64_t w = blockIdx.x * (int64_t)kWarps + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (w >= (int64_t)a.total_k * a.kv_heads) return;
+    const int t = (int)(w / a.kv_heads), hk = (int)(w % a.kv_heads), group = a.q_heads / a.kv_heads;
+    const int b = sequence_at(r.k_offsets, r.batch, r.total_k, t);
+    if (b < 0) return;
+    const Sequence sq = sequence_of(r, b);
+    const int j = t - sq.k0, shift = sq.lk - sq.lq;
+    float q[kSlots], k[kSlots], v[kSlots], go[kSlots], o[kSlots], dk[kSlots] = {}, dv[kSlots] = {};
+    load_row(row_of<const T>(a.k, t, hk), a.dim, lane, k);
+    load_row(row_of<const T>(a.v, t, hk), a.dim, lane, v);
+    const int i0 = max(j - shift, 0);
+    const int64_t last = j < a.sinks ? (int64_t)sq.lq : (int64_t)j + a.window - shift;
+    const int i1 = (int)(last < sq.lq ? last : sq.lq);
+    for (int h = hk * group; h < (hk + 1) * group; ++h) {
+        for (int i = i0; i < i1; ++i) {
+            const int tq = sq.q0 + i;
+            load_row(row_of<const T>(a.q, tq, h), a.dim, lane, q);
+            load_row(row_of<const T>(a.d_o, tq, h), a.dim, lane, go);
+            load_row(row_of<const T>(a.o, tq, h), a.dim, lane, o);
+            const float delta = dot(go, o);
+            const float pr = expf(dot(q, k) * a.scale - a.lse[(int64_t)h * a.total_q + tq]);
+            const float ds = pr * (dot(go, v) - delta) * a.scale;
+#pragma unroll
+            for (int d = 0; d < kSlots; ++d) {
+                dk[d] = fmaf(ds, q[d], dk[d]);
+                dv[d] = fmaf(pr, go[d], dv[d]);
+            }
+        }
+    }
+    store_row(row_of<T>(a.dk, t, hk), a.dim, lane, dk);
+    store_row(row_of<T>(a.dv, t, hk), a.dim, lane, dv);
+}
+
+// One block per (sequence, query head): the warps take the keys in turn, the block joins their softmaxes.
+template <typename T>
+__global__ void __launch_bounds__(32 * kWarps) window_rows_decode_kernel(DecodeArgs a) {
+    __shared__ float s_m[kWarps], s_l[kWarps], s_o[kWarps][32 * kSlots];
+    const int b = (int)(blockIdx.x / a.q_heads), h = (int)(blockIdx.x % a.q_heads), hk = h / (a.q_heads / a.kv_heads);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t room = a.max_pages * a.page_size;
+    const int len = (int)min((int64_t)max(__ldg(a.lengths + b), 0), room);
+    const int p = len - 1, low = max(p - a.window + 1, 0), first = min(low, a.sinks);
+    float q[kSlots], k[kSlots], v[kSlots];
+    load_row(row_of<const T>(a.q, b, h), a.dim, lane, q);
+    Softmax sm;
+    for (int n = warp; n < first + (p - low + 1); n += kWarps) {
+        const int j = n < first ? n : low + (n - first);
+        const int64_t page = a.page_table != nullptr ? (int64_t)__ldg(a.page_table + b * a.max_pages + j / a.page_size) : (int64_t)b;
+        if (page < 0 || page >= a.num_pages) continue;
+        const int64_t at = j % a.page_size;
+        load_row(static_cast<const T*>(a.k.p) + page * a.k_page + at * a.k.token + hk * a.k.head, a.dim, lane, k);
+        load_row(static_cast<const T*>(a.v.p) + page * a.v_page + at * a.v.token + hk * a.v.head, a.dim, lane, v);
+        sm.add(dot(q, k) * a.scale, v);
+    }
+    if (lane == 0) s_m[warp] = sm.m, s_l[warp] = sm.l;
+#pragma unroll
+    for (int i = 0; i < kSlots; ++i) s_o[warp][lane + 32 * i] = sm.o[i];
+    __syncthreads();
+    float m = -INFINITY, l = 0.0f;
+    for (int i = 0; i < kWarps; ++i) m = fmaxf(m, s_m[i]);
+    const float ref = m == -INFINITY ? 0.0f : m;
+    for (int i = 0; i < kWarps; ++i) l += s_l[i] * expf(s_m[i] - ref);
+    if ((int)threadIdx.x < a.dim) {
+        float o = 0.0f;
+        for (int i = 0; i < kWarps; ++i) o += s_o[i][threadIdx.x] * expf(s_m[i] - ref);
+        row_of<T>(a.o, b, h)[threadIdx.x] = from_float<T>(l == 0.0f ? 0.0f : o / l);
+    }
+    if (a.lse != nullptr && threadIdx.x == 0) a.lse[(int64_t)b * a.q_heads + h] = l == 0.0f ? -INFINITY : m + logf(l);
+}
+
+unsigned row_blocks(int64_t rows) { return (unsigned)((rows + kWarps - 1) / kWarps); }
+
+}  // namespace
+
+template <typename T>
+cudaError_t window_rows(cudaStream_t s, const AttentionArgs& a) {
+    const Ragged r{a.q_offsets, a.k_offsets, a.batch, a.total_q, a.total_k};
+    window_rows_kernel<T><<<row_blocks((int64_t)a.total_q * a.q_heads), 32 * kWarps, 0, s>>>(a, r);
+    return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t window_rows_backward(cudaStream_t s, const AttentionArgs& a) {
+    const Ragged r{a.q_offsets, a.k_offsets, a.batch, a.total_q, a.total_k};
+    if (a.total_q > 0) window_rows_dq_kernel<T><<<row_blocks((int64_t)a.total_q * a.q_heads), 32 * kWarps, 0, s>>>(a, r);
+    if (a.total_k > 0) window_rows_dkv_kernel<T><<<row_blocks((int64_t)a.total_k * a.kv_heads), 32 * kWarps, 0, s>>>(a, r);
+    return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t window_rows_decode(cudaStream_t s, const DecodeArgs& a) {
+    window_rows_decode_kernel<T><<<(unsigned)((int64_t)a.batch * a.q_heads), 32 * kWarps, 0, s>>>(a);
+    return cudaGetLastError();
+}
+
+// The type switch.
+#define MCSP_BY_TYPE(call)                                   \
+    do {                                                     \
+        switch (a.type) {                                    \
+            case MACA_R_32F: return call<float>(s, a);       \
+            case MACA_R_16F: return call<__half>(s, a);      \
+            case MACA_R_16BF: return call<__nv_bfloat16>(s, a); \
+            default: return cudaErrorInvalidValue;           \
+        }                                                    \
+    } while (0)
+
+cudaError_t window_attention(cudaStream_t s, const AttentionArgs& a) {
+    if (a.total_q == 0 || a.batch == 0) return cudaSuccess;
+    MCSP_BY_TYPE(window_rows);
+}
+
+size_t window_attention_backward_bytes(const AttentionArgs&) { return 256; }
+
+cudaError_t window_attention_backward(cudaStream_t s, const AttentionArgs& a, void*) {
+    if (a.batch == 0) return cudaSuccess;
+    MCSP_BY_TYPE(window_rows_backward);
+}
+
+size_t window_attention_decode_bytes(const DecodeArgs&) { return 256; }
+
+cudaError_t window_attention_decode(cudaStream_t s, const DecodeArgs& a, void*) {
+    if (a.batch == 0) return cudaSuccess;
+    MCSP_BY_TYPE(window_rows_decode);
+}
+
+}  // namespace mcsp_b200

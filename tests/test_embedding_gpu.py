@@ -1,0 +1,228 @@
+"""mcsparseB200EmbeddingLookup / EmbeddingGradient against a 64-bit restatement, on a GPU."""
+
+import ctypes as C
+
+import pytest
+import torch
+
+import mcsparse_b200 as mc
+from mcsparse_b200 import capi
+from mcsparse_b200.capi import lib
+from tests import operators_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [(torch.float32, torch.float32), (torch.float16, torch.float16), (torch.bfloat16, torch.bfloat16),
+         (torch.float32, torch.bfloat16), (torch.bfloat16, torch.float32), (torch.float16, torch.float32)]
+
+
+def mat(t):
+    return mc.DnMat(t, t.shape[0], t.shape[1], t.stride(0) if t.shape[0] > 1 else t.shape[1])
+
+
+def ids_for(count, rows, kind, device, seed=1, index=torch.int64, base=0):
+    g = torch.Generator().manual_seed(seed)
+    if kind == "one":  # one token fills the batch
+        ids = torch.full((count,), rows // 2)
+    elif kind == "each":  # no token twice
+        ids = torch.randperm(max(rows, count), generator=g)[:count] % rows
+    elif kind == "outside":  # half of them padding, on both sides of the table
+        ids = torch.randint(-rows, 2 * rows, (count,), generator=g)
+    elif kind == "edges":
+        ids = torch.randint(0, 2, (count,), generator=g) * (rows - 1)
+    else:
+        ids = (torch.rand(count, generator=g) ** 4 * rows).long()
+    return (ids + base).to(index).to(device)
+
+
+def strided(rows, cols, dtype, device, pad, offset, gen):
+    """A rows x cols view with a leading dimension of cols + pad, starting `offset` elements into its storage."""
+    whole = torch.empty(offset + rows * (cols + pad) + 16, dtype=dtype, device=device).normal_(generator=gen)
+    return whole, whole[offset:offset + rows * (cols + pad)].view(rows, cols + pad)[:, :cols]
+
+
+@pytest.mark.parametrize("types", TYPES, ids=lambda t: f"{str(t[0])[6:]}-{str(t[1])[6:]}")
+@pytest.mark.parametrize("width,pad,offset", [(1, 0, 0), (64, 0, 0), (1000, 24, 8), (777, 2, 0), (4096, 0, 0), (256, 1, 1)])
+@pytest.mark.parametrize("count", [1, 65])
+def test_lookup(handle, device, types, width, pad, offset, count):
+    te, ty = types
+    gen = torch.Generator(device=device).manual_seed(7)
+    rows, base = 37, count % 2
+    _, table = strided(rows, width, te, device, pad, offset, gen)
+    whole, out = strided(count, width, ty, device, pad, offset, gen)
+    before = whole.clone()
+    ids = ids_for(count, rows, "outside", device, index=torch.int32 if width % 2 else torch.int64, base=base)
+    mc.embedding_lookup(handle, ids, mat(table), mc.DnMat(out, count, width, width + pad), alpha=1.7, base=base)
+    i = ids.long() - base
+    ok = (i >= 0) & (i < rows)
+    # alpha reaches the kernel as an fp32 number
+    want = torch.where(ok[:, None], table.double()[i.clamp(0, rows - 1)] * float(torch.tensor(1.7)), 0.0)
+    ref.close(out, (want, (ref.U[ty] + 2 * ref.U32) * want.abs() + ref.TINY[ty]), "lookup")
+    after = whole.clone()
+    inside = torch.zeros_like(whole, dtype=torch.bool)
+    inside[offset:offset + count * (width + pad)].view(count, width + pad)[:, :width] = True
+    assert torch.equal(after[~inside], before[~inside]), "wrote outside its rows"
+
+
+def test_lookup_keeps_bits_and_device_alpha(handle, device):
+    table = torch.randn(500, 264, device=device, dtype=torch.bfloat16)
+    table[3] = float("nan")
+    table[4] = float("inf")
+    ids = torch.randint(5, 500, (300,), device=device)
+    out = torch.empty(300, 264, device=device, dtype=torch.bfloat16)
+    mc.embedding_lookup(handle, ids, mat(table), mat(out), alpha=2.0)
+    assert torch.equal(out, table[ids] * 2)
+    handle.set_pointer_mode(capi.MCSPARSE_POINTER_MODE_DEVICE)
+    try:
+        alpha = torch.full((1,), float("inf"), device=device)
+        ids[::3] = -1
+        mc.embedding_lookup(handle, ids, mat(table), mat(out), alpha=alpha)
+    finally:
+        handle.set_pointer_mode(capi.MCSPARSE_POINTER_MODE_HOST)
+    assert bool((out[::3] == 0).all()), "padding is zero whatever alpha is"
+
+
+def run_gradient(handle, ids, dy, table, alpha=1.0, beta=0.0, base=0):
+    m_y, m_e = mc.DnMat(dy, dy.shape[0], dy.shape[1], dy.stride(0)), mc.DnMat(table, *table.shape, table.stride(0))
+    buf = torch.empty(mc.embedding_gradient_buffer_size(handle, ids, m_y, m_e), dtype=torch.uint8, device=dy.device)
+    buf.fill_(0xA5)
+    mc.embedding_gradient(handle, ids, m_y, m_e, buf, alpha=alpha, beta=beta, base=base)
+
+
+@pytest.mark.parametrize("types", TYPES, ids=lambda t: f"{str(t[0])[6:]}-{str(t[1])[6:]}")
+@pytest.mark.parametrize("kind", ["one", "each", "outside", "edges", "skewed"])
+@pytest.mark.parametrize("count,rows,width", [(1, 1, 1), (7, 300, 40), (513, 301, 136), (4099, 97, 72), (3000, 5000, 515)])
+def test_gradient(handle, device, types, kind, count, rows, width):
+    te, ty = types
+    gen = torch.Generator(device=device).manual_seed(11)
+    index, base = (torch.int32, 1) if width % 2 else (torch.int64, 0)
+    ids = ids_for(count, rows, kind, device, index=index, base=base)
+    dy = torch.empty(count, width, dtype=ty, device=device).normal_(generator=gen)
+    for beta in (0.0, 1.0, -0.5):
+        table = torch.empty(rows, width, dtype=te, device=device).normal_(generator=gen)
+        if beta == 0.0:
+            table.fill_(float("nan"))  # not read
+        want = ref.gradient(ids, dy, rows, 0.75, beta, table, base)
+        run_gradient(handle, ids, dy, table, 0.75, beta, base)
+        ref.close(table, want, f"beta {beta}")
+
+
+@pytest.mark.parametrize("count", [2047, 2049, 16384, 16385, 40000, 131072, 140001])
+def test_gradient_long_batches(handle, device, count):
+    gen = torch.Generator(device=device).manual_seed(count)
+    ids = ids_for(count, 70000, "skewed", device, seed=count)
+    dy = torch.empty(count, 24, dtype=torch.bfloat16, device=device).normal_(generator=gen)
+    table = torch.empty(70000, 24, dtype=torch.float32, device=device)
+    run_gradient(handle, ids, dy, table)
+    ref.close(table, ref.gradient(ids, dy, 70000, 1.0, 0.0, table), "gradient")
+    again = torch.empty_like(table)
+    run_gradient(handle, ids, dy, again)
+    assert torch.equal(table, again), "equal inputs, equal bits"
+
+
+def test_gradient_strides_and_untouched_rows(handle, device):
+    gen = torch.Generator(device=device).manual_seed(3)
+    for pad, offset in ((8, 8), (3, 1)):
+        whole_y, dy = strided(600, 136, torch.bfloat16, device, pad, offset, gen)
+        whole, table = strided(90, 136, torch.float32, device, pad, offset, gen)
+        table[7] = float("nan")  # a row without tokens
+        ids = ids_for(600, 90, "skewed", device, index=torch.int32)
+        ids[ids == 7] = 8
+        before = whole.clone()
+        want = ref.gradient(ids, dy, 90, 1.0, 1.0, table)
+        run_gradient(handle, ids, dy, table, 1.0, 1.0)
+        keep = torch.ones(90, dtype=torch.bool, device=device)
+        keep[7] = False
+        ref.close(table[keep], (want[0][keep], want[1][keep]), "strided")
+        inside = torch.zeros_like(whole, dtype=torch.bool)
+        touched = torch.bincount(ids.long(), minlength=90) > 0
+        inside[offset:offset + 90 * (136 + pad)].view(90, 136 + pad)[:, :136] = touched[:, None]
+        same = (whole == before) | (whole.isnan() & before.isnan())
+        assert bool(same[~inside].all()), "beta = 1 leaves rows without tokens as they were"
+
+
+def test_gradient_empty(handle, device):
+    table = torch.randn(5, 8, device=device)
+    ids = torch.empty(1, dtype=torch.int64, device=device)[:0]
+    dy = torch.empty(1, 8, device=device)
+    m_y, m_e = mc.DnMat(dy, 0, 8, 8), mat(table)
+    buf = torch.empty(mc.embedding_gradient_buffer_size(handle, ids, m_y, m_e), dtype=torch.uint8, device=device)
+    before = table.clone()
+    mc.embedding_gradient(handle, ids, m_y, m_e, buf, beta=1.0)
+    assert torch.equal(table, before)
+    mc.embedding_gradient(handle, ids, m_y, m_e, buf, beta=2.0)
+    assert torch.equal(table, before * 2)
+    mc.embedding_gradient(handle, ids, m_y, m_e, buf, beta=0.0)
+    assert bool((table == 0).all())
+    mc.embedding_lookup(handle, ids, m_e, m_y)
+
+
+def test_gradient_captured_and_replayed(device):
+    """Two graphs that share one work buffer, replayed in turn on a stream of their own."""
+    stream = torch.cuda.Stream()
+    handle = mc.Handle(stream)
+    gen = torch.Generator(device=device).manual_seed(5)
+    sets = []
+    for n in (900, 2500):
+        ids = ids_for(n, 400, "skewed", device, seed=n)
+        dy = torch.empty(n, 128, dtype=torch.float16, device=device).normal_(generator=gen)
+        sets.append((ids, dy, torch.empty(400, 128, device=device)))
+    plans = [(i, mat(y), mat(e)) for i, y, e in sets]
+    buf = torch.empty(max(mc.embedding_gradient_buffer_size(handle, *p) for p in plans), dtype=torch.uint8, device=device)
+    graphs = []
+    torch.cuda.synchronize()
+    for p in plans:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            mc.embedding_gradient(handle, *p, buf)
+        graphs.append(g)
+    with torch.cuda.stream(stream):
+        for turn in range(3):
+            for (ids, dy, e), g in zip(sets, graphs):
+                dy.normal_(generator=gen)
+                ids.copy_(ids_for(ids.numel(), 400, ["skewed", "one", "outside"][turn], device, seed=turn))
+                e.fill_(float("nan"))
+                g.replay()
+                stream.synchronize()
+                ref.close(e, ref.gradient(ids, dy, 400, 1.0, 0.0, e), f"replay {turn}")
+    handle.close()
+
+
+def test_refusals(handle, device):
+    E, Y = torch.zeros(10, 16, device=device), torch.zeros(4, 16, device=device)
+    ids = torch.zeros(4, dtype=torch.int64, device=device)
+    one = C.c_float(1.0)
+    p1 = C.cast(C.byref(one), C.c_void_p)
+
+    def lookup(h=handle.h, alpha=p1, count=4, i=ids.data_ptr(), it=capi.MCSPARSE_INDEX_64I, base=0, e=None, y=None):
+        e, y = e or mat(E), y or mat(Y)
+        return lib.mcsparseB200EmbeddingLookup(h, alpha, count, i, it, base, e.d, y.d)
+
+    assert lookup() == 0
+    assert lookup(h=None) == capi.MCSPARSE_STATUS_NOT_INITIALIZED
+    invalid, refused = capi.MCSPARSE_STATUS_INVALID_VALUE, capi.MCSPARSE_STATUS_NOT_SUPPORTED
+    assert lookup(alpha=None) == invalid
+    assert lookup(i=None) == invalid
+    assert lookup(i=ids.data_ptr() + 4) == invalid
+    assert lookup(count=-1) == invalid
+    assert lookup(count=3) == invalid
+    assert lookup(base=2) == invalid
+    assert lookup(it=capi.MCSPARSE_INDEX_16U) == refused
+    assert lookup(e=mc.DnMat(E, 10, 16, 15)) == invalid
+    assert lookup(y=mc.DnMat(Y, 4, 8, 16)) == invalid
+    assert lookup(e=mc.DnMat(E, 10, 16, 16, order=capi.MCSPARSE_ORDER_COL)) == refused
+    assert lookup(e=mc.DnMat(E.double(), 10, 16, 16)) == refused
+    half, brain = mat(E.half()), mat(Y.bfloat16())
+    assert lookup(e=half, y=brain) == refused
+    size = C.c_size_t()
+    assert lib.mcsparseB200EmbeddingGradient_bufferSize(handle.h, 4, 3, mat(Y).d, mat(E).d, None) == invalid
+    assert lib.mcsparseB200EmbeddingGradient_bufferSize(handle.h, 4, 3, mat(Y).d, None, C.byref(size)) == invalid
+    m_y, m_e = mat(Y), mat(E)
+    assert lib.mcsparseB200EmbeddingGradient(handle.h, p1, 4, ids.data_ptr(), 3, 0, m_y.d, p1, m_e.d, None) == invalid
+    assert lib.mcsparseB200EmbeddingGradient(handle.h, p1, 4, ids.data_ptr(), 3, 0, m_y.d, None, m_e.d, 256) == invalid
+    with pytest.raises(ValueError):
+        mc.embedding_lookup(handle, ids.cpu(), m_e, m_y)
+    with pytest.raises(ValueError):
+        mc.embedding_lookup(handle, ids.float(), m_e, m_y)
+    with pytest.raises(ValueError):
+        mc.embedding_gradient(handle, ids, m_y, m_e, torch.empty(8, dtype=torch.uint8, device=device))
