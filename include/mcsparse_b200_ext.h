@@ -300,7 +300,7 @@ typedef struct mcsparseB200Heads {
  * mcsparseB200WindowAttention: forward over a ragged batch. Sequence b holds queries [qOffsets[b], qOffsets[b + 1]) and keys
  * [kOffsets[b], kOffsets[b + 1]) (device arrays of batch + 1 ascending int32; both NULL with batch == 1: one sequence of all
  * tokens). totalQ / totalK: rows of the tensors; rows in no sequence are left as they were. lse: qHeads x totalQ floats
- * (natural logarithm of the softmax sums), may be NULL. A result does not depend on keys and values that no query of its
+ * (natural logarithm of the softmax sums), may be NULL. totalQ, totalK and a sequence's cache are below 2^30 tokens. A result does not depend on keys and values that no query of its
  * sequence sees; a value that is not finite in a key that some query sees may reach the sequence's other queries.
  * fp32 scores, softmax statistics and sums; 16-bit inputs: the softmax weights are rounded to the inputs' type for the
  * product with V, and O is rounded once. Asynchronous, no buffer, no allocation.

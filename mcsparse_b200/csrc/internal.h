@@ -412,6 +412,16 @@ struct DecodeArgs {
     AttentionTensor q, k, v, o;
     float* lse = nullptr;
 };
+// One warp per row (window_rows.cu): every type, size and stride.
+cudaError_t window_rows_forward(cudaStream_t s, const AttentionArgs& a);
+cudaError_t window_rows_backward(cudaStream_t s, const AttentionArgs& a);
+cudaError_t window_rows_decode(cudaStream_t s, const DecodeArgs& a);
+// Tensor cores (window_forward.cu, window_backward.cu); cudaErrorNotSupported: the driver makes no tensor map of these tensors.
+bool window_tensor_ready(const AttentionTensor& t, int64_t tokens, int heads, int dim);
+cudaError_t window_forward_mma(cudaStream_t s, const AttentionArgs& a);
+size_t window_backward_mma_bytes(const AttentionArgs& a);
+cudaError_t window_backward_mma(cudaStream_t s, const AttentionArgs& a, void* buffer);
+// The choice between them (window_attention.cpp).
 cudaError_t window_attention(cudaStream_t s, const AttentionArgs& a);
 size_t window_attention_backward_bytes(const AttentionArgs& a);
 cudaError_t window_attention_backward(cudaStream_t s, const AttentionArgs& a, void* buffer);

@@ -91,7 +91,10 @@ AttentionTensor tensor(const mcsparseB200Heads_t* t) {
     return a;
 }
 
-int clip31(int64_t v) { return v > 0x7fffffffLL ? 0x7fffffff : (int)v; }
+// Token counts stay below 2^30, so that positions, and positions less a window, are int32; a longer window is all of them.
+constexpr int64_t kMostTokens = int64_t(1) << 30;
+bool too_many(int64_t v) { return v >= kMostTokens; }
+int clip(int64_t v) { return (int)(v > kMostTokens ? kMostTokens : v); }
 
 St attention_sizes(mcsparseHandle_t h, const mcsparseB200WindowDescr* d, int64_t batch, int64_t totalQ, int64_t totalK,
                    AttentionArgs* a) {
@@ -99,10 +102,10 @@ St attention_sizes(mcsparseHandle_t h, const mcsparseB200WindowDescr* d, int64_t
     if (d == nullptr) return BAD_POINTER;
     if (batch < 0 || totalQ < 0 || totalK < 0) return BAD_SIZE;
     // blocks of a launch: one per (row tile or row, head)
-    if (too_big(batch) || too_big(totalQ) || too_big(totalK) || (totalQ + totalK) / 8 + batch >= (int64_t(1) << 31) / d->q_heads)
+    if (too_big(batch) || too_many(totalQ) || too_many(totalK) || (totalQ + totalK) / 8 + batch >= (int64_t(1) << 31) / d->q_heads)
         return NOT_IMPL;
     a->batch = (int)batch, a->total_q = (int)totalQ, a->total_k = (int)totalK;
-    a->window = clip31(d->window), a->sinks = clip31(d->sinks);
+    a->window = clip(d->window), a->sinks = clip(d->sinks);
     a->q_heads = d->q_heads, a->kv_heads = d->kv_heads, a->dim = d->head_dim;
     a->scale = d->scale, a->type = d->valueType;
     a->sm_count = h->sm_count > 0 ? h->sm_count : 148;
@@ -124,11 +127,11 @@ St decode_sizes(mcsparseHandle_t h, const mcsparseB200WindowDescr* d, int64_t ba
     if (h == nullptr) return BAD_HANDLE;
     if (d == nullptr) return BAD_POINTER;
     if (batch < 0 || maxPages < 0 || pageSize < 1) return BAD_SIZE;
-    if (too_big(batch) || too_big(maxPages) || too_big(pageSize) || (maxPages > 0 && pageSize > 0x7fffffffLL / maxPages) ||
+    if (too_big(batch) || too_big(maxPages) || too_big(pageSize) || (maxPages > 0 && pageSize > (kMostTokens - 1) / maxPages) ||
         batch >= (int64_t(1) << 31) / d->q_heads)
         return NOT_IMPL;
     a->batch = (int)batch, a->max_pages = maxPages, a->page_size = pageSize;
-    a->window = clip31(d->window), a->sinks = clip31(d->sinks);
+    a->window = clip(d->window), a->sinks = clip(d->sinks);
     a->q_heads = d->q_heads, a->kv_heads = d->kv_heads, a->dim = d->head_dim;
     a->scale = d->scale, a->type = d->valueType;
     a->sm_count = h->sm_count > 0 ? h->sm_count : 148;

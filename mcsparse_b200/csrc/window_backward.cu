@@ -1,0 +1,604 @@
+// Windowed attention backward on the tensor cores (fp16 / bf16, rows of 16-byte multiples). With P = exp(S - lse) and
+// dS = P * (dP - delta), delta = rowsum(dO * O):
+//   keys kernel     one block per 128 keys and key head: S^T = K Q^T, dP^T = V dO^T, dV += P^T dO, dK += dS^T Q over the query
+//                   tiles of 64 that see them, for all query heads that share the keys (their sum stays in tensor memory);
+//   queries kernel  one block per 128 queries and query head: S = Q K^T, dP = dO V^T, dQ += dS K over the key tiles of 64.
+// Both are one kernel template: 128 stationary rows against a stream of 64-row tiles. S and dP have two buffers in tensor
+// memory, each with 128 threads (one row each) that turn them into P and dS in place, in 16 bits, while the tensor cores work
+// on the other buffer; P and dS enter the second products from tensor memory. Two kernels compute S and dP twice (7 products
+// instead of 5), which buys sums without atomics: equal inputs give equal bits, and nothing is kept in fp32 in HBM.
+//
+// The first tokens of a sequence are seen by all its queries. Their key tiles would run far longer than the others: what
+// lies past their window is cut into pieces of `chunk` queries, blocks of their own, whose partial sums (fp32) a last kernel
+// adds in order.
+#include <type_traits>
+
+#include "tensor_core.h"
+#include "window_common.h"
+#include "window_maps.h"
+
+namespace mcsp_b200 {
+namespace {
+
+using namespace window;
+using namespace tc;
+
+constexpr int kRows = 128;  // stationary rows of a block
+constexpr int kTile = 64;   // rows of a streamed tile
+constexpr int kStages = 4;
+constexpr int kThreads = 320;  // 2 x 128 for the element-wise part, the loading warp, the warp that issues the products
+constexpr float kLog2e = 1.4426950408889634f;
+
+template <int DP>
+struct Smem {
+    static constexpr int kFixed = kRows * DP * 2;   // one stationary operand
+    static constexpr int kStream = kTile * DP * 2;  // one streamed operand
+    static constexpr int kVectors = 2 * kTile * 4;  // -lse and delta of a streamed tile
+    static constexpr int kRing = 2 * kFixed;
+    static constexpr int kVec = kRing + kStages * 2 * kStream;
+    static constexpr int kBars = kVec + kStages * kVectors;
+    static constexpr int kTotal = kBars + 256 + 1024;
+};
+
+struct Params {
+    Ragged r;
+    int window, sinks, q_heads, kv_heads, group, dim, slots;
+    int q_mul, k_mul, v_mul, go_mul;
+    uint32_t negate;
+    float scale, scale_log2;
+    const float* lse;
+    const float* delta;  // q_heads x total_q
+    void *out1, *out2;   // dQ, or dV and dK
+    int64_t out1_token, out1_head, out2_token, out2_head;
+    // the first tokens' far queries
+    int chunk, far_slots, far_tiles;
+    float* partial;  // [2 * far_slots][far_tiles][kv_heads][2][kRows][DP]: far pieces, then what their own windows hold
+    long long limit;
+    int* fault;
+};
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// How the queries of a key tile (its first key key0) are shared out. [begin, mid): the block's own; pieces of `chunk` queries
+// from there when the tile holds first tokens and at least one whole piece is left (the last piece takes the remainder).
+struct Split {
+    int begin, mid, pieces;
+};
+__device__ __forceinline__ Split split_of(const Sequence& s, int key0, int window, int sinks, int chunk) {
+    const int shift = s.lk - s.lq;
+    const int last_key = min(key0 + kRows, s.lk) - 1;
+    Split v;
+    v.begin = max(key0 - shift, 0);
+    v.mid = (int)min((int64_t)s.lq, max((int64_t)last_key + window - shift, (int64_t)0));
+    v.pieces = 0;
+    if (key0 < sinks) {
+        const int left = s.lq - max(v.mid, v.begin);
+        if (left >= chunk)
+            v.pieces = left / chunk;
+        else
+            v.mid = s.lq;
+        v.mid = max(v.mid, v.begin);
+    }
+    return v;
+}
+// The sequence of far slot `number`, and its first number. Numbers start at k_offset / chunk: a sequence with n pieces is at
+// least n * chunk keys long, so that the numbers of different sequences differ.
+__device__ __forceinline__ RaggedBlock far_block(const Ragged& r, int number, int chunk, int lane) {
+    if (r.k_offsets == nullptr) return RaggedBlock{0, number};
+    int lo = 0, hi = r.batch;
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32;
+        const int b = lo + step * lane;
+        const bool below = b < hi && clamp_offset(__ldg(r.k_offsets + b), r.total_k) / chunk <= number;
+        const unsigned hits = __ballot_sync(0xffffffffu, below);
+        lo += step * (hits == 0 ? 0 : 31 - __clz(hits));
+        hi = min(lo + step, hi);
+    }
+    const int start = clamp_offset(__ldg(r.k_offsets + lo), r.total_k) / chunk;
+    return RaggedBlock{number >= start ? lo : -1, number - start};
+}
+
+// delta = rowsum(dO * O): 16 lanes per row, 8 values each.
+template <typename T>
+__global__ void __launch_bounds__(256) delta_kernel(AttentionArgs a, float* __restrict__ delta) {
+    const int64_t g = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> 4;
+    const int part = threadIdx.x & 15;
+    float sum = 0.0f;
+    const bool live = g < (int64_t)a.total_q * a.q_heads;
+    const int64_t t = live ? g / a.q_heads : 0, h = live ? g % a.q_heads : 0;
+    if (live && 8 * part < a.dim) {
+        const uint4 x = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.o.p) + t * a.o.token + h * a.o.head + 8 * part);
+        const uint4 y = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.d_o.p) + t * a.d_o.token + h * a.d_o.head + 8 * part);
+        const T *xv = reinterpret_cast<const T*>(&x), *yv = reinterpret_cast<const T*>(&y);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum = fmaf(to_float(xv[i]), to_float(yv[i]), sum);
+    }
+#pragma unroll
+    for (int d = 8; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    if (live && part == 0) delta[h * a.total_q + t] = sum;
+}
+
+// KEYS: stationary K, V; streamed Q, dO. Otherwise: stationary Q, dO; streamed K, V.
+template <typename T, int DP, bool KEYS>
+__global__ void __launch_bounds__(kThreads, 1)
+    window_backward_kernel(const __grid_constant__ CUtensorMap map_fixed1, const __grid_constant__ CUtensorMap map_fixed2,
+                           const __grid_constant__ CUtensorMap map_stream1, const __grid_constant__ CUtensorMap map_stream2,
+                           const Params a) {
+    using S = Smem<DP>;
+    constexpr bool kHalf = std::is_same<T, __half>::value;
+    constexpr int kBlocks = DP / 64;
+    // fp16 P is held 2^8 times too large (at most 256): weights below 2^-14 would lose bits to fp16's subnormal numbers. The
+    // factor leaves dS through the other factor of its product and dV at the end.
+    constexpr float kLift = kHalf ? 8.0f : 0.0f, kLower = kHalf ? 1.0f / 256.0f : 1.0f;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t smem = (smem_u32(smem_raw) + 1023) & ~1023u;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t bars = smem + S::kBars;
+    // barriers: stationary operands, full[stages], empty[stages], S and dP ready[2], P and dS ready[2], sums ready
+    const uint32_t bar_fixed = bars, bar_full = bars + 8, bar_empty = bar_full + 8 * kStages, bar_s = bar_empty + 8 * kStages,
+                   bar_p = bar_s + 16, bar_out = bar_p + 16, slot = bar_out + 8;
+
+    // ---- the block's rows and its stream
+    const int heads = KEYS ? a.kv_heads : a.q_heads;
+    const int head = blockIdx.x % heads;
+    const int number = (int)(blockIdx.x / heads);
+    const int far_blocks = KEYS ? a.far_slots * a.far_tiles : 0;
+    Sequence sq;
+    int row0, begin = 0, end = 0, hops = 1;  // streamed rows [begin, end), once per head that streams
+    int first = 0, low = 0;                  // queries kernel: key tiles [0, first) and from `low` on
+    int64_t partial = -1;                    // where the sums go instead of the outputs
+    if (KEYS) {
+        hops = a.group;
+        if (number < far_blocks) {
+            const int far = number / a.far_tiles, tile = number % a.far_tiles;
+            const RaggedBlock fb = far_block(a.r, far, a.chunk, lane);
+            if (fb.b < 0) return;
+            sq = sequence_of(a.r, fb.b);
+            row0 = tile * kRows;
+            if (row0 >= sq.lk) return;
+            const Split v = split_of(sq, row0, a.window, a.sinks, a.chunk);
+            if (fb.index >= v.pieces) return;
+            begin = v.mid + fb.index * a.chunk;
+            end = fb.index + 1 < v.pieces ? begin + a.chunk : sq.lq;
+            partial = ((int64_t)far * a.far_tiles + tile) * a.kv_heads + head;
+        } else {
+            const RaggedBlock rb = ragged_block(a.r.k_offsets, a.r.batch, a.r.total_k, number - far_blocks, kRows, lane);
+            if (rb.b < 0) return;
+            sq = sequence_of(a.r, rb.b);
+            if ((int64_t)rb.index * kRows >= sq.lk) return;
+            row0 = rb.index * kRows;
+            const Split v = split_of(sq, row0, a.window, a.sinks, a.chunk);
+            begin = v.begin, end = v.mid;
+            if (v.pieces > 0) {
+                const int far = (a.r.k_offsets == nullptr ? 0 : sq.k0 / a.chunk) + a.far_slots;
+                partial = ((int64_t)far * a.far_tiles + rb.index) * a.kv_heads + head;
+            }
+        }
+    } else {
+        const RaggedBlock rb = ragged_block(a.r.q_offsets, a.r.batch, a.r.total_q, a.slots - 1 - number, kRows, lane);
+        if (rb.b < 0) return;
+        sq = sequence_of(a.r, rb.b);
+        if ((int64_t)rb.index * kRows >= sq.lq) return;
+        row0 = rb.index * kRows;
+    }
+    const int shift = sq.lk - sq.lq;
+    const int rows = min(kRows, (KEYS ? sq.lk : sq.lq) - row0);
+    const int p_low = shift + row0, p_high = p_low + rows - 1;  // queries kernel: positions of the block
+    int tiles = 0;                                              // of one hop
+    if (KEYS) {
+        tiles = end > begin ? (end - begin + kTile - 1) / kTile : 0;
+    } else if (p_high >= 0) {
+        low = max(p_low - a.window + 1, 0) / kTile;
+        first = min((min(a.sinks, p_high + 1) + kTile - 1) / kTile, low);
+        tiles = first + p_high / kTile - low + 1;
+    }
+    const int n = tiles * hops;
+    // first streamed row of tile i, relative to the sequence
+    const auto tile_row = [&](int i) {
+        if (KEYS) return begin + (i % tiles) * kTile;
+        return (i < first ? i : low + (i - first)) * kTile;
+    };
+
+    if (warp == 9) {
+        tmem_alloc(slot, 512);
+    } else if (threadIdx.x == 256) {
+        bar_init(bar_fixed, 1);
+        for (int i = 0; i < kStages; ++i) bar_init(bar_full + 8 * i, 1), bar_init(bar_empty + 8 * i, 1);
+        for (int i = 0; i < 2; ++i) bar_init(bar_s + 8 * i, 1), bar_init(bar_p + 8 * i, kRows);
+        bar_init(bar_out, 1);
+        bar_init_fence();
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    uint32_t tmem;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(slot));
+    // tensor memory: S[2] and dP[2] of 64 columns, then the sums (dV and dK, or dQ)
+    const uint32_t t_s = tmem, t_dp = tmem + 2 * kTile, t_out1 = tmem + 4 * kTile, t_out2 = t_out1 + DP;
+    bool failed = false;
+
+    if (warp == 8) {
+        // ---- loads
+        if (n > 0) {
+            const int hk = KEYS ? head : head / a.group;
+            if (lane == 0) {
+                bar_expect(bar_fixed, 2 * S::kFixed);
+                const int h1 = head * (KEYS ? a.k_mul : a.q_mul), h2 = head * (KEYS ? a.v_mul : a.go_mul);
+                const int row = (KEYS ? sq.k0 : sq.q0) + row0;
+                for (int c = 0; c < kBlocks; ++c) {
+                    tma_load_3d(smem + c * (kRows * 128), &map_fixed1, 64 * c, h1, row, bar_fixed);
+                    tma_load_3d(smem + S::kFixed + c * (kRows * 128), &map_fixed2, 64 * c, h2, row, bar_fixed);
+                }
+            }
+            // -lse (base 2) and delta of the tile's queries, fetched one tile ahead; a row that is none has -lse = -inf: P = 0
+            float l[2], d[2];
+            const auto fetch = [&](int i) {
+                if (!KEYS || i >= n) return;
+                const int h = head * a.group + i / tiles, row = tile_row(i);
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const int q = row + 2 * lane + x;
+                    l[x] = -INFINITY, d[x] = 0.0f;
+                    if (q < end) {
+                        const int64_t at = (int64_t)h * a.r.total_q + sq.q0 + q;
+                        const float v = __ldg(a.lse + at);
+                        if (v != -INFINITY) l[x] = kLift - v * kLog2e;
+                        d[x] = -kLower * __ldg(a.delta + at);
+                    }
+                }
+            };
+            fetch(0);
+            int issued = 0;
+            for (int i = 0; i < n; ++i) {
+                const int st = i % kStages;
+                if (i >= kStages && !bar_wait_warp(bar_empty + 8 * st, (i / kStages - 1) & 1, a.limit)) {
+                    failed = true;
+                    break;
+                }
+                if (KEYS) {
+                    const uint32_t vec = smem + S::kVec + st * S::kVectors + 8 * lane;
+                    asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(vec), "f"(l[0]), "f"(l[1]) : "memory");
+                    asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(vec + 4 * kTile), "f"(d[0]), "f"(d[1]) : "memory");
+                    fetch(i + 1);
+                    __syncwarp();
+                }
+                if (lane == 0) {
+                    bar_expect(bar_full + 8 * st, 2 * S::kStream);
+                    const int h = KEYS ? head * a.group + i / tiles : hk;
+                    const int h1 = h * (KEYS ? a.q_mul : a.k_mul), h2 = h * (KEYS ? a.go_mul : a.v_mul);
+                    const int row = (KEYS ? sq.q0 : sq.k0) + tile_row(i);
+                    const uint32_t to = smem + S::kRing + st * 2 * S::kStream;
+                    for (int c = 0; c < kBlocks; ++c) {
+                        tma_load_3d(to + c * (kTile * 128), &map_stream1, 64 * c, h1, row, bar_full + 8 * st);
+                        tma_load_3d(to + S::kStream + c * (kTile * 128), &map_stream2, 64 * c, h2, row, bar_full + 8 * st);
+                    }
+                }
+                issued = i + 1;
+            }
+            if (failed) {  // nothing of this block's memory is given back while a copy is on its way
+                bar_wait(bar_fixed, 0, a.limit);
+                for (int i = max(0, issued - kStages); i < issued; ++i) bar_wait(bar_full + 8 * (i % kStages), (i / kStages) & 1, a.limit);
+            }
+        }
+        __syncwarp();
+    } else if (warp == 9) {
+        // ---- products
+        constexpr uint32_t kDescS = mma_desc(!kHalf, kTile, false), kDescOut = mma_desc(!kHalf, DP, true);
+        const int first_seen = max(p_low - a.window + 1, 0);  // queries kernel: keys that some row here sees
+        if (n > 0) failed = !bar_wait_warp(bar_fixed, 0, a.limit);
+        for (int i = 0; i <= n && n > 0 && !failed; ++i) {
+            if (i < n) {
+                const int st = i % kStages, b = i & 1;
+                if (!bar_wait_warp(bar_full + 8 * st, (i / kStages) & 1, a.limit)) {
+                    failed = true;
+                    break;
+                }
+                const uint32_t s1 = smem + S::kRing + st * 2 * S::kStream, s2 = s1 + S::kStream;
+                // Rows whose weight is zero for every row here are cleared before they enter a sum: zero times a NaN that
+                // lies there would not be zero. Keys kernel: queries behind the last one; queries kernel: keys nobody sees.
+                const int row = tile_row(i);
+                const int clear_low = KEYS ? 0 : min(max(first_seen - row, 0), kTile);
+                const int keep = KEYS ? 0 : min(max(a.sinks - row, 0), kTile);
+                const int clear_high = min(max((KEYS ? end : p_high + 1) - row, 0), kTile);
+                if (clear_low > keep || clear_high < kTile) {
+                    for (int x = lane; x < (KEYS ? 2 : 1) * kTile * 8 * kBlocks; x += 32) {  // (stream 2 lies behind stream 1)
+                        const int at = (x >> 3) & (kTile - 1);
+                        if ((at < clear_low && at >= keep) || at >= clear_high)
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(s1 + x * 16), "r"(0) : "memory");
+                    }
+                    fence_async();
+                    __syncwarp();
+                }
+                if (lane == 0) {
+#pragma unroll
+                    for (int k = 0; k < DP / 16; ++k) {
+                        const uint32_t fixed = (k >> 2) * (kRows * 128) + (k & 3) * 32, stream = (k >> 2) * (kTile * 128) + (k & 3) * 32;
+                        mma_ss(t_s + kTile * b, smem_desc(smem + fixed), smem_desc(s1 + stream), kDescS | a.negate, k > 0);
+                    }
+#pragma unroll
+                    for (int k = 0; k < DP / 16; ++k) {
+                        const uint32_t fixed = (k >> 2) * (kRows * 128) + (k & 3) * 32, stream = (k >> 2) * (kTile * 128) + (k & 3) * 32;
+                        mma_ss(t_dp + kTile * b, smem_desc(smem + S::kFixed + fixed), smem_desc(s2 + stream), kDescS, k > 0);
+                    }
+                    mma_commit(bar_s + 8 * b);
+                }
+                __syncwarp();
+            }
+            if (i > 0) {
+                const int st = (i - 1) % kStages, b = (i - 1) & 1;
+                if (!bar_wait_warp(bar_p + 8 * b, ((i - 1) >> 1) & 1, a.limit)) {
+                    failed = true;
+                    break;
+                }
+                fence_after();
+                if (lane == 0) {
+                    const uint32_t s1 = smem + S::kRing + st * 2 * S::kStream, s2 = s1 + S::kStream;
+                    if (KEYS) {
+#pragma unroll
+                        for (int k = 0; k < kTile / 16; ++k)
+                            mma_ts(t_out1, t_s + kTile * b + 8 * k, smem_desc(s2 + k * 2048, kTile * 128), kDescOut, i > 1 || k > 0);
+                    }
+#pragma unroll
+                    for (int k = 0; k < kTile / 16; ++k)
+                        mma_ts(KEYS ? t_out2 : t_out1, t_dp + kTile * b + 8 * k, smem_desc(s1 + k * 2048, kTile * 128), kDescOut, i > 1 || k > 0);
+                    mma_commit(bar_empty + 8 * st);
+                    if (i == n) mma_commit(bar_out);
+                }
+                __syncwarp();
+            }
+        }
+        if (failed && lane == 0) {  // the tensor memory is given back only when no product uses it any more
+            mma_commit(bar_fixed);
+            bar_wait(bar_fixed, 1, a.limit);
+        }
+        __syncwarp();
+    } else {
+        // ---- P and dS: thread = stationary row, buffer b = its warpgroup
+        const int b = warp >> 2;
+        const int r = threadIdx.x & (kRows - 1);
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21;
+        const int64_t token = (int64_t)(KEYS ? sq.k0 : sq.q0) + row0 + r;
+        float own_l = -INFINITY, own_d = 0.0f;  // queries kernel: the row's -lse and -delta
+        if (!KEYS && r < rows) {
+            const int64_t at = (int64_t)head * a.r.total_q + token;
+            const float v = __ldg(a.lse + at);
+            if (v != -INFINITY) own_l = kLift - v * kLog2e;
+            own_d = -kLower * __ldg(a.delta + at);
+        }
+        int done = 0;
+        for (int i = b; i < n; i += 2) {
+            // (the second wait is over by then; it is there for the vectors, which ordinary stores wrote)
+            if (!bar_wait_warp(bar_s + 8 * b, done & 1, a.limit) ||
+                (KEYS && !bar_wait_warp(bar_full + 8 * (i % kStages), (i / kStages) & 1, a.limit))) {
+                failed = true;
+                break;
+            }
+            fence_after();
+            uint32_t s[kTile], d[kTile];
+            tmem_load32(t_s + kTile * b + lanes, s);
+            tmem_load32(t_s + kTile * b + lanes + 32, s + 32);
+            tmem_load32(t_dp + kTile * b + lanes, d);
+            tmem_load32(t_dp + kTile * b + lanes + 32, d + 32);
+            wait_loads();
+            after_loads32(s), after_loads32(s + 32), after_loads32(d), after_loads32(d + 32);
+            const int row = tile_row(i);
+            uint64_t seen = ~0ull;
+            if (KEYS) {
+                // key j = row0 + r, query at position p = shift + row + c: seen iff p >= j and (p < j + window or j < sinks)
+                const int p0 = shift + row, j = row0 + r;
+                if (p0 < row0 + kRows - 1 || (p0 + kTile - 1 >= row0 + a.window && row0 + kRows > a.sinks)) {
+                    const int from = min(max(j - p0, 0), 64);
+                    const int upto = j < a.sinks ? 64 : min(max(j + a.window - p0, 0), 64);
+                    seen = (from < 64 ? ~0ull << from : 0ull) & (upto < 64 ? (1ull << upto) - 1 : ~0ull);
+                }
+            } else {
+                // query at p, key j = row + c: seen iff j <= p and (j > p - window or j < sinks)
+                const int p = p_low + r;
+                if (row + kTile - 1 > p_low || (row <= p_low + kRows - 1 - a.window && row + kTile > a.sinks)) {
+                    const int upto = min(max(p + 1 - row, 0), 64), from = min(max(p - a.window + 1 - row, 0), 64);
+                    const int keep = min(max(a.sinks - row, 0), 64);
+                    const uint64_t near = from < 64 ? ~0ull << from : 0ull, kept = keep < 64 ? (1ull << keep) - 1 : ~0ull;
+                    seen = (near | kept) & (upto < 64 ? (1ull << upto) - 1 : ~0ull);
+                }
+            }
+            const uint32_t vec = smem + S::kVec + (i % kStages) * S::kVectors;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint32_t wp[16], wd[16];
+                const uint32_t bits = (uint32_t)(seen >> (32 * h));
+#pragma unroll
+                for (int c = 0; c < 32; c += 4) {
+                    float l[4], e[4], p[4], g[4];
+                    if (KEYS) {
+                        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                     : "=f"(l[0]), "=f"(l[1]), "=f"(l[2]), "=f"(l[3])
+                                     : "r"(vec + 4 * (32 * h + c)));
+                        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                     : "=f"(e[0]), "=f"(e[1]), "=f"(e[2]), "=f"(e[3])
+                                     : "r"(vec + 4 * (kTile + 32 * h + c)));
+                    }
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const int at = 32 * h + c + x;
+                        p[x] = exp2_fast(fmaf(__uint_as_float(s[at]), a.scale_log2, KEYS ? l[x] : own_l));
+                        g[x] = p[x] * fmaf(__uint_as_float(d[at]), kLower, KEYS ? e[x] : own_d);
+                        if (!(bits >> (c + x) & 1)) p[x] = 0.0f, g[x] = 0.0f;
+                    }
+                    wp[c >> 1] = pack2<T>(p[0], p[1]);
+                    wp[(c >> 1) + 1] = pack2<T>(p[2], p[3]);
+                    wd[c >> 1] = pack2<T>(g[0], g[1]);
+                    wd[(c >> 1) + 1] = pack2<T>(g[2], g[3]);
+                }
+                if (KEYS) tmem_store16(t_s + kTile * b + lanes + 16 * h, wp);
+                tmem_store16(t_dp + kTile * b + lanes + 16 * h, wd);
+            }
+            wait_stores();
+            fence_before();
+            bar_arrive(bar_p + 8 * b);
+            ++done;
+        }
+        // ---- outputs: keys kernel: one warpgroup writes dV, the other dK; queries kernel: each half of dQ's columns
+        if (n > 0 && !failed) {
+            failed = !bar_wait_warp(bar_out, 0, a.limit);
+            fence_after();
+        }
+        const uint32_t t_out = KEYS && b == 1 ? t_out2 : t_out1;
+        const float factor = KEYS && b == 0 ? kLower : a.scale;
+        T* out = b == 1 && KEYS ? static_cast<T*>(a.out2) + token * a.out2_token + (int64_t)head * a.out2_head
+                                : static_cast<T*>(a.out1) + token * a.out1_token + (int64_t)head * a.out1_head;
+        float* part = partial < 0 ? nullptr : a.partial + ((partial * 2 + b) * kRows + r) * DP;
+        const int c0 = KEYS ? 0 : b * (DP / 2), c1 = KEYS ? DP : c0 + DP / 2;
+#pragma unroll 1
+        for (int c = c0; c < c1; c += 32) {
+            uint32_t o[32];
+            if (n > 0 && !failed) {
+                tmem_load32(t_out + lanes + c, o);
+                wait_loads();
+                after_loads32(o);
+            } else {
+#pragma unroll
+                for (int x = 0; x < 32; ++x) o[x] = 0u;
+            }
+            if (failed) continue;
+            if (part != nullptr) {
+#pragma unroll
+                for (int x = 0; x < 32; x += 4) *reinterpret_cast<uint4*>(part + c + x) = make_uint4(o[x], o[x + 1], o[x + 2], o[x + 3]);
+            } else if (r < rows) {
+#pragma unroll
+                for (int x = 0; x < 32; x += 8) {
+                    if (c + x < a.dim) {
+                        uint4 w;
+                        w.x = pack2<T>(__uint_as_float(o[x]) * factor, __uint_as_float(o[x + 1]) * factor);
+                        w.y = pack2<T>(__uint_as_float(o[x + 2]) * factor, __uint_as_float(o[x + 3]) * factor);
+                        w.z = pack2<T>(__uint_as_float(o[x + 4]) * factor, __uint_as_float(o[x + 5]) * factor);
+                        w.w = pack2<T>(__uint_as_float(o[x + 6]) * factor, __uint_as_float(o[x + 7]) * factor);
+                        *reinterpret_cast<uint4*>(out + c + x) = w;
+                    }
+                }
+            }
+        }
+        fence_before();
+    }
+    if (failed && a.fault != nullptr) *reinterpret_cast<volatile int*>(a.fault) = 1;
+    __syncthreads();
+    if (warp == 9) {
+        fence_after();
+        tmem_free(tmem, 512);
+    }
+}
+
+// The sums of a first-tokens tile: what its own window holds, then its far pieces in order. One block per (sequence by its
+// first far slot, key tile, key head, which of dV and dK); thread = 4 values.
+template <typename T, int DP>
+__global__ void __launch_bounds__(256) window_backward_join_kernel(const Params a) {
+    const int lane = threadIdx.x & 31;
+    int64_t x = blockIdx.x;
+    const int which = (int)(x & 1), head = (int)((x >> 1) % a.kv_heads);
+    x = (x >> 1) / a.kv_heads;
+    const int tile = (int)(x % a.far_tiles), far = (int)(x / a.far_tiles);
+    const RaggedBlock fb = far_block(a.r, far, a.chunk, lane);
+    if (fb.b < 0 || fb.index != 0) return;
+    const Sequence sq = sequence_of(a.r, fb.b);
+    const int row0 = tile * kRows;
+    if (row0 >= sq.lk) return;
+    const Split v = split_of(sq, row0, a.window, a.sinks, a.chunk);
+    if (v.pieces == 0) return;
+    const float factor = which == 0 ? (std::is_same<T, __half>::value ? 1.0f / 256.0f : 1.0f) : a.scale;
+    const auto part = [&](int64_t f) { return a.partial + ((((f * a.far_tiles + tile) * a.kv_heads + head) * 2 + which) * (int64_t)kRows) * DP; };
+    for (int i = threadIdx.x * 4; i < kRows * DP; i += 256 * 4) {
+        const int r = i / DP, c = i % DP;
+        if (row0 + r >= sq.lk || c >= a.dim) continue;
+        float4 s = *reinterpret_cast<const float4*>(part((int64_t)a.far_slots + far) + i);
+        for (int f = 0; f < v.pieces; ++f) {
+            const float4 y = *reinterpret_cast<const float4*>(part(far + f) + i);
+            s.x += y.x, s.y += y.y, s.z += y.z, s.w += y.w;
+        }
+        const int64_t token = (int64_t)sq.k0 + row0 + r;
+        T* out = which == 0 ? static_cast<T*>(a.out1) + token * a.out1_token + (int64_t)head * a.out1_head
+                            : static_cast<T*>(a.out2) + token * a.out2_token + (int64_t)head * a.out2_head;
+        uint2 w;
+        w.x = pack2<T>(s.x * factor, s.y * factor);
+        w.y = pack2<T>(s.z * factor, s.w * factor);
+        *reinterpret_cast<uint2*>(out + c) = w;
+    }
+}
+
+size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
+
+// Queries of one far piece: about what a key tile's own window holds, so that the blocks are alike.
+int far_chunk(const AttentionArgs& a) {
+    const int64_t c = (int64_t)a.window + kRows;
+    return (int)(c < 1024 ? 1024 : c);
+}
+int far_tiles(const AttentionArgs& a) {
+    const int seen = a.sinks < a.total_k ? a.sinks : a.total_k;
+    // no sequence reaches past its window by a whole piece when all keys together do not
+    return a.total_k < far_chunk(a) ? 0 : (seen + kRows - 1) / kRows;
+}
+int far_slots(const AttentionArgs& a) { return a.total_k / far_chunk(a) + 1; }
+
+template <typename T, int DP>
+cudaError_t launch(cudaStream_t s, const AttentionArgs& a, void* buffer) {
+    using S = Smem<DP>;
+    CUtensorMap q_rows, go_rows, k_rows, v_rows, q_tile, go_tile, k_tile, v_tile;
+    if (!head_map(&q_rows, a.q, a.total_q, a.q_heads, a.dim, a.type, kRows) || !head_map(&go_rows, a.d_o, a.total_q, a.q_heads, a.dim, a.type, kRows) ||
+        !head_map(&k_rows, a.k, a.total_k, a.kv_heads, a.dim, a.type, kRows) || !head_map(&v_rows, a.v, a.total_k, a.kv_heads, a.dim, a.type, kRows) ||
+        !head_map(&q_tile, a.q, a.total_q, a.q_heads, a.dim, a.type, kTile) || !head_map(&go_tile, a.d_o, a.total_q, a.q_heads, a.dim, a.type, kTile) ||
+        !head_map(&k_tile, a.k, a.total_k, a.kv_heads, a.dim, a.type, kTile) || !head_map(&v_tile, a.v, a.total_k, a.kv_heads, a.dim, a.type, kTile))
+        return cudaErrorNotSupported;
+    char* b = static_cast<char*>(align_up_256(buffer));
+    float* delta = reinterpret_cast<float*>(b);
+    Params p = {};
+    p.r = Ragged{a.q_offsets, a.k_offsets, a.batch, a.total_q, a.total_k};
+    p.window = a.window, p.sinks = a.sinks, p.q_heads = a.q_heads, p.kv_heads = a.kv_heads, p.group = a.q_heads / a.kv_heads, p.dim = a.dim;
+    p.q_mul = a.q.head != 0, p.k_mul = a.k.head != 0, p.v_mul = a.v.head != 0, p.go_mul = a.d_o.head != 0;
+    p.negate = a.scale < 0.0f ? kNegateA : 0;
+    p.scale = a.scale, p.scale_log2 = fabsf(a.scale) * kLog2e;
+    p.lse = a.lse, p.delta = delta;
+    p.chunk = far_chunk(a), p.far_tiles = far_tiles(a), p.far_slots = p.far_tiles > 0 ? far_slots(a) : 0;
+    p.partial = reinterpret_cast<float*>(b + align256(size_t(a.q_heads) * a.total_q * 4));
+    p.limit = a.wait.limit_cycles, p.fault = a.wait.fault_word;
+    delta_kernel<T><<<(unsigned)(((int64_t)a.total_q * a.q_heads + 15) / 16), 256, 0, s>>>(a, delta);
+    cudaError_t e = cudaGetLastError();
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(window_backward_kernel<T, DP, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kTotal);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(window_backward_kernel<T, DP, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kTotal);
+    if (e != cudaSuccess) return e;
+    Params pk = p;
+    pk.out1 = a.dv.p, pk.out1_token = a.dv.token, pk.out1_head = a.dv.head;
+    pk.out2 = a.dk.p, pk.out2_token = a.dk.token, pk.out2_head = a.dk.head;
+    const int64_t key_blocks = ragged_slots(a.total_k, a.batch, a.k_offsets != nullptr, kRows) + (int64_t)p.far_slots * p.far_tiles;
+    window_backward_kernel<T, DP, true><<<(unsigned)(key_blocks * a.kv_heads), kThreads, S::kTotal, s>>>(k_rows, v_rows, q_tile, go_tile, pk);
+    if (p.far_tiles > 0)
+        window_backward_join_kernel<T, DP><<<(unsigned)((int64_t)p.far_slots * p.far_tiles * a.kv_heads * 2), 256, 0, s>>>(pk);
+    p.out1 = a.dq.p, p.out1_token = a.dq.token, p.out1_head = a.dq.head;
+    p.slots = ragged_slots(a.total_q, a.batch, a.q_offsets != nullptr, kRows);
+    window_backward_kernel<T, DP, false><<<(unsigned)((int64_t)p.slots * a.q_heads), kThreads, S::kTotal, s>>>(q_rows, go_rows, k_tile, v_tile, p);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+size_t window_backward_mma_bytes(const AttentionArgs& a) {
+    const int dp = a.dim <= 64 ? 64 : 128;
+    const int tiles = far_tiles(a);
+    const size_t partial = tiles > 0 ? size_t(2) * far_slots(a) * tiles * a.kv_heads * 2 * kRows * dp * 4 : 0;
+    return align256(size_t(a.q_heads) * a.total_q * 4) + partial + 256;
+}
+
+cudaError_t window_backward_mma(cudaStream_t s, const AttentionArgs& a, void* buffer) {
+    if (a.type == MACA_R_16BF) return a.dim <= 64 ? launch<__nv_bfloat16, 64>(s, a, buffer) : launch<__nv_bfloat16, 128>(s, a, buffer);
+    return a.dim <= 64 ? launch<__half, 64>(s, a, buffer) : launch<__half, 128>(s, a, buffer);
+}
+
+}  // namespace mcsp_b200

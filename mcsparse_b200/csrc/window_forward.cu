@@ -1,0 +1,417 @@
+// Windowed attention forward on the tensor cores (fp16 / bf16, rows of 16-byte multiples).
+//
+// One thread block takes 256 consecutive queries of a sequence and one query head: two tiles of 128 rows that share every
+// key tile of 128. S = Q K^T and O += P V are tcgen05.mma with S, P and O in tensor memory (P overwrites its S, half as
+// wide); the tensor cores work on one tile's products while the other tile's 128 threads, one row each, take the row's
+// maximum, exponentials and sum in registers. Key tiles outside window and first tokens are never loaded; a tile needs its
+// mask only at an edge of the pattern.
+//
+// Bound by the tensor cores and, about equally at headDim 128, by the exponentials (16 per clock and SM): 128 x 128 x 128
+// takes 512 clocks twice and 1024 clocks of exponentials.
+#include <type_traits>
+
+#include "tensor_core.h"
+#include "window_common.h"
+#include "window_maps.h"
+
+namespace mcsp_b200 {
+namespace {
+
+using namespace window;
+using namespace tc;
+
+constexpr int kRows = 128;           // query rows of a tile
+constexpr int kKeys = 128;           // keys of a tile
+constexpr int kSoftmaxThreads = 256;  // two tiles
+constexpr int kThreads = kSoftmaxThreads + 64;  // + the loading warp + the warp that issues the products
+constexpr float kLog2e = 1.4426950408889634f;
+// The running reference of a row's exponentials is only moved when its maximum has grown past it by more than 2^8: until
+// then the weights are at most 256 (exact in fp32 sums, far from fp16's 65504) and O needs no rescaling.
+constexpr float kSlack = 8.0f;
+
+template <int DP>
+struct Smem {
+    static constexpr int kTile = 128 * DP * 2;          // bytes of a 128-row operand
+    static constexpr int kStages = DP == 128 ? 5 : 8;   // key and value tiles in turn
+    static constexpr int kQ = 0;
+    static constexpr int kRing = 2 * kTile;
+    static constexpr int kBars = kRing + kStages * kTile;
+    static constexpr int kTotal = kBars + 256 + 1024;   // the start is aligned to 1024
+};
+
+struct Params {
+    Ragged r;
+    int window, sinks, q_heads, group, dim, total_q, slots;
+    int q_mul, k_mul, v_mul;  // 0: the heads of a tensor share one (a head stride of 0)
+    uint32_t negate;
+    float scale_log2, scale_ln;
+    void* o;
+    int64_t o_token, o_head;
+    float* lse;
+    long long limit;
+    int* fault;
+};
+
+// What one tile of 128 rows has to visit: key tiles [0, first) and [low, high].
+struct Visit {
+    int rows, p_low, first, low, high;
+    __device__ __forceinline__ bool has(int j) const { return j < first || (j >= low && j <= high); }
+};
+__device__ __forceinline__ Visit visit_of(const Sequence& s, int row0, int window, int sinks) {
+    Visit v;
+    v.rows = min(max(s.lq - row0, 0), kRows);
+    v.p_low = s.lk - s.lq + row0;
+    const int p_high = v.p_low + v.rows - 1;
+    if (v.rows == 0 || p_high < 0) {
+        v.first = 0, v.low = 1, v.high = 0;
+        return v;
+    }
+    v.low = max(v.p_low - window + 1, 0) / kKeys;
+    v.high = p_high / kKeys;
+    v.first = min((min(sinks, p_high + 1) + kKeys - 1) / kKeys, v.low);
+    return v;
+}
+
+// The key tiles of a block in the order they are visited: [0, first), then [low, high].
+struct Order {
+    int first, low, n;
+    __device__ __forceinline__ int tile(int i) const { return i < first ? i : low + (i - first); }
+};
+__device__ __forceinline__ Order order_of(const Visit& a, const Visit& b) {
+    Order o;
+    const bool ha = a.low <= a.high, hb = b.low <= b.high;
+    if (!ha && !hb) return Order{0, 0, 0};
+    o.low = ha ? a.low : b.low;
+    if (hb) o.low = min(o.low, b.low);
+    const int high = max(ha ? a.high : -1, hb ? b.high : -1);
+    o.first = min(max(a.first, b.first), o.low);
+    o.n = o.first + (high - o.low + 1);
+    return o;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads, 1)
+    window_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                          const __grid_constant__ CUtensorMap map_v, const Params a) {
+    using S = Smem<DP>;
+    constexpr bool kBf16 = sizeof(T) == 2 && !std::is_same<T, __half>::value;
+    constexpr int kBlocks = DP / 64;  // 64-value column blocks of an operand
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t smem = (smem_u32(smem_raw) + 1023) & ~1023u;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // barriers: Q, full[stages], empty[stages], S ready[2], P ready[2], O ready[2]
+    const uint32_t bars = smem + S::kBars;
+    const uint32_t bar_q = bars, bar_full = bars + 8, bar_empty = bar_full + 8 * S::kStages, bar_s = bar_empty + 8 * S::kStages,
+                   bar_p = bar_s + 16, bar_o = bar_p + 16, slot = bar_o + 16;
+
+    const int head = blockIdx.x % a.q_heads;
+    const int block = a.slots - 1 - (int)(blockIdx.x / a.q_heads);  // the later rows of a sequence have more to do: first
+    const RaggedBlock rb = ragged_block(a.r.q_offsets, a.r.batch, a.r.total_q, block, 2 * kRows, lane);
+    const Sequence sq = rb.b < 0 ? Sequence{0, 0, 0, 0} : sequence_of(a.r, rb.b);
+    if (rb.b < 0 || (int64_t)rb.index * 2 * kRows >= sq.lq) return;  // (the same for the whole block)
+    const int row0 = rb.index * 2 * kRows;
+    const Visit va = visit_of(sq, row0, a.window, a.sinks), vb = visit_of(sq, row0 + kRows, a.window, a.sinks);
+    const Order order = order_of(va, vb);
+
+    if (warp == 9) {
+        tmem_alloc(slot, 512);
+    } else if (threadIdx.x == kSoftmaxThreads) {
+        bar_init(bar_q, 1);
+        for (int i = 0; i < S::kStages; ++i) bar_init(bar_full + 8 * i, 1), bar_init(bar_empty + 8 * i, 1);
+        for (int i = 0; i < 2; ++i) bar_init(bar_s + 8 * i, 1), bar_init(bar_p + 8 * i, kRows), bar_init(bar_o + 8 * i, 1);
+        bar_init_fence();
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    uint32_t tmem;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(slot));
+    // tensor memory: S (and P) of the two tiles, O of the two tiles
+    const uint32_t t_s[2] = {tmem, tmem + 128}, t_o[2] = {tmem + 256, tmem + 256 + DP};
+    bool failed = false;
+
+    if (warp == 8) {
+        // ---- loads
+        if (lane == 0 && order.n > 0) {
+            const int hk = head / a.group;
+            bar_expect(bar_q, 2 * S::kTile);
+            for (int t = 0; t < 2; ++t)
+                for (int c = 0; c < kBlocks; ++c)
+                    tma_load_3d(smem + S::kQ + t * S::kTile + c * (kRows * 128), &map_q, 64 * c, head * a.q_mul,
+                                sq.q0 + row0 + t * kRows, bar_q);
+            int issued = 0;
+            for (int i = 0; i < 2 * order.n; ++i) {
+                const int st = i % S::kStages;
+                if (i >= S::kStages && !bar_wait(bar_empty + 8 * st, (i / S::kStages - 1) & 1, a.limit)) {
+                    failed = true;
+                    break;
+                }
+                bar_expect(bar_full + 8 * st, S::kTile);
+                const int key = sq.k0 + order.tile(i >> 1) * kKeys;
+                for (int c = 0; c < kBlocks; ++c)
+                    tma_load_3d(smem + S::kRing + st * S::kTile + c * (kKeys * 128), (i & 1) ? &map_v : &map_k, 64 * c,
+                                hk * ((i & 1) ? a.v_mul : a.k_mul), key, bar_full + 8 * st);
+                issued = i + 1;
+            }
+            // nothing of this block's memory is given back while a copy is on its way
+            if (failed) {
+                bar_wait(bar_q, 0, a.limit);
+                for (int i = max(0, issued - S::kStages); i < issued; ++i)
+                    bar_wait(bar_full + 8 * (i % S::kStages), (i / S::kStages) & 1, a.limit);
+            }
+        }
+        __syncwarp();
+    } else if (warp == 9) {
+        // ---- products
+        constexpr uint32_t kDescS = mma_desc(kBf16, kKeys, false), kDescO = mma_desc(kBf16, DP, true);
+        const int first_seen = max(va.rows > 0 ? va.p_low - a.window + 1 : 0, 0);
+        const int last_seen = min(sq.lk, sq.lk - sq.lq + min(row0 + 2 * kRows, sq.lq)) - 1;
+        int n_p[2] = {0, 0};  // P tiles taken
+        const int n = order.n;
+        if (n > 0) {
+            failed = !bar_wait_warp(bar_q, 0, a.limit);
+            for (int i = 0; i <= n && !failed; ++i) {
+                const int j = i < n ? order.tile(i) : 0, before = i > 0 ? order.tile(i - 1) : 0;
+                const int st_k = (2 * i) % S::kStages, st_v = (2 * i - 1 + S::kStages) % S::kStages;
+                if (i > 0) {
+                    if (!bar_wait_warp(bar_full + 8 * st_v, ((2 * i - 1) / S::kStages) & 1, a.limit)) {
+                        failed = true;
+                        break;
+                    }
+                    // Values nobody here sees (behind the last query, before the first window) have weight zero, but zero
+                    // times a NaN that lies there would not be zero: such rows are cleared first.
+                    const int key0 = before * kKeys;
+                    const int clear_low = min(max(first_seen - key0, 0), kKeys);
+                    const int clear_high = min(max(last_seen + 1 - key0, 0), kKeys);
+                    const int keep = min(max(a.sinks - key0, 0), kKeys);  // first tokens stay
+                    if (clear_low > keep || clear_high < kKeys) {
+                        for (int x = lane; x < kKeys * 8 * kBlocks; x += 32) {
+                            const int row = (x >> 3) & (kKeys - 1);
+                            if ((row < clear_low && row >= keep) || row >= clear_high)
+                                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(smem + S::kRing + st_v * S::kTile + x * 16),
+                                             "r"(0)
+                                             : "memory");
+                        }
+                        fence_async();
+                        __syncwarp();
+                    }
+                }
+                if (i < n && !bar_wait_warp(bar_full + 8 * st_k, ((2 * i) / S::kStages) & 1, a.limit)) {
+                    failed = true;
+                    break;
+                }
+                for (int t = 0; t < 2; ++t) {
+                    const Visit& v = t == 0 ? va : vb;
+                    if (i > 0 && v.has(before)) {
+                        if (!bar_wait_warp(bar_p + 8 * t, n_p[t] & 1, a.limit)) {
+                            failed = true;
+                            break;
+                        }
+                        fence_after();
+                        if (lane == 0) {
+                            const uint32_t base = smem + S::kRing + st_v * S::kTile;
+#pragma unroll
+                            for (int k = 0; k < kKeys / 16; ++k)
+                                mma_ts(t_o[t], t_s[t] + 8 * k, smem_desc(base + k * 2048, kKeys * 128), kDescO, n_p[t] > 0 || k > 0);
+                            if (before == v.high) mma_commit(bar_o + 8 * t);
+                        }
+                        ++n_p[t];
+                        __syncwarp();
+                    }
+                    if (i < n && v.has(j)) {
+                        if (lane == 0) {
+                            const uint32_t qb = smem + S::kQ + t * S::kTile, kb = smem + S::kRing + st_k * S::kTile;
+#pragma unroll
+                            for (int k = 0; k < DP / 16; ++k) {
+                                const uint32_t off = (k >> 2) * (kRows * 128) + (k & 3) * 32;
+                                mma_ss(t_s[t], smem_desc(qb + off), smem_desc(kb + off), kDescS | a.negate, k > 0);
+                            }
+                            mma_commit(bar_s + 8 * t);
+                        }
+                        __syncwarp();
+                    }
+                }
+                if (lane == 0 && !failed) {
+                    if (i > 0) mma_commit(bar_empty + 8 * st_v);
+                    if (i < n) mma_commit(bar_empty + 8 * st_k);
+                }
+                __syncwarp();
+            }
+        }
+        if (failed && lane == 0) {  // the tensor memory is given back only when no product uses it any more
+            mma_commit(bar_q);
+            bar_wait(bar_q, 1, a.limit);
+        }
+        __syncwarp();
+    } else {
+        // ---- softmax: thread = row
+        const int t = warp >> 2;
+        const Visit v = t == 0 ? va : vb;
+        const int r = threadIdx.x & (kRows - 1);
+        const int p = v.p_low + r;
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // tensor-memory lane of the warp's first row
+        float ref = -INFINITY, sum = 0.0f;
+        int done = 0;
+        for (int i = 0; i < order.n; ++i) {
+            const int j = order.tile(i);
+            if (!v.has(j)) continue;
+            if (!bar_wait_warp(bar_s + 8 * t, done & 1, a.limit)) {
+                failed = true;
+                break;
+            }
+            fence_after();
+            uint32_t s[kKeys];
+#pragma unroll
+            for (int c = 0; c < kKeys; c += 32) tmem_load32(t_s[t] + lanes + c, s + c);
+            wait_loads();
+#pragma unroll
+            for (int c = 0; c < kKeys; c += 32) after_loads32(s + c);
+            const int key0 = j * kKeys;
+            const int last_p = v.p_low + kRows - 1;
+            if (key0 + kKeys - 1 > v.p_low || (key0 <= last_p - a.window && key0 + kKeys > a.sinks)) {
+                // column c is seen iff c <= above and (c > below or c < keep)
+                const int above = p - key0, below = p - key0 - a.window, keep = a.sinks - key0;
+#pragma unroll
+                for (int c = 0; c < kKeys; ++c)
+                    if (!(c <= above && (c > below || c < keep))) s[c] = 0xff800000u;
+            }
+            float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int c = 0; c < kKeys; c += 4)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) top[x] = fmaxf(top[x], __uint_as_float(s[c + x]));
+            const float m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2;
+            const bool move = m > ref + kSlack || (ref == -INFINITY && m > ref);
+            if (__any_sync(0xffffffffu, move)) {
+                const float next = move ? m : ref;
+                const float factor = ref == -INFINITY ? 0.0f : exp2_fast(ref - next);
+                sum *= factor;
+                if (done > 0) {
+#pragma unroll 1
+                    for (int c = 0; c < DP; c += 32) {
+                        uint32_t o[32];
+                        tmem_load32(t_o[t] + lanes + c, o);
+                        wait_loads();
+                        after_loads32(o);
+#pragma unroll
+                        for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * factor);
+                        tmem_store32(t_o[t] + lanes + c, o);
+                    }
+                }
+                ref = next;
+            }
+            const float minus = ref == -INFINITY ? 0.0f : -ref;
+            float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint32_t w[32];
+#pragma unroll
+                for (int c = 0; c < 64; c += 2) {
+                    const float x = exp2_fast(fmaf(__uint_as_float(s[64 * h + c]), a.scale_log2, minus));
+                    const float y = exp2_fast(fmaf(__uint_as_float(s[64 * h + c + 1]), a.scale_log2, minus));
+                    part[c & 2] += x;
+                    part[(c & 2) + 1] += y;
+                    w[c >> 1] = pack2<T>(x, y);
+                }
+                tmem_store32(t_s[t] + lanes + 32 * h, w);
+            }
+            sum += (part[0] + part[1]) + (part[2] + part[3]);
+            wait_stores();
+            fence_before();
+            bar_arrive(bar_p + 8 * t);
+            ++done;
+        }
+        // ---- epilogue
+        if (done > 0 && !failed) {
+            failed = !bar_wait_warp(bar_o + 8 * t, 0, a.limit);
+            fence_after();
+        }
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const int64_t row = (int64_t)sq.q0 + row0 + t * kRows + r;
+        if (a.lse != nullptr && r < v.rows)
+            a.lse[(int64_t)head * a.total_q + row] = sum == 0.0f ? -INFINITY : ref * a.scale_ln + logf(sum);
+        T* out = static_cast<T*>(a.o) + row * a.o_token + (int64_t)head * a.o_head;
+#pragma unroll 1
+        for (int c = 0; c < DP; c += 32) {
+            uint32_t o[32];
+            if (done > 0 && !failed) {
+                tmem_load32(t_o[t] + lanes + c, o);
+                wait_loads();
+                after_loads32(o);
+            }
+            if (r < v.rows && !failed) {
+#pragma unroll
+                for (int x = 0; x < 32; x += 8) {
+                    if (c + x < a.dim) {
+                        uint4 w = make_uint4(0, 0, 0, 0);
+                        if (sum != 0.0f) {
+                            w.x = pack2<T>(__uint_as_float(o[x]) * inv, __uint_as_float(o[x + 1]) * inv);
+                            w.y = pack2<T>(__uint_as_float(o[x + 2]) * inv, __uint_as_float(o[x + 3]) * inv);
+                            w.z = pack2<T>(__uint_as_float(o[x + 4]) * inv, __uint_as_float(o[x + 5]) * inv);
+                            w.w = pack2<T>(__uint_as_float(o[x + 6]) * inv, __uint_as_float(o[x + 7]) * inv);
+                        }
+                        *reinterpret_cast<uint4*>(out + c + x) = w;
+                    }
+                }
+            }
+        }
+        fence_before();
+    }
+    if (failed && a.fault != nullptr) *reinterpret_cast<volatile int*>(a.fault) = 1;
+    __syncthreads();
+    if (warp == 9) {
+        fence_after();
+        tmem_free(tmem, 512);
+    }
+}
+
+template <typename T, int DP>
+cudaError_t launch(cudaStream_t s, const AttentionArgs& a) {
+    using S = Smem<DP>;
+    CUtensorMap mq, mk, mv;
+    if (!head_map(&mq, a.q, a.total_q, a.q_heads, a.dim, a.type, kRows) || !head_map(&mk, a.k, a.total_k, a.kv_heads, a.dim, a.type, kKeys) ||
+        !head_map(&mv, a.v, a.total_k, a.kv_heads, a.dim, a.type, kKeys))
+        return cudaErrorNotSupported;
+    Params p = {};
+    p.r = Ragged{a.q_offsets, a.k_offsets, a.batch, a.total_q, a.total_k};
+    p.window = a.window, p.sinks = a.sinks, p.q_heads = a.q_heads, p.group = a.q_heads / a.kv_heads, p.dim = a.dim;
+    p.total_q = a.total_q;
+    p.slots = ragged_slots(a.total_q, a.batch, a.q_offsets != nullptr, 2 * kRows);
+    p.q_mul = a.q.head != 0, p.k_mul = a.k.head != 0, p.v_mul = a.v.head != 0;
+    p.negate = a.scale < 0.0f ? kNegateA : 0;
+    p.scale_log2 = fabsf(a.scale) * kLog2e, p.scale_ln = 1.0f / kLog2e;
+    p.o = a.o.p, p.o_token = a.o.token, p.o_head = a.o.head, p.lse = a.lse;
+    p.limit = a.wait.limit_cycles, p.fault = a.wait.fault_word;
+    const cudaError_t e = cudaFuncSetAttribute(window_forward_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kTotal);
+    if (e != cudaSuccess) return e;
+    window_forward_kernel<T, DP><<<(unsigned)((int64_t)p.slots * a.q_heads), kThreads, S::kTotal, s>>>(mq, mk, mv, p);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+bool window_tensor_ready(const AttentionTensor& t, int64_t tokens, int heads, int dim) {
+    // TMA: 16-byte rows and strides (a head stride of 0 is read as one head; a token stride of 0 has no such form)
+    return (reinterpret_cast<uintptr_t>(t.p) & 15) == 0 && dim % 8 == 0 && (t.token % 8 == 0 || tokens <= 1) &&
+           (t.head % 8 == 0 || heads <= 1) && (t.token > 0 || tokens <= 1);
+}
+
+cudaError_t window_forward_mma(cudaStream_t s, const AttentionArgs& a) {
+    if (a.type == MACA_R_16BF) return a.dim <= 64 ? launch<__nv_bfloat16, 64>(s, a) : launch<__nv_bfloat16, 128>(s, a);
+    return a.dim <= 64 ? launch<__half, 64>(s, a) : launch<__half, 128>(s, a);
+}
+
+}  // namespace mcsp_b200

@@ -187,17 +187,15 @@ __global__ void __launch_bounds__(32 * kWarps) window_rows_decode_kernel(DecodeA
 
 unsigned row_blocks(int64_t rows) { return (unsigned)((rows + kWarps - 1) / kWarps); }
 
-}  // namespace
-
 template <typename T>
-cudaError_t window_rows(cudaStream_t s, const AttentionArgs& a) {
+cudaError_t rows_forward(cudaStream_t s, const AttentionArgs& a) {
     const Ragged r{a.q_offsets, a.k_offsets, a.batch, a.total_q, a.total_k};
     window_rows_kernel<T><<<row_blocks((int64_t)a.total_q * a.q_heads), 32 * kWarps, 0, s>>>(a, r);
     return cudaGetLastError();
 }
 
 template <typename T>
-cudaError_t window_rows_backward(cudaStream_t s, const AttentionArgs& a) {
+cudaError_t rows_backward(cudaStream_t s, const AttentionArgs& a) {
     const Ragged r{a.q_offsets, a.k_offsets, a.batch, a.total_q, a.total_k};
     if (a.total_q > 0) window_rows_dq_kernel<T><<<row_blocks((int64_t)a.total_q * a.q_heads), 32 * kWarps, 0, s>>>(a, r);
     if (a.total_k > 0) window_rows_dkv_kernel<T><<<row_blocks((int64_t)a.total_k * a.kv_heads), 32 * kWarps, 0, s>>>(a, r);
@@ -205,39 +203,26 @@ cudaError_t window_rows_backward(cudaStream_t s, const AttentionArgs& a) {
 }
 
 template <typename T>
-cudaError_t window_rows_decode(cudaStream_t s, const DecodeArgs& a) {
+cudaError_t rows_decode(cudaStream_t s, const DecodeArgs& a) {
     window_rows_decode_kernel<T><<<(unsigned)((int64_t)a.batch * a.q_heads), 32 * kWarps, 0, s>>>(a);
     return cudaGetLastError();
 }
 
+}  // namespace
+
 // The type switch.
-#define MCSP_BY_TYPE(call)                                   \
-    do {                                                     \
-        switch (a.type) {                                    \
-            case MACA_R_32F: return call<float>(s, a);       \
-            case MACA_R_16F: return call<__half>(s, a);      \
+#define MCSP_BY_TYPE(call)                                      \
+    do {                                                        \
+        switch (a.type) {                                       \
+            case MACA_R_32F: return call<float>(s, a);          \
+            case MACA_R_16F: return call<__half>(s, a);         \
             case MACA_R_16BF: return call<__nv_bfloat16>(s, a); \
-            default: return cudaErrorInvalidValue;           \
-        }                                                    \
+            default: return cudaErrorInvalidValue;              \
+        }                                                       \
     } while (0)
 
-cudaError_t window_attention(cudaStream_t s, const AttentionArgs& a) {
-    if (a.total_q == 0 || a.batch == 0) return cudaSuccess;
-    MCSP_BY_TYPE(window_rows);
-}
-
-size_t window_attention_backward_bytes(const AttentionArgs&) { return 256; }
-
-cudaError_t window_attention_backward(cudaStream_t s, const AttentionArgs& a, void*) {
-    if (a.batch == 0) return cudaSuccess;
-    MCSP_BY_TYPE(window_rows_backward);
-}
-
-size_t window_attention_decode_bytes(const DecodeArgs&) { return 256; }
-
-cudaError_t window_attention_decode(cudaStream_t s, const DecodeArgs& a, void*) {
-    if (a.batch == 0) return cudaSuccess;
-    MCSP_BY_TYPE(window_rows_decode);
-}
+cudaError_t window_rows_forward(cudaStream_t s, const AttentionArgs& a) { MCSP_BY_TYPE(rows_forward); }
+cudaError_t window_rows_backward(cudaStream_t s, const AttentionArgs& a) { MCSP_BY_TYPE(rows_backward); }
+cudaError_t window_rows_decode(cudaStream_t s, const DecodeArgs& a) { MCSP_BY_TYPE(rows_decode); }
 
 }  // namespace mcsp_b200
