@@ -421,6 +421,10 @@ bool window_tensor_ready(const AttentionTensor& t, int64_t tokens, int heads, in
 cudaError_t window_forward_mma(cudaStream_t s, const AttentionArgs& a);
 size_t window_backward_mma_bytes(const AttentionArgs& a);
 cudaError_t window_backward_mma(cudaStream_t s, const AttentionArgs& a, void* buffer);
+// Warp-level products over a streamed cache (window_decode.cu).
+bool window_decode_ready(const DecodeArgs& a);
+size_t window_decode_mma_bytes(const DecodeArgs& a);
+cudaError_t window_decode_mma(cudaStream_t s, const DecodeArgs& a, void* buffer);
 // The choice between them (window_attention.cpp).
 cudaError_t window_attention(cudaStream_t s, const AttentionArgs& a);
 size_t window_attention_backward_bytes(const AttentionArgs& a);

@@ -71,11 +71,11 @@ cudaError_t window_attention_backward(cudaStream_t s, const AttentionArgs& a, vo
     return window_rows_backward(s, a);
 }
 
-size_t window_attention_decode_bytes(const DecodeArgs&) { return 256; }
+size_t window_attention_decode_bytes(const DecodeArgs& a) { return a.type != MACA_R_32F ? window_decode_mma_bytes(a) : 256; }
 
-cudaError_t window_attention_decode(cudaStream_t s, const DecodeArgs& a, void*) {
+cudaError_t window_attention_decode(cudaStream_t s, const DecodeArgs& a, void* buffer) {
     if (a.batch == 0) return cudaSuccess;
-    return window_rows_decode(s, a);
+    return window_decode_ready(a) ? window_decode_mma(s, a, buffer) : window_rows_decode(s, a);
 }
 
 }  // namespace mcsp_b200
