@@ -61,7 +61,7 @@ _CSRMM = [_vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _
 
 
 class Heads(C.Structure):
-    """mcsparseB200Heads_t: a tokens x heads x head-dim tensor, strides in elements."""
+    """mcsparseB200Heads_t: a tokens x heads x head-dim tensor, strides in elements (passed by address)."""
     _fields_ = [("values", _vp), ("tokenStride", _i64), ("headStride", _i64)]
 
 
@@ -70,7 +70,6 @@ class Cache(C.Structure):
     _fields_ = [("values", _vp), ("pageStride", _i64), ("tokenStride", _i64), ("headStride", _i64)]
 
 
-_ph, _pc = C.POINTER(Heads), C.POINTER(Cache)
 PROTOTYPES = {
     "mcsparseCreate": (_i, [_pvp]),
     "mcsparseDestroy": (_i, [_vp]),
@@ -165,12 +164,12 @@ PROTOTYPES = {
     "mcsparseB200EmbeddingGradient": (_i, [_vp, _vp, _i64, _vp, _i, _i, _vp, _vp, _vp, _vp]),
     "mcsparseB200CreateWindow": (_i, [_pvp, _i64, _i64, _i, _i, _i, C.c_float, _i]),
     "mcsparseB200DestroyWindow": (_i, [_vp]),
-    "mcsparseB200WindowAttention": (_i, [_vp, _vp, _i64, _vp, _vp, _i64, _i64, _ph, _ph, _ph, _ph, _vp]),
+    "mcsparseB200WindowAttention": (_i, [_vp, _vp, _i64, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp]),
     "mcsparseB200WindowAttentionBackward_bufferSize": (_i, [_vp, _vp, _i64, _i64, _i64, _psz]),
-    "mcsparseB200WindowAttentionBackward": (_i, [_vp, _vp, _i64, _vp, _vp, _i64, _i64, _ph, _ph, _ph, _ph, _vp,
-                                                 _ph, _ph, _ph, _ph, _vp]),
+    "mcsparseB200WindowAttentionBackward": (_i, [_vp, _vp, _i64, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp,
+                                                 _vp, _vp, _vp, _vp, _vp]),
     "mcsparseB200WindowAttentionDecode_bufferSize": (_i, [_vp, _vp, _i64, _i64, _i64, _psz]),
-    "mcsparseB200WindowAttentionDecode": (_i, [_vp, _vp, _i64, _vp, _ph, _pc, _pc, _i64, _i64, _vp, _i64, _ph, _vp, _vp]),
+    "mcsparseB200WindowAttentionDecode": (_i, [_vp, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _vp, _vp, _vp]),
 }
 
 

@@ -12,76 +12,70 @@ import torch
 
 from . import capi
 from .capi import check, lib
-from .host import _DTYPE, _ptr, _scalar
+from .host import _DTYPE
+
+_INDEX = {torch.int32: capi.MCSPARSE_INDEX_32I, torch.int64: capi.MCSPARSE_INDEX_64I}
+# Several mcsparseB200Heads_t / mcsparseB200Cache_t side by side: one allocation per call, addressed by its parts.
+_Tensors4, _Tensors8 = C.c_int64 * 12, C.c_int64 * 24
+_Decode = C.c_int64 * 14
+_HEADS = C.sizeof(capi.Heads)
+_CACHE = C.sizeof(capi.Cache)
 
 
-def _index_type(indices):
-    if indices.dtype == torch.int64:
-        return capi.MCSPARSE_INDEX_64I
-    if indices.dtype == torch.int32:
-        return capi.MCSPARSE_INDEX_32I
-    raise ValueError(f"indices must be int32 or int64, got {indices.dtype}")
-
-
-def _float_scalar(handle, value):
+def _scalar(handle, value):
     """A float as a C argument: a host scalar, or a one-element fp32 device tensor in device pointer mode."""
     if handle.pointer_mode == capi.MCSPARSE_POINTER_MODE_DEVICE:
         if not (isinstance(value, torch.Tensor) and value.dtype == torch.float32 and value.numel() == 1 and value.is_cuda):
             raise ValueError("device pointer mode: alpha and beta are one-element float32 device tensors")
-        return _ptr(value), value
-    v = _scalar(value, torch.float32)
-    return C.cast(C.byref(v), C.c_void_p), v
+        return value.data_ptr()
+    return C.byref(C.c_float(value))
 
 
-def _same_device(handle, *tensors):
-    device = handle.stream.device
+def _on_device(handle, *tensors):
+    device = handle.stream.device_index
     for t in tensors:
-        if t is not None and t.device != device:
-            raise ValueError(f"tensor on {t.device}, handle on {device}")
+        if t.get_device() != device:
+            raise ValueError(f"tensor on {t.device}, handle on device {device}")
 
 
 def _indices(handle, indices):
-    _same_device(handle, indices)
-    if indices.dim() != 1 or not (indices.is_contiguous() or indices.numel() <= 1):
+    kind = _INDEX.get(indices.dtype)
+    if kind is None:
+        raise ValueError(f"indices must be int32 or int64, got {indices.dtype}")
+    if indices.dim() != 1 or not indices.is_contiguous():
         raise ValueError("indices must be one contiguous row")
-    return _index_type(indices)
+    return kind
 
 
 def embedding_lookup(handle, indices, E, Y, alpha=1.0, base=0):
     """Y[t] = alpha * E[indices[t] - base]; a row of zeros for an index outside the table. E, Y: ``DnMat`` in row order."""
     kind = _indices(handle, indices)
-    _same_device(handle, E.values, Y.values)
-    pa, keep = _float_scalar(handle, alpha)
-    check(lib.mcsparseB200EmbeddingLookup(handle.h, pa, indices.numel(), _ptr(indices), kind, base, E.d, Y.d),
+    _on_device(handle, indices, E.values, Y.values)
+    check(lib.mcsparseB200EmbeddingLookup(handle.h, _scalar(handle, alpha), indices.numel(), indices.data_ptr(), kind, base, E.d, Y.d),
           "mcsparseB200EmbeddingLookup")
-    del keep
 
 
 def embedding_gradient_buffer_size(handle, indices, dY, dE):
     size = C.c_size_t()
-    check(lib.mcsparseB200EmbeddingGradient_bufferSize(handle.h, indices.numel(), _index_type(indices), dY.d, dE.d,
+    check(lib.mcsparseB200EmbeddingGradient_bufferSize(handle.h, indices.numel(), _indices(handle, indices), dY.d, dE.d,
                                                        C.byref(size)), "mcsparseB200EmbeddingGradient_bufferSize")
     return size.value
 
 
-def _buffer(handle, buffer, need):
-    """The caller's work buffer, checked: its device, type and size."""
-    _same_device(handle, buffer)
-    if buffer.dtype != torch.uint8 or not buffer.is_contiguous() or buffer.numel() < need:
+def _buffer(buffer, need):
+    """Address of the caller's work buffer, once it is large enough."""
+    if buffer is None or buffer.dtype != torch.uint8 or not buffer.is_contiguous() or buffer.numel() < need:
         raise ValueError(f"the work buffer must be {need} contiguous bytes (uint8) or more")
-    return _ptr(buffer)
+    return buffer.data_ptr()
 
 
 def embedding_gradient(handle, indices, dY, dE, buffer, alpha=1.0, beta=0.0, base=0):
     """dE = alpha * S^T dY + beta * dE, S the 0/1 matrix of the indices. Indices outside the table contribute nothing."""
-    kind = _indices(handle, indices)
-    _same_device(handle, dY.values, dE.values)
-    work = _buffer(handle, buffer, embedding_gradient_buffer_size(handle, indices, dY, dE))
-    pa, keep_a = _float_scalar(handle, alpha)
-    pb, keep_b = _float_scalar(handle, beta)
-    check(lib.mcsparseB200EmbeddingGradient(handle.h, pa, indices.numel(), _ptr(indices), kind, base, dY.d, pb, dE.d, work),
+    need = embedding_gradient_buffer_size(handle, indices, dY, dE)
+    _on_device(handle, indices, dY.values, dE.values, buffer)
+    check(lib.mcsparseB200EmbeddingGradient(handle.h, _scalar(handle, alpha), indices.numel(), indices.data_ptr(), _INDEX[indices.dtype],
+                                            base, dY.d, _scalar(handle, beta), dE.d, _buffer(buffer, need)),
           "mcsparseB200EmbeddingGradient")
-    del keep_a, keep_b
 
 
 class Window:
@@ -95,6 +89,7 @@ class Window:
         self.dtype = dtype
         self.scale = 1.0 / math.sqrt(head_dim) if scale is None and head_dim > 0 else float(scale or 0.0)
         self.d = None
+        self._sizes = {}  # buffer sizes asked for so far
         if dtype not in _DTYPE:
             raise ValueError(f"no value type for {dtype}")
         d = C.c_void_p()
@@ -107,46 +102,52 @@ class Window:
             lib.mcsparseB200DestroyWindow(self.d)
             self.d = None
 
+    def _size(self, handle, name, *sizes):
+        """What the library's `name` call reports for these sizes."""
+        key = (handle.stream.device_index, name, *sizes)
+        need = self._sizes.get(key)
+        if need is None:
+            size = C.c_size_t()
+            check(getattr(lib, name)(handle.h, self.d, *sizes, C.byref(size)), name)
+            if len(self._sizes) >= 1024:
+                self._sizes.clear()
+            need = self._sizes[key] = size.value
+        return need
 
-def _heads(handle, t, tokens, heads, window, what):
-    """mcsparseB200Heads_t of a tokens x heads x head_dim tensor with consecutive values in its last dimension."""
-    _same_device(handle, t)
-    if t.dtype != window.dtype or tuple(t.shape) != (tokens, heads, window.head_dim):
-        raise ValueError(f"{what}: {t.dtype} {tuple(t.shape)}, expected {window.dtype} {(tokens, heads, window.head_dim)}")
-    if window.head_dim > 1 and t.stride(2) != 1:
+
+def _heads(device, t, tokens, heads, window, what):
+    """Address and strides of a tokens x heads x head_dim tensor with consecutive values in its last dimension."""
+    if t.dtype is not window.dtype or t.shape != (tokens, heads, window.head_dim) or t.get_device() != device:
+        raise ValueError(f"{what}: {t.dtype} {tuple(t.shape)} on {t.device}, expected {window.dtype} "
+                         f"{(tokens, heads, window.head_dim)} on the handle's device")
+    stride = t.stride()
+    if stride[2] != 1 and window.head_dim > 1:
         raise ValueError(f"{what}: the last dimension must be consecutive")
-    return capi.Heads(_ptr(t).value, t.stride(0), t.stride(1))
+    return t.data_ptr(), stride[0], stride[1]
 
 
-def _offsets(handle, offsets, what):
-    if offsets is None:
-        return None
-    _same_device(handle, offsets)
-    if offsets.dtype != torch.int32 or offsets.dim() != 1 or offsets.numel() < 1 or not offsets.is_contiguous():
-        raise ValueError(f"{what} must be a contiguous int32 row of sequences + 1 offsets")
-    return offsets
-
-
-def _batch(handle, q_offsets, k_offsets):
-    q_offsets, k_offsets = _offsets(handle, q_offsets, "q_offsets"), _offsets(handle, k_offsets, "k_offsets")
+def _offsets(device, q_offsets, k_offsets):
+    """Sequences, and the addresses of their offsets."""
+    if q_offsets is None:
+        if k_offsets is not None:
+            raise ValueError("k_offsets without q_offsets")
+        return 1, None, None
     if k_offsets is None:
         k_offsets = q_offsets
-    if q_offsets is None and k_offsets is not None:
-        raise ValueError("k_offsets without q_offsets")
-    if q_offsets is None:
-        return 1, None, None
-    if q_offsets.numel() != k_offsets.numel():
+    for t in (q_offsets, k_offsets):
+        if t.dtype is not torch.int32 or t.dim() != 1 or t.shape[0] < 1 or not t.is_contiguous() or t.get_device() != device:
+            raise ValueError("offsets must be a contiguous int32 row of sequences + 1 entries on the handle's device")
+    if q_offsets.shape != k_offsets.shape:
         raise ValueError("q_offsets and k_offsets must describe the same number of sequences")
-    return q_offsets.numel() - 1, _ptr(q_offsets), _ptr(k_offsets)
+    return q_offsets.shape[0] - 1, q_offsets.data_ptr(), k_offsets.data_ptr()
 
 
-def _lse(handle, lse, shape):
+def _lse(device, lse, shape):
     if lse is None:
         return None
-    _same_device(handle, lse)
-    if lse.dtype != torch.float32 or tuple(lse.shape) != shape or not lse.is_contiguous():
-        raise ValueError(f"lse must be a contiguous float32 tensor of {shape}")
-    return _ptr(lse)
+    if lse.dtype is not torch.float32 or lse.shape != shape or not lse.is_contiguous() or lse.get_device() != device:
+        raise ValueError(f"lse must be a contiguous float32 tensor of {shape} on the handle's device")
+    return lse.data_ptr()
 
 
 def window_attention(handle, window, q, k, v, out, lse=None, q_offsets=None, k_offsets=None):
@@ -154,53 +155,54 @@ def window_attention(handle, window, q, k, v, out, lse=None, q_offsets=None, k_o
 
     q, out: queries x q_heads x head_dim; k, v: keys x kv_heads x head_dim, any token and head strides. q_offsets,
     k_offsets: int32 offsets of the sequences (k_offsets defaults to q_offsets; neither: one sequence). lse: q_heads x queries."""
-    batch, qo, ko = _batch(handle, q_offsets, k_offsets)
-    tq, tk = q.shape[0], k.shape[0]
-    tensors = [_heads(handle, t, n, h, window, name) for t, n, h, name in (
-        (q, tq, window.q_heads, "q"), (k, tk, window.kv_heads, "k"), (v, tk, window.kv_heads, "v"), (out, tq, window.q_heads, "out"))]
-    check(lib.mcsparseB200WindowAttention(handle.h, window.d, batch, qo, ko, tq, tk, *(C.byref(t) for t in tensors),
-                                          _lse(handle, lse, (window.q_heads, tq))), "mcsparseB200WindowAttention")
+    device = handle.stream.device_index
+    tq, tk, hq, hk = q.shape[0], k.shape[0], window.q_heads, window.kv_heads
+    t = _Tensors4(*_heads(device, q, tq, hq, window, "q"), *_heads(device, k, tk, hk, window, "k"),
+                  *_heads(device, v, tk, hk, window, "v"), *_heads(device, out, tq, hq, window, "out"))
+    batch, qo, ko = _offsets(device, q_offsets, k_offsets)
+    p = C.addressof(t)
+    check(lib.mcsparseB200WindowAttention(handle.h, window.d, batch, qo, ko, tq, tk, p, p + _HEADS, p + 2 * _HEADS, p + 3 * _HEADS,
+                                          _lse(device, lse, (hq, tq))), "mcsparseB200WindowAttention")
 
 
 def window_attention_backward_buffer_size(handle, window, batch, total_q, total_k):
-    size = C.c_size_t()
-    check(lib.mcsparseB200WindowAttentionBackward_bufferSize(handle.h, window.d, batch, total_q, total_k, C.byref(size)),
-          "mcsparseB200WindowAttentionBackward_bufferSize")
-    return size.value
+    return window._size(handle, "mcsparseB200WindowAttentionBackward_bufferSize", batch, total_q, total_k)
 
 
 def window_attention_backward(handle, window, q, k, v, out, lse, dout, dq, dk, dv, buffer, q_offsets=None, k_offsets=None):
     """Gradients dq, dk, dv of :func:`window_attention`; ``out`` and ``lse`` are what it wrote."""
-    batch, qo, ko = _batch(handle, q_offsets, k_offsets)
-    tq, tk = q.shape[0], k.shape[0]
-    hq, hk = window.q_heads, window.kv_heads
-    t = [_heads(handle, x, n, h, window, name) for x, n, h, name in (
-        (q, tq, hq, "q"), (k, tk, hk, "k"), (v, tk, hk, "v"), (out, tq, hq, "out"), (dout, tq, hq, "dout"), (dq, tq, hq, "dq"),
-        (dk, tk, hk, "dk"), (dv, tk, hk, "dv"))]
+    device = handle.stream.device_index
+    tq, tk, hq, hk = q.shape[0], k.shape[0], window.q_heads, window.kv_heads
+    t = _Tensors8(*_heads(device, q, tq, hq, window, "q"), *_heads(device, k, tk, hk, window, "k"),
+                  *_heads(device, v, tk, hk, window, "v"), *_heads(device, out, tq, hq, window, "out"),
+                  *_heads(device, dout, tq, hq, window, "dout"), *_heads(device, dq, tq, hq, window, "dq"),
+                  *_heads(device, dk, tk, hk, window, "dk"), *_heads(device, dv, tk, hk, window, "dv"))
+    batch, qo, ko = _offsets(device, q_offsets, k_offsets)
     if lse is None:
         raise ValueError("the backward pass needs lse")
-    p = [C.byref(x) for x in t]
-    work = _buffer(handle, buffer, window_attention_backward_buffer_size(handle, window, batch, tq, tk))
-    check(lib.mcsparseB200WindowAttentionBackward(handle.h, window.d, batch, qo, ko, tq, tk, *p[:4], _lse(handle, lse, (hq, tq)),
-                                                  *p[4:], work), "mcsparseB200WindowAttentionBackward")
+    work = _buffer(buffer, window_attention_backward_buffer_size(handle, window, batch, tq, tk))
+    _on_device(handle, buffer)
+    p = C.addressof(t)
+    check(lib.mcsparseB200WindowAttentionBackward(
+        handle.h, window.d, batch, qo, ko, tq, tk, p, p + _HEADS, p + 2 * _HEADS, p + 3 * _HEADS, _lse(device, lse, (hq, tq)),
+        p + 4 * _HEADS, p + 5 * _HEADS, p + 6 * _HEADS, p + 7 * _HEADS, work), "mcsparseB200WindowAttentionBackward")
 
 
 def window_attention_decode_buffer_size(handle, window, batch, max_pages, page_size=1):
     """Bytes for sequences of at most max_pages * page_size tokens."""
-    size = C.c_size_t()
-    check(lib.mcsparseB200WindowAttentionDecode_bufferSize(handle.h, window.d, batch, max_pages, page_size, C.byref(size)),
-          "mcsparseB200WindowAttentionDecode_bufferSize")
-    return size.value
+    return window._size(handle, "mcsparseB200WindowAttentionDecode_bufferSize", batch, max_pages, page_size)
 
 
-def _cache(handle, t, window, what):
-    _same_device(handle, t)
-    if t.dtype != window.dtype or t.dim() != 4 or tuple(t.shape[2:]) != (window.kv_heads, window.head_dim):
-        raise ValueError(f"{what}: {t.dtype} {tuple(t.shape)}, expected {window.dtype} (pages, page size, "
-                         f"{window.kv_heads}, {window.head_dim})")
-    if window.head_dim > 1 and t.stride(3) != 1:
+def _cache(device, t, window, what):
+    shape = t.shape
+    if (t.dtype is not window.dtype or len(shape) != 4 or shape[2] != window.kv_heads or shape[3] != window.head_dim
+            or t.get_device() != device):
+        raise ValueError(f"{what}: {t.dtype} {tuple(shape)} on {t.device}, expected {window.dtype} (pages, page size, "
+                         f"{window.kv_heads}, {window.head_dim}) on the handle's device")
+    stride = t.stride()
+    if stride[3] != 1 and window.head_dim > 1:
         raise ValueError(f"{what}: the last dimension must be consecutive")
-    return capi.Cache(_ptr(t).value, t.stride(0), t.stride(1), t.stride(2))
+    return t.data_ptr(), stride[0], stride[1], stride[2]
 
 
 def window_attention_decode(handle, window, q, k_cache, v_cache, lengths, out, lse=None, buffer=None, page_table=None):
@@ -208,27 +210,27 @@ def window_attention_decode(handle, window, q, k_cache, v_cache, lengths, out, l
 
     q, out: batch x q_heads x head_dim; k_cache, v_cache: pages x page size x kv_heads x head_dim; page_table: int32,
     batch x pages of a sequence (None: page b is all of sequence b); lse: batch x q_heads."""
-    batch = q.shape[0]
-    tq = [_heads(handle, t, batch, window.q_heads, window, name) for t, name in ((q, "q"), (out, "out"))]
-    kc, vc = _cache(handle, k_cache, window, "k_cache"), _cache(handle, v_cache, window, "v_cache")
-    if k_cache.shape[:2] != v_cache.shape[:2]:
-        raise ValueError("k_cache and v_cache must hold the same pages")
+    device = handle.stream.device_index
+    batch, hq = q.shape[0], window.q_heads
+    t = _Decode(*_heads(device, q, batch, hq, window, "q"), *_heads(device, out, batch, hq, window, "out"),
+                *_cache(device, k_cache, window, "k_cache"), *_cache(device, v_cache, window, "v_cache"))
     pages, page_size = k_cache.shape[:2]
-    _same_device(handle, lengths, page_table)
-    if lengths.dtype != torch.int32 or tuple(lengths.shape) != (batch,) or not lengths.is_contiguous():
-        raise ValueError("lengths must be a contiguous int32 row, one per sequence")
+    if v_cache.shape != k_cache.shape:
+        raise ValueError("k_cache and v_cache must hold the same pages")
+    if lengths.dtype is not torch.int32 or lengths.shape != (batch,) or not lengths.is_contiguous() or lengths.get_device() != device:
+        raise ValueError("lengths must be a contiguous int32 row on the handle's device, one per sequence")
     if page_table is None:
-        max_pages = 1
+        table, max_pages = None, 1
         if pages < batch:
             raise ValueError("without a page table the cache holds a page for every sequence")
     else:
-        if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != batch or not page_table.is_contiguous():
-            raise ValueError("page_table must be a contiguous int32 tensor of batch x pages")
-        max_pages = page_table.shape[1]
-    if buffer is None:
-        raise ValueError("a work buffer is needed (window_attention_decode_buffer_size)")
-    work = _buffer(handle, buffer, window_attention_decode_buffer_size(handle, window, batch, max_pages, page_size))
-    check(lib.mcsparseB200WindowAttentionDecode(handle.h, window.d, batch, _ptr(lengths), C.byref(tq[0]), C.byref(kc), C.byref(vc),
-                                                pages, page_size, None if page_table is None else _ptr(page_table), max_pages,
-                                                C.byref(tq[1]), _lse(handle, lse, (batch, window.q_heads)), work),
+        if (page_table.dtype is not torch.int32 or page_table.dim() != 2 or page_table.shape[0] != batch or not page_table.is_contiguous()
+                or page_table.get_device() != device):
+            raise ValueError("page_table must be a contiguous int32 tensor of batch x pages on the handle's device")
+        table, max_pages = page_table.data_ptr(), page_table.shape[1]
+    work = _buffer(buffer, window_attention_decode_buffer_size(handle, window, batch, max_pages, page_size))
+    _on_device(handle, buffer)
+    p = C.addressof(t)
+    check(lib.mcsparseB200WindowAttentionDecode(handle.h, window.d, batch, lengths.data_ptr(), p, p + 2 * _HEADS, p + 2 * _HEADS + _CACHE,
+                                                pages, page_size, table, max_pages, p + _HEADS, _lse(device, lse, (batch, hq)), work),
           "mcsparseB200WindowAttentionDecode")

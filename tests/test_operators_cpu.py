@@ -18,7 +18,7 @@ class Stub:
     pointer_mode = capi.MCSPARSE_POINTER_MODE_HOST
 
     class stream:
-        device = torch.device("cpu")
+        device_index = -1  # what a CPU tensor reports
 
 
 def test_window_descriptor():
