@@ -375,6 +375,7 @@ struct EmbeddingArgs {
     int64_t ld_tokens = 0;
     macaDataType token_type = MACA_R_32F;
     ScalarArg<float> alpha{1.0f, nullptr}, beta{0.0f, nullptr};
+    int sm_count = 148;
 };
 cudaError_t embedding_lookup(cudaStream_t s, const EmbeddingArgs& a);
 size_t embedding_gradient_bytes(int64_t count, int64_t rows, int64_t width);

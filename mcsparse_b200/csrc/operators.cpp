@@ -184,6 +184,7 @@ mcsparseStatus_t mcsparseB200EmbeddingGradient(mcsparseHandle_t handle, const vo
     EmbeddingArgs a = embedding_args(count, indices, indexType, idxBase, matDE, matDY);
     a.alpha = scalar(handle, alpha);
     a.beta = scalar(handle, beta);
+    if (handle->sm_count > 0) a.sm_count = handle->sm_count;
     return pub(from_cuda(embedding_gradient(handle->stream, a, externalBuffer)));
 }
 
