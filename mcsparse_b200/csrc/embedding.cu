@@ -4,16 +4,17 @@
 // Lookup: one pass; a warp moves a piece of one row with 16-byte loads and stores. Bound by memory (count * width read,
 // unless rows repeat, and written).
 //
-// Gradient, three launches:
+// Gradient, four launches, each prepared while the one before it runs (programmatic dependent launch):
 //   1. S^T in CSR form is the tokens sorted by id: a stable radix sort of (id, position) pairs. Up to 131072 tokens one cluster
 //      of 8 thread blocks sorts them in two passes or three (ids below 2^18: two 9-bit digits), its digit counts exchanged over
-//      distributed shared memory, its barriers the cluster's; more tokens take the multi-launch sort of transpose.cu. The
-//      other blocks of the launch meanwhile write the rows no token names (beta = 0: zeros, most of the traffic of a large
-//      table); each finds them by marking the ids of its own range of rows in shared memory, so it need not wait for the sort.
-//   2. The sorted tokens are cut into chunks of equal size whatever the ids are, so a token that fills half the batch costs no
+//      distributed shared memory, its barriers the cluster's; more tokens take the multi-launch sort of transpose.cu.
+//   2. Beside the sort, the rows no token names are written (beta = 0: zeros, most of the traffic of a large table). A block
+//      finds those of its rows by marking the ids that are its own in shared memory, so it need not wait for the sort. (As
+//      further blocks of the sort's own launch they came up in clusters of 8, 16 of which the GPU holds: 116 us against 65.)
+//   3. The sorted tokens are cut into chunks of equal size whatever the ids are, so a token that fills half the batch costs no
 //      more than any other; a warp owns one chunk and a slab of columns, adds in fp32 and writes every sum that lies inside
 //      its chunk. A sum that crosses chunks is left as one partial per chunk.
-//   3. Those partials are put together in chunk order.
+//   4. Those partials are put together in chunk order.
 // No atomics: the order of every addition follows from ids and sizes. Bound by memory: count * width read, rows * width written.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -40,13 +41,37 @@ __device__ __forceinline__ __half from_float<__half>(float v) { return __float2h
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// V consecutive values, moved with the widest accesses their size allows (16 bytes).
+// V consecutive values of one thread, moved in one access of up to 32 bytes.
 template <typename T, int V>
-struct alignas(sizeof(T) * V >= 16 ? 16 : sizeof(T) * V) Pack {
+struct alignas(sizeof(T) * V) Pack {
     T v[V];
 };
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> load_pack(const T* p) {
+    Pack<T, V> r;
+    if constexpr (sizeof(r) == 32) {
+        float* f = reinterpret_cast<float*>(&r);
+        asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3]), "=f"(f[4]), "=f"(f[5]), "=f"(f[6]), "=f"(f[7])
+                     : "l"(p));
+    } else {
+        r = *reinterpret_cast<const Pack<T, V>*>(p);
+    }
+    return r;
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_pack(T* p, const Pack<T, V>& r) {
+    if constexpr (sizeof(r) == 32) {
+        const float* f = reinterpret_cast<const float*>(&r);
+        asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]),
+                     "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7])
+                     : "memory");
+    } else {
+        *reinterpret_cast<Pack<T, V>*>(p) = r;
+    }
+}
 
-// How a thread holds its columns: V consecutive ones when every row starts on a 16-byte boundary and the width is a
+// How a thread holds its columns: V consecutive ones when every row starts on a boundary of V values and the width is a
 // multiple of V; otherwise kLoose single columns, 32 apart, so that a warp's accesses stay together.
 constexpr int kLoose = 4;
 template <int V>
@@ -61,7 +86,7 @@ __device__ __forceinline__ void load_columns(const T* row, int64_t first, int64_
     if (V > 1) {
         const int64_t c = first + lane * V;
         if (c < width) {
-            const Pack<T, V> p = *reinterpret_cast<const Pack<T, V>*>(row + c);
+            const Pack<T, V> p = load_pack<T, V>(row + c);
 #pragma unroll
             for (int i = 0; i < V; ++i) out[i] = to_float(p.v[i]);
         }
@@ -82,7 +107,7 @@ __device__ __forceinline__ void store_columns(T* row, int64_t first, int64_t wid
             Pack<T, V> p;
 #pragma unroll
             for (int i = 0; i < V; ++i) p.v[i] = from_float<T>(in[i]);
-            *reinterpret_cast<Pack<T, V>*>(row + c) = p;
+            store_pack<T, V>(row + c, p);
         }
     } else {
 #pragma unroll
@@ -135,12 +160,78 @@ __global__ void __launch_bounds__(256)
 
 // ----------------------------------------------------------------------------- gradient
 
+// Waits until the launch before this one in the stream is done and its writes are seen (programmatic dependent launch).
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// Lets the next launch's blocks come up early; they wait in grid_wait().
+__device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// The rows of a warp's chunk on their way. Vectors: a ring of asynchronous copies in shared memory, a thread reads back what it
+// copied itself; the copies of 16 (8) rows are in flight whatever the warp is doing. (Loads into registers, as many ahead,
+// waited for the newest of them at every row: 52 us against 25 for 16384 rows of 2048 bf16 values.)
+template <typename T, int V>
+struct Rows {
+    static constexpr int kBytes = sizeof(Pack<T, V>);      // 16 or 32, per thread and row
+    static constexpr int kAhead = kBytes == 16 ? 16 : 8, kGroup = 4;
+    static constexpr int kShared = kAhead * kBytes * 256;  // of a block
+    uint32_t ring;
+    const T* from;
+    int64_t ld;
+    bool inside;
+    __device__ __forceinline__ Rows(uint8_t* smem, const T* dy, int64_t ld_y, int64_t first, int64_t width, int lane)
+        : ring(static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + threadIdx.x * 16), from(dy + first + lane * V), ld(ld_y),
+          inside(first + lane * V < width) {}
+    // slot of row j: 16-byte pieces of all threads side by side
+    __device__ __forceinline__ uint32_t slot(int j) const { return ring + (j % kAhead) * (kBytes * 256); }
+    __device__ __forceinline__ void fetch(int j, int, unsigned token) const {
+        if (!inside) return;
+        const char* src = reinterpret_cast<const char*>(from + (int64_t)token * ld);
+#pragma unroll
+        for (int b = 0; b < kBytes; b += 16)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slot(j) + b * 256), "l"(src + b) : "memory");
+    }
+    __device__ __forceinline__ void commit() const { asm volatile("cp.async.commit_group;" ::: "memory"); }
+    __device__ __forceinline__ void wait() const { asm volatile("cp.async.wait_group %0;" ::"n"(kAhead / kGroup - 1) : "memory"); }
+    __device__ __forceinline__ void drain() const { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
+    __device__ __forceinline__ void add(int j, int, float* sum) const {  // (columns behind the width hold anything and are not stored)
+        Pack<T, V> p;
+        uint32_t* w = reinterpret_cast<uint32_t*>(&p);
+#pragma unroll
+        for (int b = 0; b < kBytes; b += 16)
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(w[b / 4]), "=r"(w[b / 4 + 1]), "=r"(w[b / 4 + 2]), "=r"(w[b / 4 + 3])
+                         : "r"(slot(j) + b * 256));
+#pragma unroll
+        for (int i = 0; i < V; ++i) sum[i] += to_float(p.v[i]);
+    }
+};
+// Single columns: eight rows at a time in registers.
+template <typename T>
+struct Rows<T, 1> {
+    static constexpr int kAhead = 8, kGroup = 8, kShared = 0;
+    T v[kGroup][kLoose];
+    const T* from;
+    int64_t ld, left;  // columns from the thread's first one on
+    __device__ __forceinline__ Rows(uint8_t*, const T* dy, int64_t ld_y, int64_t first, int64_t width, int lane)
+        : from(dy + first + lane), ld(ld_y), left(width - first - lane) {}
+    __device__ __forceinline__ void fetch(int, int x, unsigned token) {
+#pragma unroll
+        for (int i = 0; i < kLoose; ++i)
+            if (32 * i < left) v[x][i] = from[(int64_t)token * ld + 32 * i];
+    }
+    __device__ __forceinline__ void commit() const {}
+    __device__ __forceinline__ void wait() const {}
+    __device__ __forceinline__ void drain() const {}
+    __device__ __forceinline__ void add(int, int x, float* sum) const {
+#pragma unroll
+        for (int i = 0; i < kLoose; ++i) sum[i] += to_float(v[x][i]);
+    }
+};
+
 struct GradientArgs {
     int64_t count, rows, width, ld_y, ld_e, chunks;
     int chunk, slabs;
-    const int* keys;       // sorted
-    const unsigned* perm;  // token of every sorted place
-    float* partial;        // [chunk][2][width]: a sum that came in open, a sum that goes out open
+    const uint2* sorted;  // (row, token) by row, then token; row = rows: none
+    float* partial;       // [chunk][2][width]: a sum that came in open, a sum that goes out open
 };
 
 // dE[r, slab] = beta * dE[r, slab] + alpha * sum
@@ -168,49 +259,62 @@ template <typename Y, typename E, int V>
 __global__ void __launch_bounds__(256)
     embedding_sum_kernel(GradientArgs a, const Y* __restrict__ dy, E* __restrict__ table, ScalarArg<float> alpha_arg,
                          ScalarArg<float> beta_arg) {
-    constexpr int kPer = Columns<V>::kPer, kSlab = Columns<V>::kSlab, kDepth = 8;
+    constexpr int kPer = Columns<V>::kPer, kSlab = Columns<V>::kSlab;
     const int64_t warp = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> 5;
     const int lane = threadIdx.x & 31;
     const float alpha = alpha_arg.get(), beta = beta_arg.get();
+    grid_release();
     if (warp >= a.chunks * a.slabs) return;
     const int64_t c = warp / a.slabs;
     const int64_t first = (warp - c * a.slabs) * kSlab;
     const int64_t k0 = c * a.chunk, k1 = min(k0 + a.chunk, a.count);
+    grid_wait();  // the sort
     float sum[kPer];
 #pragma unroll
     for (int i = 0; i < kPer; ++i) sum[i] = 0.0f;
-    int row = __ldg(a.keys + k0);
-    bool open = k0 > 0 && __ldg(a.keys + k0 - 1) == row;  // the first sum began in an earlier chunk
-    for (int64_t k = k0; k < k1; k += kDepth) {
-        float v[kDepth][kPer];
-        int key[kDepth];
+    int row = (int)__ldcg(&a.sorted[k0].x);
+    bool open = k0 > 0 && (int)__ldcg(&a.sorted[k0 - 1].x) == row;  // the first sum began in an earlier chunk
+    extern __shared__ __align__(16) uint8_t smem_raw[];
+    Rows<Y, V> rows(smem_raw, dy, a.ld_y, first, a.width, lane);
+    for (int64_t k = k0; k < k1; k += 32) {
+        // lane l holds token k + l
+        const uint2 token = k + lane < k1 ? __ldcg(a.sorted + k + lane) : make_uint2((unsigned)a.rows, 0u);
+        const int n = (int)min(k1 - k, (int64_t)32);
+        const auto fetch = [&](int j) {  // the next kGroup tokens
 #pragma unroll
-        for (int j = 0; j < kDepth; ++j) {
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) v[j][i] = 0.0f;
-            key[j] = k + j < k1 ? __ldg(a.keys + k + j) : (int)a.rows;
-            if (key[j] < a.rows) load_columns<Y, V>(dy + (int64_t)__ldg(a.perm + k + j) * a.ld_y, first, a.width, lane, v[j]);
-        }
-#pragma unroll
-        for (int j = 0; j < kDepth; ++j) {
-            if (k + j < k1) {
-                if (key[j] != row) {
-                    if (open)
-                        store_columns<float, V>(a.partial + (2 * c) * a.width, first, a.width, lane, sum);
-                    else
-                        finish_row<E, V>(table, a, row, first, lane, alpha, beta, sum);
-                    open = false;
-                    row = key[j];
-#pragma unroll
-                    for (int i = 0; i < kPer; ++i) sum[i] = 0.0f;
-                }
-#pragma unroll
-                for (int i = 0; i < kPer; ++i) sum[i] += v[j][i];
+            for (int x = 0; x < Rows<Y, V>::kGroup; ++x) {
+                const unsigned key = __shfl_sync(0xffffffffu, token.x, (j + x) & 31), t = __shfl_sync(0xffffffffu, token.y, (j + x) & 31);
+                if (j + x < n && key < (unsigned)a.rows) rows.fetch(j + x, x, t);
             }
+            rows.commit();
+        };
+#pragma unroll
+        for (int j = 0; j < Rows<Y, V>::kAhead; j += Rows<Y, V>::kGroup) fetch(j);
+        for (int j0 = 0; j0 < n; j0 += Rows<Y, V>::kGroup) {
+            rows.wait();
+#pragma unroll
+            for (int x = 0; x < Rows<Y, V>::kGroup; ++x) {
+                const int key = (int)__shfl_sync(0xffffffffu, token.x, (j0 + x) & 31);
+                if (j0 + x < n) {
+                    if (key != row) {
+                        if (open)
+                            store_columns<float, V>(a.partial + (2 * c) * a.width, first, a.width, lane, sum);
+                        else
+                            finish_row<E, V>(table, a, row, first, lane, alpha, beta, sum);
+                        open = false;
+                        row = key;
+#pragma unroll
+                        for (int i = 0; i < kPer; ++i) sum[i] = 0.0f;
+                    }
+                    if (key < a.rows) rows.add(j0 + x, x, sum);
+                }
+            }
+            fetch(j0 + Rows<Y, V>::kAhead);
         }
+        rows.drain();
     }
     if (row >= a.rows) return;
-    const bool goes_on = k1 < a.count && __ldg(a.keys + k1) == row;
+    const bool goes_on = k1 < a.count && (int)__ldcg(&a.sorted[k1].x) == row;
     if (open)
         store_columns<float, V>(a.partial + (2 * c) * a.width, first, a.width, lane, sum);
     else if (goes_on)
@@ -219,46 +323,64 @@ __global__ void __launch_bounds__(256)
         finish_row<E, V>(table, a, row, first, lane, alpha, beta, sum);
 }
 
-// One warp per (chunk, slab): if a sum starts in this chunk and goes on, its partials are added in chunk order.
+// One block per chunk: if a sum starts in this chunk and goes on, its partials are added. The warps share out the slabs of
+// columns, kWays of them a slab's chunks (each adds its own in order, then the kWays sums are added in order).
+constexpr int kWays = 2;
+constexpr int kJoinThreads = 512;
+
 template <typename E, int V>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kJoinThreads)
     embedding_join_kernel(GradientArgs a, E* __restrict__ table, ScalarArg<float> alpha_arg, ScalarArg<float> beta_arg) {
-    constexpr int kPer = Columns<V>::kPer, kSlab = Columns<V>::kSlab, kDepth = 8;
-    const int64_t warp = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> 5;
-    const int lane = threadIdx.x & 31;
-    const int64_t c = warp / a.slabs;
-    if (c + 1 >= a.chunks) return;
-    const int64_t first = (warp - c * a.slabs) * kSlab;
+    constexpr int kPer = Columns<V>::kPer, kSlab = Columns<V>::kSlab, kDepth = 8, kSlabs = kJoinThreads / 32 / kWays;
+    __shared__ float s_sum[kJoinThreads / 32][kPer][32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, way = warp % kWays;
+    const int64_t c = blockIdx.x;
     const int64_t k0 = c * a.chunk, k1 = k0 + a.chunk;
-    const int row = __ldg(a.keys + k1 - 1);
-    if (row >= a.rows || __ldg(a.keys + k1) != row) return;          // nothing goes on
-    if (k0 > 0 && __ldg(a.keys + k0 - 1) == row) return;              // it started earlier
-    // its last chunk: the keys at the chunks' starts ascend, 32 of them are looked at in one step
+    grid_wait();  // the sums
+    if (c + 1 >= a.chunks) return;
+    const unsigned row = __ldcg(&a.sorted[k1 - 1].x);
+    if (row >= (unsigned)a.rows || __ldcg(&a.sorted[k1].x) != row) return;  // nothing goes on
+    if (k0 > 0 && __ldcg(&a.sorted[k0 - 1].x) == row) return;               // it started earlier
+    // its last chunk: the rows at the chunks' starts ascend, 32 of them are looked at in one step
     int64_t last = c + 1, beyond = a.chunks;
     while (beyond - last > 1) {
         const int64_t step = (beyond - last + 31) / 32, d = last + step * lane;
-        const unsigned same = __ballot_sync(0xffffffffu, d < beyond && __ldg(a.keys + d * a.chunk) == row);
+        const unsigned same = __ballot_sync(0xffffffffu, d < beyond && __ldcg(&a.sorted[d * a.chunk].x) == row);
         last += step * (31 - __clz(same));
         beyond = min(last + step, beyond);
     }
-    float sum[kPer];
+    const float alpha = alpha_arg.get(), beta = beta_arg.get();
+    for (int slab0 = 0; slab0 < a.slabs; slab0 += kSlabs) {  // block-uniform
+        const int64_t first = (int64_t)(slab0 + warp / kWays) * kSlab;
+        float sum[kPer];
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) sum[i] = 0.0f;
-    load_columns<float, V>(a.partial + (2 * c + 1) * a.width, first, a.width, lane, sum);
-    for (int64_t d = c + 1; d <= last; d += kDepth) {
-        float v[kDepth][kPer];
+        for (int i = 0; i < kPer; ++i) sum[i] = 0.0f;
+        if (way == 0) load_columns<float, V>(a.partial + (2 * c + 1) * a.width, first, a.width, lane, sum);
+        for (int64_t d = c + 1 + way; d <= last; d += kWays * kDepth) {
+            float v[kDepth][kPer];
 #pragma unroll
-        for (int j = 0; j < kDepth; ++j) {
+            for (int j = 0; j < kDepth; ++j) {
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) v[j][i] = 0.0f;
-            if (d + j <= last) load_columns<float, V>(a.partial + (2 * (d + j)) * a.width, first, a.width, lane, v[j]);
+                for (int i = 0; i < kPer; ++i) v[j][i] = 0.0f;
+                if (d + kWays * j <= last) load_columns<float, V>(a.partial + (2 * (d + kWays * j)) * a.width, first, a.width, lane, v[j]);
+            }
+#pragma unroll
+            for (int j = 0; j < kDepth; ++j)
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) sum[i] += v[j][i];
         }
 #pragma unroll
-        for (int j = 0; j < kDepth; ++j)
+        for (int i = 0; i < kPer; ++i) s_sum[warp][i][lane] = sum[i];
+        __syncthreads();
+        if (way == 0) {
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) sum[i] += v[j][i];
+            for (int w = 1; w < kWays; ++w)
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) sum[i] += s_sum[warp + w][i][lane];
+            finish_row<E, V>(table, a, row, first, lane, alpha, beta, sum);
+        }
+        __syncthreads();
     }
-    finish_row<E, V>(table, a, row, first, lane, alpha_arg.get(), beta_arg.get(), sum);
 }
 
 // ----------------------------------------------------------------------------- sort, and the rows without a token
@@ -274,14 +396,14 @@ struct SortArgs {
     const void* ids;
     bool wide;
     int base;
-    int* keys[2];       // ping-pong; the last pass writes the one `passes` says
-    unsigned* perm[2];
+    uint2* sorted[2];   // (key, token); the passes write them in turn
     int passes, bits;   // digits of `bits` bits, at most 9
-    int sorters;        // thread blocks that sort: the first cluster, or none
+    int sorters;        // thread blocks that sort (one cluster)
     // rows without a token
     void* table;
     int64_t ld, width;
-    int64_t fill_rows;  // rows a block looks after at a time
+    int fill_shift;     // 2^fill_shift thread blocks look after them: row r belongs to block r % 2^fill_shift
+    int fill_rows;      // rows of a block that are marked at a time
 };
 
 // key = the row of the table, or `rows` for an id outside it (sorted behind every row and then left out).
@@ -304,58 +426,69 @@ __device__ __forceinline__ unsigned load_remote(const unsigned* p, int rank) {
 
 struct SortShared {
     unsigned short warp[32][kMostDigits];  // digit counts of every warp, then their exclusive sums over the warps
+    unsigned quarter[4][kMostDigits / 2];  // sums over 8 warps each, two digits to a word
     unsigned total[kMostDigits];           // digit counts of the block, read by the whole cluster
     unsigned base[kMostDigits];            // first place of the block's items with a digit
     unsigned part[32];
 };
 
 // Items are owned in ascending order by (block, warp, round, lane), so that equal keys keep their order.
-__device__ __forceinline__ void sort_block(const SortArgs& a, SortShared& s) {
-    const int rank = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+__device__ __forceinline__ void sort_block(const SortArgs& a, SortShared& s, int rank) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rounds = (int)((a.count + (int64_t)a.sorters * kSortThreads - 1) / ((int64_t)a.sorters * kSortThreads));
     const int64_t begin = ((int64_t)rank * 32 + warp) * rounds * 32 + lane;
     const int digits = 1 << a.bits;
     for (int pass = 0; pass < a.passes; ++pass) {
         const int shift = pass * a.bits, to = pass & 1;
-        const int* in_keys = a.keys[to ^ 1];
-        const unsigned* in_perm = a.perm[to ^ 1];
+        const uint2* in = a.sorted[to ^ 1];
         for (int i = threadIdx.x; i < 32 * kMostDigits / 2; i += kSortThreads) reinterpret_cast<unsigned*>(s.warp)[i] = 0u;
-        int key[kSortRounds];
-        unsigned perm[kSortRounds];
-        unsigned short rank_in_warp[kSortRounds];
+        uint2 pair[kSortRounds];
+        unsigned ranks[kSortRounds / 2];  // place of an item among its warp's items with the same digit, two to a word
 #pragma unroll
         for (int r = 0; r < kSortRounds; ++r) {
             const int64_t t = begin + 32 * r;
-            key[r] = 0, perm[r] = 0;
-            if (r < rounds && t < a.count) {
-                // (the previous pass's output was written by other blocks of the cluster: read past L1)
-                key[r] = pass == 0 ? key_of(a, t) : __ldcg(in_keys + t);
-                perm[r] = pass == 0 ? (unsigned)t : __ldcg(in_perm + t);
-            }
+            pair[r] = make_uint2(0u, 0u);
+            // (the previous pass's output was written by other blocks of the cluster: read past L1)
+            if (r < rounds && t < a.count) pair[r] = pass == 0 ? make_uint2((unsigned)key_of(a, t), (unsigned)t) : __ldcg(in + t);
         }
         __syncthreads();
 #pragma unroll
         for (int r = 0; r < kSortRounds; ++r) {
             if (r < rounds) {
                 const bool live = begin + 32 * r < a.count;
-                const unsigned d = live ? ((unsigned)key[r] >> shift) & (digits - 1) : 0xffffu;
+                const unsigned d = live ? (pair[r].x >> shift) & (digits - 1) : 0xffffu;
                 const unsigned peers = __match_any_sync(0xffffffffu, d);
                 const unsigned before = live ? s.warp[warp][d] : 0;
                 __syncwarp();
                 if (live && lane == __ffs(peers) - 1) s.warp[warp][d] = (unsigned short)(before + __popc(peers));
                 __syncwarp();
-                rank_in_warp[r] = (unsigned short)(before + __popc(peers & ((1u << lane) - 1u)));
+                const unsigned rank_here = before + __popc(peers & ((1u << lane) - 1u));
+                ranks[r / 2] = r & 1 ? ranks[r / 2] | rank_here << 16 : rank_here;
             }
         }
         __syncthreads();
-        if ((int)threadIdx.x < digits) {  // counts of the warps -> exclusive sums over the warps
-            unsigned sum = 0;
-            for (int w = 0; w < 32; ++w) {
-                const unsigned c = s.warp[w][threadIdx.x];
-                s.warp[w][threadIdx.x] = (unsigned short)sum;
-                sum += c;
+        {  // counts of the warps -> exclusive sums over the warps: a thread takes two digits (one word) of 8 warps
+            const int word = threadIdx.x & (kMostDigits / 2 - 1), q = threadIdx.x / (kMostDigits / 2);
+            unsigned* const col = reinterpret_cast<unsigned*>(s.warp[8 * q]) + word;
+            unsigned c[8], sum = 0;
+#pragma unroll
+            for (int w = 0; w < 8; ++w) c[w] = col[w * (kMostDigits / 2)];
+#pragma unroll
+            for (int w = 0; w < 8; ++w) {  // (a block has at most 2^14 items: the halves of a word do not meet)
+                const unsigned x = c[w];
+                c[w] = sum;
+                sum += x;
             }
-            s.total[threadIdx.x] = sum;
+            s.quarter[q][word] = sum;
+            __syncthreads();
+            unsigned ahead = 0;
+            for (int x = 0; x < q; ++x) ahead += s.quarter[x][word];
+#pragma unroll
+            for (int w = 0; w < 8; ++w) col[w * (kMostDigits / 2)] = ahead + c[w];
+            if (q == 3) {
+                const unsigned all = ahead + sum;
+                s.total[2 * word] = all & 0xffffu, s.total[2 * word + 1] = all >> 16;
+            }
         }
         cluster_sync();
         // places: all smaller digits of the cluster, then the same digit in the blocks before this one
@@ -382,66 +515,102 @@ __device__ __forceinline__ void sort_block(const SortArgs& a, SortShared& s) {
 #pragma unroll
         for (int r = 0; r < kSortRounds; ++r) {
             if (r < rounds && begin + 32 * r < a.count) {
-                const unsigned d = ((unsigned)key[r] >> shift) & (digits - 1);
-                const unsigned at = s.base[d] + s.warp[warp][d] + rank_in_warp[r];
-                a.keys[to][at] = key[r];
-                a.perm[to][at] = perm[r];
+                const unsigned d = (pair[r].x >> shift) & (digits - 1);
+                const unsigned at = s.base[d] + s.warp[warp][d] + (r & 1 ? ranks[r / 2] >> 16 : ranks[r / 2] & 0xffffu);
+                a.sorted[to][at] = pair[r];
             }
         }
         cluster_sync();  // the pass is in memory, and nobody reads this block's counts any more
     }
 }
 
-constexpr int kMostFillRows = 65536;
+constexpr int kMostFillRows = 65536;      // 8 KB of marks
+constexpr int kZeroBytes = 16384;         // behind them: zeros to copy from
+constexpr int kFillShared = kMostFillRows / 8 + kZeroBytes;
 
-// The rows [row0, row1) that no id names become beta times what they are (beta = 0: zero). One warp per row.
+// Of the rows `block`, block + fillers, ..., those that no id names become beta times what they are (beta = 0: zero). Their
+// marks are set from all ids, for fill_rows of them at a time; one warp per row then. Zeros leave as bulk copies of shared
+// memory: one instruction per row keeps HBM's write path full (ordinary 32-byte stores reached 3.1 TB/s, these 6).
 template <typename E, int V>
-__device__ __forceinline__ void fill_block(const SortArgs& a, float beta, unsigned* bits, int64_t row0, int64_t row1) {
-    for (int i = threadIdx.x; i < (row1 - row0 + 31) / 32; i += kSortThreads) bits[i] = 0u;
-    __syncthreads();
-    for (int64_t t = threadIdx.x; t < a.count; t += 4 * kSortThreads) {
-        int key[4];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) key[x] = t + x * kSortThreads < a.count ? key_of(a, t + x * kSortThreads) : -1;
-#pragma unroll
-        for (int x = 0; x < 4; ++x)
-            if (key[x] >= row0 && key[x] < row1) atomicOr(&bits[(key[x] - row0) >> 5], 1u << ((key[x] - row0) & 31));
+__device__ __forceinline__ void fill_block(const SortArgs& a, float beta, uint8_t* smem, int block) {
+    unsigned* const bits = reinterpret_cast<unsigned*>(smem);
+    const uint32_t zeros = static_cast<uint32_t>(__cvta_generic_to_shared(smem + kMostFillRows / 8));
+    const bool bulk = V > 1 && beta == 0.0f;
+    if (bulk) {
+        for (int i = threadIdx.x; i < kZeroBytes / 16; i += kSortThreads)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(zeros + 16 * i), "r"(0) : "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    __syncthreads();
-    const int lane = threadIdx.x & 31;
-    for (int64_t r = row0 + (threadIdx.x >> 5); r < row1; r += kSortThreads / 32) {
-        if (bits[(r - row0) >> 5] >> ((r - row0) & 31) & 1) continue;
-        E* row = static_cast<E*>(a.table) + r * a.ld;
-        for (int64_t c = 0; c < a.width; c += Columns<V>::kSlab) {
-            float v[Columns<V>::kPer] = {};
-            if (beta != 0.0f) {
-                load_columns<E, V>(row, c, a.width, lane, v);
+    const int fillers = 1 << a.fill_shift;
+    const int64_t mine = (a.rows - block + fillers - 1) >> a.fill_shift;
+    for (int64_t from = 0; from < mine; from += a.fill_rows) {
+        const int n = (int)min((int64_t)a.fill_rows, mine - from);
+        for (int i = threadIdx.x; i < (n + 31) / 32; i += kSortThreads) bits[i] = 0u;
+        __syncthreads();
+        for (int64_t t = threadIdx.x; t < a.count; t += 8 * kSortThreads) {
+            int key[8];
 #pragma unroll
-                for (int i = 0; i < Columns<V>::kPer; ++i) v[i] *= beta;
+            for (int x = 0; x < 8; ++x) key[x] = t + x * kSortThreads < a.count ? key_of(a, t + x * kSortThreads) : (int)a.rows;
+#pragma unroll
+            for (int x = 0; x < 8; ++x) {
+                const int64_t i = (key[x] >> a.fill_shift) - from;
+                if (key[x] < a.rows && (key[x] & (fillers - 1)) == block && i >= 0 && i < n) atomicOr(&bits[i >> 5], 1u << (i & 31));
             }
-            store_columns<E, V>(row, c, a.width, lane, v);
         }
+        __syncthreads();
+        const int lane = threadIdx.x & 31;
+        for (int i = threadIdx.x >> 5; i < n; i += kSortThreads / 32) {
+            if (bits[i >> 5] >> (i & 31) & 1) continue;
+            E* row = static_cast<E*>(a.table) + (((from + i) << a.fill_shift) + block) * a.ld;
+            if (bulk) {
+                const int64_t bytes = a.width * (int64_t)sizeof(E);
+                if (lane == 0)
+                    for (int64_t x = 0; x < bytes; x += kZeroBytes)
+                        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(reinterpret_cast<char*>(row) + x),
+                                     "r"(zeros), "r"((int)min(bytes - x, (int64_t)kZeroBytes))
+                                     : "memory");
+                continue;
+            }
+            for (int64_t c = 0; c < a.width; c += Columns<V>::kSlab) {
+                float v[Columns<V>::kPer] = {};
+                if (beta != 0.0f) {
+                    load_columns<E, V>(row, c, a.width, lane, v);
+#pragma unroll
+                    for (int x = 0; x < Columns<V>::kPer; ++x) v[x] *= beta;
+                }
+                store_columns<E, V>(row, c, a.width, lane, v);
+            }
+        }
+        __syncthreads();
     }
-    __syncthreads();
+    if (bulk) asm volatile("cp.async.bulk.commit_group;\ncp.async.bulk.wait_group 0;" ::: "memory");
 }
 
+__global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(const SortArgs a) {
+    __shared__ SortShared s;
+    grid_release();
+    sort_block(a, s, (int)blockIdx.x);
+}
+
+// Runs beside the sort, which lets it start at once; it ends no earlier than the sort does, so that what waits for this launch
+// waits for both. A sort by one block is its last block.
 template <typename E, int V>
-__global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(const SortArgs a, ScalarArg<float> beta_arg) {
-    extern __shared__ __align__(16) uint8_t smem_raw[];
-    if ((int)blockIdx.x < a.sorters) {
-        sort_block(a, *reinterpret_cast<SortShared*>(smem_raw));
+__global__ void __launch_bounds__(kSortThreads) embedding_fill_kernel(const SortArgs a, ScalarArg<float> beta_arg) {
+    constexpr size_t kShared = sizeof(SortShared) > kFillShared ? sizeof(SortShared) : kFillShared;
+    __shared__ __align__(16) uint8_t smem[kShared];
+    grid_release();
+    if ((int)blockIdx.x == 1 << a.fill_shift) {
+        sort_block(a, *reinterpret_cast<SortShared*>(smem), 0);
         return;
     }
     const float beta = beta_arg.get();
-    if (beta == 1.0f) return;
-    for (int64_t row0 = (blockIdx.x - a.sorters) * a.fill_rows; row0 < a.rows; row0 += (gridDim.x - a.sorters) * a.fill_rows)
-        fill_block<E, V>(a, beta, reinterpret_cast<unsigned*>(smem_raw), row0, min(row0 + a.fill_rows, a.rows));
+    if (beta != 1.0f && (int64_t)blockIdx.x < a.rows) fill_block<E, V>(a, beta, smem, (int)blockIdx.x);
+    grid_wait();
 }
 
 template <typename T, int V>
 bool wide_rows(const void* p, int64_t ld, int64_t width) {
-    return (reinterpret_cast<uintptr_t>(p) & (sizeof(T) * V >= 16 ? 15 : sizeof(T) * V - 1)) == 0 && ld % V == 0 &&
-           width % V == 0;
+    return (reinterpret_cast<uintptr_t>(p) & (sizeof(T) * V - 1)) == 0 && ld % V == 0 && width % V == 0;
 }
 
 // Warps of a launch as a grid of 8-warp blocks; 0 when the grid would be too large.
@@ -463,7 +632,7 @@ cudaError_t launch_lookup(cudaStream_t s, const EmbeddingArgs& a, const I* ids) 
 
 template <typename E, typename Y>
 cudaError_t lookup_typed(cudaStream_t s, const EmbeddingArgs& a) {
-    // 16 bytes of the wider of the two types' rows per thread
+    // 8 values per thread (16 or 32 bytes); fp32 on both sides: 4, so that narrow tables still fill a warp
     constexpr int V = sizeof(E) == 4 && sizeof(Y) == 4 ? 4 : 8;
     const bool wide = wide_rows<E, V>(a.table, a.ld_table, a.width) && wide_rows<Y, V>(a.tokens, a.ld_tokens, a.width);
     if (a.wide_ids) {
@@ -477,12 +646,12 @@ cudaError_t lookup_typed(cudaStream_t s, const EmbeddingArgs& a) {
 size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
 
 // Tokens per chunk: long enough that few sums cross chunks, short enough that the chunks fill the GPU
-// (148 SMs x 32 warps) when there are few tokens.
+// (148 SMs x 16 warps) when there are few tokens.
 int gradient_chunk(int64_t count, int64_t width) {
-    const int64_t slabs = (width + 127) / 128;
-    const int64_t want = count * slabs / (148 * 32);
+    const int64_t slabs = (width + 255) / 256;
+    const int64_t want = count * slabs / (148 * 16);
     int chunk = 8;
-    while (chunk < 64 && chunk < want) chunk *= 2;
+    while (chunk < 64 && 2 * chunk <= want) chunk *= 2;
     return chunk;
 }
 
@@ -491,7 +660,7 @@ struct GradientLayout {
     TransposePlan sort;  // more tokens than one cluster sorts
     int chunk;
     int64_t chunks;
-    size_t off_raw, off_keys[2], off_perm[2], off_partial, bytes;
+    size_t off_raw, off_sorted[2], off_partial, bytes;
 };
 
 GradientLayout gradient_layout(int64_t count, int64_t rows, int64_t width) {
@@ -500,17 +669,15 @@ GradientLayout gradient_layout(int64_t count, int64_t rows, int64_t width) {
     l.chunk = gradient_chunk(count, width);
     l.chunks = (count + l.chunk - 1) / l.chunk;
     size_t off = 0;
-    if (l.one_cluster) {
-        for (size_t* p : {&l.off_keys[0], &l.off_keys[1], &l.off_perm[0], &l.off_perm[1]}) {
-            *p = off;
-            off += align256(size_t(count) * 4);
-        }
-    } else {
+    if (!l.one_cluster) {
         l.sort = transpose_plan(rows, rows + 1, count, 0);
-        for (int i = 0; i < 2; ++i) l.off_keys[i] = l.sort.off_keys[i], l.off_perm[i] = l.sort.off_perm[i];
         off = l.sort.bytes;
         l.off_raw = off;
         off += align256(size_t(count) * 4);
+    }
+    for (int i = 0; i < (l.one_cluster ? 2 : 1); ++i) {
+        l.off_sorted[i] = off;
+        off += align256(size_t(count) * 8);
     }
     l.off_partial = off;
     off += align256(size_t(l.chunks) * 2 * size_t(width) * 4);
@@ -522,6 +689,28 @@ __global__ void __launch_bounds__(256) embedding_keys_kernel(const SortArgs a, i
     const int64_t t = blockIdx.x * (int64_t)blockDim.x + threadIdx.x;
     if (t < a.count) keys[t] = key_of(a, t);
 }
+__global__ void __launch_bounds__(256)
+    embedding_pairs_kernel(int64_t count, const int* __restrict__ keys, const unsigned* __restrict__ perm, uint2* __restrict__ sorted) {
+    const int64_t t = blockIdx.x * (int64_t)blockDim.x + threadIdx.x;
+    if (t < count) sorted[t] = make_uint2((unsigned)keys[t], perm[t]);
+}
+
+// A launch whose blocks may come up before the launch ahead of it is done (they wait in grid_wait()); early = false: an
+// ordinary one.
+template <typename... P, typename... A>
+cudaError_t launch_behind(cudaStream_t s, bool early, void (*kernel)(P...), unsigned blocks, int threads, int shared, A... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(blocks);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = (size_t)shared;
+    cfg.stream = s;
+    cudaLaunchAttribute attr = {};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = early ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
 
 template <typename Y, typename E, int V>
 cudaError_t launch_gradient(cudaStream_t s, const EmbeddingArgs& a, char* b) {
@@ -530,47 +719,44 @@ cudaError_t launch_gradient(cudaStream_t s, const EmbeddingArgs& a, char* b) {
     SortArgs so = {};
     so.count = a.count, so.rows = a.rows, so.ids = a.ids, so.wide = a.wide_ids, so.base = a.base;
     so.table = a.table, so.ld = a.ld_table, so.width = a.width;
-    for (int i = 0; i < 2; ++i)
-        so.keys[i] = reinterpret_cast<int*>(b + l.off_keys[i]), so.perm[i] = reinterpret_cast<unsigned*>(b + l.off_perm[i]);
+    for (int i = 0; i < 2; ++i) so.sorted[i] = reinterpret_cast<uint2*>(b + l.off_sorted[i]);
     int need = 1;  // bits of a key, `rows` included
     while (need < 31 && (int64_t(1) << need) <= a.rows) ++need;
     so.passes = (need + 8) / 9;
     so.bits = (need + so.passes - 1) / so.passes;
     const bool fill = a.beta.dev != nullptr || a.beta.host != 1.0f;
-    // (few tokens: one block sorts them in two rounds, with a cluster of one)
-    const int cluster = l.one_cluster && a.count > 2 * kSortThreads ? kSortCluster : 1;
-    so.sorters = l.one_cluster && a.count > 0 ? cluster : 0;
     int last = (so.passes - 1) & 1;
+    // few tokens: one block sorts them in two rounds, as a further block of the other launch where there is one
+    so.sorters = a.count == 0 || !l.one_cluster ? 0 : a.count > 2 * kSortThreads ? kSortCluster : 1;
+    const bool together = fill && so.sorters == 1;
+    if (so.sorters > 0 && !together) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)so.sorters);
+        cfg.blockDim = dim3(kSortThreads);
+        cfg.stream = s;
+        cudaLaunchAttribute attr = {};
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = (unsigned)so.sorters, attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        const cudaError_t e = cudaLaunchKernelEx(&cfg, embedding_sort_kernel, static_cast<const SortArgs>(so));
+        if (e != cudaSuccess) return e;
+    }
     if (!l.one_cluster) {
         int* raw = reinterpret_cast<int*>(b + l.off_raw);
         embedding_keys_kernel<<<(unsigned)((a.count + 255) / 256), 256, 0, s>>>(so, raw);
         const cudaError_t e = sort_keys(s, a.rows, a.count, raw, l.sort, b);
         if (e != cudaSuccess) return e;
-        last = l.sort.final_slot();
+        const int slot = l.sort.final_slot();
+        last = 0;
+        embedding_pairs_kernel<<<(unsigned)((a.count + 255) / 256), 256, 0, s>>>(
+            a.count, reinterpret_cast<const int*>(b + l.sort.off_keys[slot]), reinterpret_cast<const unsigned*>(b + l.sort.off_perm[slot]), so.sorted[0]);
     }
-    // one block per SM beside the sorting cluster; ranges of rows small enough for their marks to fit in shared memory
-    int64_t fillers = fill ? (a.sm_count / cluster) * cluster - (cluster > 1 ? cluster : 0) : 0;
-    if (fill) {
-        so.fill_rows = (a.rows + fillers - 1) / fillers;
-        if (so.fill_rows > kMostFillRows) so.fill_rows = kMostFillRows;
-        so.fill_rows = (so.fill_rows + 31) / 32 * 32;
-        const int64_t ranges = (a.rows + so.fill_rows - 1) / so.fill_rows;
-        if (ranges < fillers) fillers = (ranges + cluster - 1) / cluster * cluster;
-    }
-    if (so.sorters + fillers > 0) {
-        constexpr size_t kShared = sizeof(SortShared) > kMostFillRows / 8 ? sizeof(SortShared) : kMostFillRows / 8;
-        static_assert(kShared <= 48 * 1024, "fits without opting in to more");
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3((unsigned)(so.sorters + fillers));
-        cfg.blockDim = dim3(kSortThreads);
-        cfg.dynamicSmemBytes = kShared;
-        cfg.stream = s;
-        cudaLaunchAttribute attr = {};
-        attr.id = cudaLaunchAttributeClusterDimension;
-        attr.val.clusterDim.x = (unsigned)cluster, attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-        cfg.attrs = &attr;
-        cfg.numAttrs = cluster > 1 ? 1 : 0;
-        const cudaError_t e = cudaLaunchKernelEx(&cfg, embedding_sort_kernel<E, V>, static_cast<const SortArgs>(so), a.beta);
+    if (fill) {  // a power of two of blocks, at most one per SM
+        while ((2 << so.fill_shift) <= a.sm_count && (int64_t(1) << so.fill_shift) < a.rows) ++so.fill_shift;
+        const int64_t each = (a.rows >> so.fill_shift) + 1;
+        so.fill_rows = (int)(each < kMostFillRows ? each : kMostFillRows);
+        const cudaError_t e = launch_behind(s, so.sorters == kSortCluster, embedding_fill_kernel<E, V>, (1u << so.fill_shift) + (together ? 1u : 0u), kSortThreads, 0, so, a.beta);
         if (e != cudaSuccess) return e;
     }
     if (a.count == 0) return cudaSuccess;
@@ -578,14 +764,19 @@ cudaError_t launch_gradient(cudaStream_t s, const EmbeddingArgs& a, char* b) {
     GradientArgs g = {};
     g.count = a.count, g.rows = a.rows, g.width = a.width, g.ld_y = a.ld_tokens, g.ld_e = a.ld_table;
     g.chunk = l.chunk, g.chunks = l.chunks;
-    g.keys = so.keys[last], g.perm = so.perm[last];
+    g.sorted = so.sorted[last];
     g.partial = reinterpret_cast<float*>(b + l.off_partial);
     g.slabs = (int)((a.width + Columns<V>::kSlab - 1) / Columns<V>::kSlab);
     const unsigned blocks = warp_blocks(g.chunks * g.slabs);
     if (blocks == 0) return cudaErrorInvalidValue;
-    embedding_sum_kernel<Y, E, V><<<blocks, 256, 0, s>>>(g, static_cast<const Y*>(a.tokens), static_cast<E*>(a.table), a.alpha, a.beta);
-    if (g.chunks > 1) embedding_join_kernel<E, V><<<blocks, 256, 0, s>>>(g, static_cast<E*>(a.table), a.alpha, a.beta);
-    return cudaGetLastError();
+    constexpr int kShared = Rows<Y, V>::kShared;
+    cudaError_t e = cudaSuccess;
+    static SharedMemoryOnce once;
+    if (kShared > 48 * 1024) e = once.allow(reinterpret_cast<const void*>(embedding_sum_kernel<Y, E, V>), kShared);
+    if (e == cudaSuccess) e = launch_behind(s, true, embedding_sum_kernel<Y, E, V>, blocks, 256, kShared, g, static_cast<const Y*>(a.tokens), static_cast<E*>(a.table), a.alpha, a.beta);
+    if (e == cudaSuccess && g.chunks > 1)
+        e = launch_behind(s, true, embedding_join_kernel<E, V>, (unsigned)(g.chunks - 1), kJoinThreads, 0, g, static_cast<E*>(a.table), a.alpha, a.beta);
+    return e;
 }
 
 template <typename E, typename Y>

@@ -3,6 +3,7 @@
 
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstddef>
 #include <cstdint>
 #include <mutex>
@@ -361,6 +362,21 @@ cudaError_t shard_row_bounds(cudaStream_t s, int64_t m, int64_t nnz, int base, c
                              int num_shards, int64_t* bounds_host);
 cudaError_t shard_local_row_offsets(cudaStream_t s, const int32_t* row_ptr, int64_t first_row, int64_t num_rows,
                                     int base, int32_t* local);
+
+// Opts a kernel in to more than 48 KB of dynamic shared memory, once per device (one object per kernel, static).
+struct SharedMemoryOnce {
+    std::atomic<uint64_t> done{0};  // a bit per device; devices beyond 63 ask every time
+    cudaError_t allow(const void* kernel, int bytes) {
+        int device = 0;
+        cudaError_t e = cudaGetDevice(&device);
+        if (e != cudaSuccess) return e;
+        const uint64_t bit = device < 64 ? uint64_t(1) << device : 0;
+        if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+        return e;
+    }
+};
 
 // Rows of a table by token ids and the table's gradient (checked arguments).
 struct EmbeddingArgs {

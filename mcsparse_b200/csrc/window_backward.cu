@@ -571,8 +571,9 @@ cudaError_t launch(cudaStream_t s, const AttentionArgs& a, void* buffer) {
     p.limit = a.wait.limit_cycles, p.fault = a.wait.fault_word;
     delta_kernel<T><<<(unsigned)(((int64_t)a.total_q * a.q_heads + 15) / 16), 256, 0, s>>>(a, delta);
     cudaError_t e = cudaGetLastError();
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(window_backward_kernel<T, DP, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kTotal);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(window_backward_kernel<T, DP, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kTotal);
+    static SharedMemoryOnce once_keys, once_queries;
+    if (e == cudaSuccess) e = once_keys.allow(reinterpret_cast<const void*>(window_backward_kernel<T, DP, true>), S::kTotal);
+    if (e == cudaSuccess) e = once_queries.allow(reinterpret_cast<const void*>(window_backward_kernel<T, DP, false>), S::kTotal);
     if (e != cudaSuccess) return e;
     Params pk = p;
     pk.out1 = a.dv.p, pk.out1_token = a.dv.token, pk.out1_head = a.dv.head;

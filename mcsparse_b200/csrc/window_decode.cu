@@ -399,7 +399,8 @@ cudaError_t launch(cudaStream_t s, const DecodeArgs& a, void* buffer) {
     const int64_t items = decode_items(a);
     if (items * p.splits > 0x7fffffffLL) return cudaErrorInvalidValue;
     if (p.splits > kCluster) p.partial = static_cast<float*>(align_up_256(buffer));
-    cudaError_t e = cudaFuncSetAttribute(window_decode_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<DP>::kTotal);
+    static SharedMemoryOnce once;
+    cudaError_t e = once.allow(reinterpret_cast<const void*>(window_decode_kernel<T, DP>), Ring<DP>::kTotal);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(items * p.splits));

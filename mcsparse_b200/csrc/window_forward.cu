@@ -395,7 +395,8 @@ cudaError_t launch(cudaStream_t s, const AttentionArgs& a) {
     p.scale_log2 = fabsf(a.scale) * kLog2e, p.scale_ln = 1.0f / kLog2e;
     p.o = a.o.p, p.o_token = a.o.token, p.o_head = a.o.head, p.lse = a.lse;
     p.limit = a.wait.limit_cycles, p.fault = a.wait.fault_word;
-    const cudaError_t e = cudaFuncSetAttribute(window_forward_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kTotal);
+    static SharedMemoryOnce once;
+    const cudaError_t e = once.allow(reinterpret_cast<const void*>(window_forward_kernel<T, DP>), S::kTotal);
     if (e != cudaSuccess) return e;
     window_forward_kernel<T, DP><<<(unsigned)((int64_t)p.slots * a.q_heads), kThreads, S::kTotal, s>>>(mq, mk, mv, p);
     return cudaGetLastError();

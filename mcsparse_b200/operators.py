@@ -22,6 +22,9 @@ _HEADS = C.sizeof(capi.Heads)
 _CACHE = C.sizeof(capi.Cache)
 
 
+_GRADIENT_SIZES = {}  # buffer sizes asked for so far, by device, tokens and table
+
+
 def _scalar(handle, value):
     """A float as a C argument: a host scalar, or a one-element fp32 device tensor in device pointer mode."""
     if handle.pointer_mode == capi.MCSPARSE_POINTER_MODE_DEVICE:
@@ -71,10 +74,15 @@ def _buffer(buffer, need):
 
 def embedding_gradient(handle, indices, dY, dE, buffer, alpha=1.0, beta=0.0, base=0):
     """dE = alpha * S^T dY + beta * dE, S the 0/1 matrix of the indices. Indices outside the table contribute nothing."""
-    need = embedding_gradient_buffer_size(handle, indices, dY, dE)
+    key = handle.stream.device_index, indices.numel(), dE.rows, dE.cols
+    need = _GRADIENT_SIZES.get(key)
+    if need is None:
+        if len(_GRADIENT_SIZES) >= 1024:
+            _GRADIENT_SIZES.clear()
+        need = _GRADIENT_SIZES[key] = embedding_gradient_buffer_size(handle, indices, dY, dE)
+    kind = _indices(handle, indices)
     _on_device(handle, indices, dY.values, dE.values, buffer)
-    check(lib.mcsparseB200EmbeddingGradient(handle.h, _scalar(handle, alpha), indices.numel(), indices.data_ptr(), _INDEX[indices.dtype],
-                                            base, dY.d, _scalar(handle, beta), dE.d, _buffer(buffer, need)),
+    check(lib.mcsparseB200EmbeddingGradient(handle.h, _scalar(handle, alpha), indices.numel(), indices.data_ptr(), kind, base, dY.d, _scalar(handle, beta), dE.d, _buffer(buffer, need)),
           "mcsparseB200EmbeddingGradient")
 
 
