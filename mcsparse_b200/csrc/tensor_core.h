@@ -19,6 +19,14 @@ namespace tc {
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 
+// True in one lane of a converged warp, always the same one. (With `lane == 0` in its place the compiler cannot tell that one
+// lane alone issues: every tcgen05.mma then sat in a loop over lanes, 95 to 210 clocks each against 64 of work.)
+__device__ __forceinline__ bool elect() {
+    uint32_t one = 0;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n @p mov.u32 %0, 1;\n}" : "+r"(one));
+    return one != 0;
+}
+
 // ---- mbarriers
 
 __device__ __forceinline__ void bar_init(uint32_t bar, int arrivals) {
@@ -131,6 +139,8 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t column_blo
     d |= (uint64_t)2 << 61;  // 128-byte swizzle
     return d;
 }
+// The descriptor of the operand `bytes` (a multiple of 16) further on.
+__device__ __forceinline__ uint64_t desc_at(uint64_t desc, uint32_t bytes) { return desc + (bytes >> 4); }
 // Instruction descriptor: D (128 x n, fp32) = A * B, bf16 or fp16; b_mn: B is MN-major; negate: A enters with its sign turned.
 __host__ __device__ constexpr uint32_t mma_desc(bool bf16, int n, bool b_mn) {
     return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
@@ -156,11 +166,45 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 
+// ---- fp32 arithmetic
+
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// The larger of three; NaN if one of them is.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+// Two values in one register pair, one instruction for both.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+    uint64_t y;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(lo), "f"(hi));
+    return y;
+}
+__device__ __forceinline__ void unpair(uint64_t x, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(x)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t y;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y) : "l"(a), "l"(b), "l"(c));
+    return y;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t y;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
+    return y;
+}
+// Bits 0 .. n - 1 (none for n <= 0, all for n >= 32).
+__device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
+
+// ---- registers of a warpgroup (all its warps call it): `N` per thread from here on
+
+template <int N>
+__device__ __forceinline__ void registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
 }  // namespace tc
 }  // namespace mcsp_b200

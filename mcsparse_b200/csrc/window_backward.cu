@@ -232,7 +232,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // ---- loads
         if (n > 0) {
             const int hk = KEYS ? head : head / a.group;
-            if (lane == 0) {
+            if (elect()) {
                 bar_expect(bar_fixed, 2 * S::kFixed);
                 const int h1 = head * (KEYS ? a.k_mul : a.q_mul), h2 = head * (KEYS ? a.v_mul : a.go_mul);
                 const int row = (KEYS ? sq.k0 : sq.q0) + row0;
@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     fetch(i + 1);
                     __syncwarp();
                 }
-                if (lane == 0) {
+                if (elect()) {
                     bar_expect(bar_full + 8 * st, 2 * S::kStream);
                     const int h = KEYS ? head * a.group + i / tiles : hk;
                     const int h1 = h * (KEYS ? a.q_mul : a.k_mul), h2 = h * (KEYS ? a.go_mul : a.v_mul);
@@ -320,16 +320,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                     fence_async();
                     __syncwarp();
                 }
-                if (lane == 0) {
+                if (elect()) {
+                    const uint64_t f1 = smem_desc(smem), f2 = smem_desc(smem + S::kFixed), m1 = smem_desc(s1), m2 = smem_desc(s2);
 #pragma unroll
                     for (int k = 0; k < DP / 16; ++k) {
                         const uint32_t fixed = (k >> 2) * (kRows * 128) + (k & 3) * 32, stream = (k >> 2) * (kTile * 128) + (k & 3) * 32;
-                        mma_ss(t_s + kTile * b, smem_desc(smem + fixed), smem_desc(s1 + stream), kDescS | a.negate, k > 0);
+                        mma_ss(t_s + kTile * b, desc_at(f1, fixed), desc_at(m1, stream), kDescS | a.negate, k > 0);
                     }
 #pragma unroll
                     for (int k = 0; k < DP / 16; ++k) {
                         const uint32_t fixed = (k >> 2) * (kRows * 128) + (k & 3) * 32, stream = (k >> 2) * (kTile * 128) + (k & 3) * 32;
-                        mma_ss(t_dp + kTile * b, smem_desc(smem + S::kFixed + fixed), smem_desc(s2 + stream), kDescS, k > 0);
+                        mma_ss(t_dp + kTile * b, desc_at(f2, fixed), desc_at(m2, stream), kDescS, k > 0);
                     }
                     mma_commit(bar_s + 8 * b);
                 }
@@ -342,23 +343,24 @@ __global__ void __launch_bounds__(kThreads, 1)
                     break;
                 }
                 fence_after();
-                if (lane == 0) {
-                    const uint32_t s1 = smem + S::kRing + st * 2 * S::kStream, s2 = s1 + S::kStream;
+                if (elect()) {
+                    const uint32_t s1 = smem + S::kRing + st * 2 * S::kStream;
+                    const uint64_t m1 = smem_desc(s1, kTile * 128), m2 = smem_desc(s1 + S::kStream, kTile * 128);
                     if (KEYS) {
 #pragma unroll
                         for (int k = 0; k < kTile / 16; ++k)
-                            mma_ts(t_out1, t_s + kTile * b + 8 * k, smem_desc(s2 + k * 2048, kTile * 128), kDescOut, i > 1 || k > 0);
+                            mma_ts(t_out1, t_s + kTile * b + 8 * k, desc_at(m2, k * 2048), kDescOut, i > 1 || k > 0);
                     }
 #pragma unroll
                     for (int k = 0; k < kTile / 16; ++k)
-                        mma_ts(KEYS ? t_out2 : t_out1, t_dp + kTile * b + 8 * k, smem_desc(s1 + k * 2048, kTile * 128), kDescOut, i > 1 || k > 0);
+                        mma_ts(KEYS ? t_out2 : t_out1, t_dp + kTile * b + 8 * k, desc_at(m1, k * 2048), kDescOut, i > 1 || k > 0);
                     mma_commit(bar_empty + 8 * st);
                     if (i == n) mma_commit(bar_out);
                 }
                 __syncwarp();
             }
         }
-        if (failed && lane == 0) {  // the tensor memory is given back only when no product uses it any more
+        if (failed && elect()) {  // the tensor memory is given back only when no product uses it any more
             mma_commit(bar_fixed);
             bar_wait(bar_fixed, 1, a.limit);
         }

@@ -22,8 +22,12 @@ using namespace tc;
 
 constexpr int kRows = 128;           // query rows of a tile
 constexpr int kKeys = 128;           // keys of a tile
-constexpr int kSoftmaxThreads = 256;  // two tiles
-constexpr int kThreads = kSoftmaxThreads + 64;  // + the loading warp + the warp that issues the products
+constexpr int kSoftmaxThreads = 256;             // two tiles
+constexpr int kThreads = kSoftmaxThreads + 128;  // + a warpgroup of which one warp loads and one issues the products
+// Registers: 384 threads start with 168 each (64512); the softmax threads hold a row of 128 scores.
+constexpr int kSoftmaxRegisters = 208, kOtherRegisters = 80;
+static_assert(kSoftmaxThreads * kSoftmaxRegisters + 128 * kOtherRegisters <= kThreads * 168, "no more than the block was launched with");
+constexpr int kNarrow = 32;  // a tile of first tokens that holds no more than these is computed 32 columns wide
 constexpr float kLog2e = 1.4426950408889634f;
 // The running reference of a row's exponentials is only moved when its maximum has grown past it by more than 2^8: until
 // then the weights are at most 256 (exact in fp32 sums, far from fp16's 65504) and O needs no rescaling.
@@ -36,7 +40,7 @@ struct Smem {
     static constexpr int kQ = 0;
     static constexpr int kRing = 2 * kTile;
     static constexpr int kBars = kRing + kStages * kTile;
-    static constexpr int kTotal = kBars + 256 + 1024;   // the start is aligned to 1024
+    static constexpr int kTotal = kBars + 256 + 1024;   // (the start is aligned to 1024)
 };
 
 struct Params {
@@ -56,6 +60,7 @@ struct Params {
 struct Visit {
     int rows, p_low, first, low, high;
     __device__ __forceinline__ bool has(int j) const { return j < first || (j >= low && j <= high); }
+    __device__ __forceinline__ bool narrow(int j, int sinks) const { return j < first && sinks - j * kKeys <= kNarrow; }
 };
 __device__ __forceinline__ Visit visit_of(const Sequence& s, int row0, int window, int sinks) {
     Visit v;
@@ -102,6 +107,96 @@ __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+// A thread's running softmax: `ref` is what its exponentials are relative to (base 2), `sum` their sum.
+struct Row {
+    float ref = -INFINITY, sum = 0.0f;
+};
+
+// One tile of NC columns for one thread: scores from tensor memory, maximum, weights back (16 bits, half the columns), O
+// rescaled if the reference moves. EDGE: column c is seen iff c <= above and (c > below or c < keep).
+// half / full: barriers that get this thread's arrival when the first half / all of the weights are in place.
+template <typename T, int DP, int NC, bool EDGE>
+__device__ __forceinline__ void softmax_tile(Row& row, uint32_t t_s, uint32_t t_o, bool rescale, float scale_log2, int above, int below, int keep,
+                                             uint32_t half, uint32_t full) {
+    uint32_t s[NC];
+    float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int c = 0; c < NC && c < 64; c += 32) tmem_load32(t_s + c, s + c);
+#pragma unroll
+    for (int h = 0; h < NC; h += 64) {
+        wait_loads();
+#pragma unroll
+        for (int c = h; c < h + 64 && c < NC; c += 32) after_loads32(s + c);
+        if (h + 64 < NC) {
+#pragma unroll
+            for (int c = h + 64; c < h + 128; c += 32) tmem_load32(t_s + c, s + c);
+        }
+        if (EDGE) {
+#pragma unroll
+            for (int c = h; c < h + 64 && c < NC; c += 32) {
+                // (bits, not comparisons: those became a branch per column, 9000 clocks a tile)
+                const uint32_t seen = low_bits(above + 1 - c) & (~low_bits(below + 1 - c) | low_bits(keep - c));
+#pragma unroll
+                for (int x = 0; x < 32; ++x) s[c + x] = seen >> x & 1 ? s[c + x] : 0xff800000u;
+            }
+        }
+#pragma unroll
+        for (int c = h; c < h + 64 && c < NC; c += 4) {
+            top[0] = max3(top[0], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
+            top[1] = max3(top[1], __uint_as_float(s[c + 2]), __uint_as_float(s[c + 3]));
+        }
+    }
+    float m = max3(top[0], top[1], -INFINITY) * scale_log2;
+    if (m == INFINITY) m = NAN;  // (a row with an infinite or a NaN score is NaN as a whole)
+    const bool move = !(m <= row.ref + kSlack);
+    if (__any_sync(0xffffffffu, move)) {
+        const float next = move ? m : row.ref;
+        const float factor = row.ref == -INFINITY ? 0.0f : exp2_fast(row.ref - next);
+        row.sum *= factor;
+        if (rescale) {
+#pragma unroll 1
+            for (int c = 0; c < DP; c += 32) {
+                uint32_t o[32];
+                tmem_load32(t_o + c, o);
+                wait_loads();
+                after_loads32(o);
+#pragma unroll
+                for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * factor);
+                tmem_store32(t_o + c, o);
+            }
+        }
+        row.ref = next;
+    }
+    const float minus = row.ref == -INFINITY ? 0.0f : -row.ref;
+    const uint64_t minus2 = pair(minus, minus), scale2 = pair(scale_log2, scale_log2);
+    uint64_t part[2] = {pair(0.0f, 0.0f), pair(0.0f, 0.0f)};
+#pragma unroll
+    for (int h = 0; h < NC; h += 64) {
+        uint32_t w[32];
+#pragma unroll
+        for (int c = 0; c < 64 && h + c < NC; c += 2) {
+            const uint64_t x = fma2(pair(__uint_as_float(s[h + c]), __uint_as_float(s[h + c + 1])), scale2, minus2);
+            float e0, e1;
+            unpair(x, e0, e1);
+            e0 = exp2_fast(e0), e1 = exp2_fast(e1);
+            part[(c / 2) & 1] = add2(part[(c / 2) & 1], pair(e0, e1));
+            w[c / 2] = pack2<T>(e0, e1);
+        }
+        if (NC - h >= 64)
+            tmem_store32(t_s + h / 2, w);
+        else
+            tmem_store16(t_s + h / 2, w);
+        wait_stores();
+        fence_before();
+        if (h == 0) bar_arrive(half);
+    }
+    bar_arrive(full);
+    float a, b, c, d;
+    unpair(part[0], a, b);
+    unpair(part[1], c, d);
+    row.sum += (a + b) + (c + d);
+}
+
 template <typename T, int DP>
 __global__ void __launch_bounds__(kThreads, 1)
     window_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
@@ -112,10 +207,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem = (smem_u32(smem_raw) + 1023) & ~1023u;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    // barriers: Q, full[stages], empty[stages], S ready[2], P ready[2], O ready[2]
+    // barriers: Q, full[stages], empty[stages], S ready[2], half of P ready[2], P ready[2], O ready[2]
     const uint32_t bars = smem + S::kBars;
     const uint32_t bar_q = bars, bar_full = bars + 8, bar_empty = bar_full + 8 * S::kStages, bar_s = bar_empty + 8 * S::kStages,
-                   bar_p = bar_s + 16, bar_o = bar_p + 16, slot = bar_o + 16;
+                   bar_h = bar_s + 16, bar_p = bar_h + 16, bar_o = bar_p + 16, slot = bar_o + 16;
 
     const int head = blockIdx.x % a.q_heads;
     const int block = a.slots - 1 - (int)(blockIdx.x / a.q_heads);  // the later rows of a sequence have more to do: first
@@ -131,7 +226,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (threadIdx.x == kSoftmaxThreads) {
         bar_init(bar_q, 1);
         for (int i = 0; i < S::kStages; ++i) bar_init(bar_full + 8 * i, 1), bar_init(bar_empty + 8 * i, 1);
-        for (int i = 0; i < 2; ++i) bar_init(bar_s + 8 * i, 1), bar_init(bar_p + 8 * i, kRows), bar_init(bar_o + 8 * i, 1);
+        for (int i = 0; i < 2; ++i) bar_init(bar_s + 8 * i, 1), bar_init(bar_h + 8 * i, kRows), bar_init(bar_p + 8 * i, kRows), bar_init(bar_o + 8 * i, 1);
         bar_init_fence();
     }
     fence_before();
@@ -143,9 +238,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t t_s[2] = {tmem, tmem + 128}, t_o[2] = {tmem + 256, tmem + 256 + DP};
     bool failed = false;
 
-    if (warp == 8) {
+    if (warp >= kSoftmaxThreads / 32) {
+      registers_down<kOtherRegisters>();
+      if (warp == 8) {
         // ---- loads
-        if (lane == 0 && order.n > 0) {
+        if (order.n > 0 && elect()) {
             const int hk = head / a.group;
             bar_expect(bar_q, 2 * S::kTile);
             for (int t = 0; t < 2; ++t)
@@ -174,9 +271,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
         __syncwarp();
-    } else if (warp == 9) {
+      } else if (warp == 9) {
         // ---- products
-        constexpr uint32_t kDescS = mma_desc(kBf16, kKeys, false), kDescO = mma_desc(kBf16, DP, true);
+        constexpr uint32_t kDescS = mma_desc(kBf16, kKeys, false), kDescNarrow = mma_desc(kBf16, kNarrow, false), kDescO = mma_desc(kBf16, DP, true);
         const int first_seen = max(va.rows > 0 ? va.p_low - a.window + 1 : 0, 0);
         const int last_seen = min(sq.lk, sq.lk - sq.lq + min(row0 + 2 * kRows, sq.lq)) - 1;
         int n_p[2] = {0, 0};  // P tiles taken
@@ -216,54 +313,71 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int t = 0; t < 2; ++t) {
                     const Visit& v = t == 0 ? va : vb;
                     if (i > 0 && v.has(before)) {
+                        if (!bar_wait_warp(bar_h + 8 * t, n_p[t] & 1, a.limit)) {
+                            failed = true;
+                            break;
+                        }
+                        fence_after();
+                        const bool narrow = v.narrow(before, a.sinks);
+                        const uint64_t values = smem_desc(smem + S::kRing + st_v * S::kTile, kKeys * 128);
+                        if (elect()) {
+#pragma unroll
+                            for (int k = 0; k < kKeys / 32; ++k)
+                                if (k < kNarrow / 16 || !narrow)
+                                    mma_ts(t_o[t], t_s[t] + 8 * k, desc_at(values, k * 2048), kDescO, n_p[t] > 0 || k > 0);
+                        }
                         if (!bar_wait_warp(bar_p + 8 * t, n_p[t] & 1, a.limit)) {
                             failed = true;
                             break;
                         }
                         fence_after();
-                        if (lane == 0) {
-                            const uint32_t base = smem + S::kRing + st_v * S::kTile;
+                        if (elect()) {
+                            if (!narrow) {
 #pragma unroll
-                            for (int k = 0; k < kKeys / 16; ++k)
-                                mma_ts(t_o[t], t_s[t] + 8 * k, smem_desc(base + k * 2048, kKeys * 128), kDescO, n_p[t] > 0 || k > 0);
+                                for (int k = kKeys / 32; k < kKeys / 16; ++k)
+                                    mma_ts(t_o[t], t_s[t] + 8 * k, desc_at(values, k * 2048), kDescO, true);
+                            }
                             if (before == v.high) mma_commit(bar_o + 8 * t);
                         }
                         ++n_p[t];
                         __syncwarp();
                     }
                     if (i < n && v.has(j)) {
-                        if (lane == 0) {
-                            const uint32_t qb = smem + S::kQ + t * S::kTile, kb = smem + S::kRing + st_k * S::kTile;
+                        if (elect()) {
+                            const uint32_t desc = (v.narrow(j, a.sinks) ? kDescNarrow : kDescS) | a.negate;
+                            const uint64_t q = smem_desc(smem + S::kQ + t * S::kTile), k = smem_desc(smem + S::kRing + st_k * S::kTile);
 #pragma unroll
-                            for (int k = 0; k < DP / 16; ++k) {
-                                const uint32_t off = (k >> 2) * (kRows * 128) + (k & 3) * 32;
-                                mma_ss(t_s[t], smem_desc(qb + off), smem_desc(kb + off), kDescS | a.negate, k > 0);
+                            for (int x = 0; x < DP / 16; ++x) {
+                                const uint32_t off = (x >> 2) * (kRows * 128) + (x & 3) * 32;
+                                mma_ss(t_s[t], desc_at(q, off), desc_at(k, off), desc, x > 0);
                             }
                             mma_commit(bar_s + 8 * t);
                         }
                         __syncwarp();
                     }
                 }
-                if (lane == 0 && !failed) {
+                if (!failed && elect()) {
                     if (i > 0) mma_commit(bar_empty + 8 * st_v);
                     if (i < n) mma_commit(bar_empty + 8 * st_k);
                 }
                 __syncwarp();
             }
         }
-        if (failed && lane == 0) {  // the tensor memory is given back only when no product uses it any more
+        if (failed && elect()) {  // the tensor memory is given back only when no product uses it any more
             mma_commit(bar_q);
             bar_wait(bar_q, 1, a.limit);
         }
         __syncwarp();
+      }
     } else {
         // ---- softmax: thread = row
+        registers_up<kSoftmaxRegisters>();
         const int t = warp >> 2;
         const Visit v = t == 0 ? va : vb;
         const int r = threadIdx.x & (kRows - 1);
         const int p = v.p_low + r;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // tensor-memory lane of the warp's first row
-        float ref = -INFINITY, sum = 0.0f;
+        Row row;
         int done = 0;
         for (int i = 0; i < order.n; ++i) {
             const int j = order.tile(i);
@@ -273,65 +387,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                 break;
             }
             fence_after();
-            uint32_t s[kKeys];
-#pragma unroll
-            for (int c = 0; c < kKeys; c += 32) tmem_load32(t_s[t] + lanes + c, s + c);
-            wait_loads();
-#pragma unroll
-            for (int c = 0; c < kKeys; c += 32) after_loads32(s + c);
-            const int key0 = j * kKeys;
-            const int last_p = v.p_low + kRows - 1;
-            if (key0 + kKeys - 1 > v.p_low || (key0 <= last_p - a.window && key0 + kKeys > a.sinks)) {
-                // column c is seen iff c <= above and (c > below or c < keep)
-                const int above = p - key0, below = p - key0 - a.window, keep = a.sinks - key0;
-#pragma unroll
-                for (int c = 0; c < kKeys; ++c)
-                    if (!(c <= above && (c > below || c < keep))) s[c] = 0xff800000u;
-            }
-            float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-            for (int c = 0; c < kKeys; c += 4)
-#pragma unroll
-                for (int x = 0; x < 4; ++x) top[x] = fmaxf(top[x], __uint_as_float(s[c + x]));
-            const float m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2;
-            const bool move = m > ref + kSlack || (ref == -INFINITY && m > ref);
-            if (__any_sync(0xffffffffu, move)) {
-                const float next = move ? m : ref;
-                const float factor = ref == -INFINITY ? 0.0f : exp2_fast(ref - next);
-                sum *= factor;
-                if (done > 0) {
-#pragma unroll 1
-                    for (int c = 0; c < DP; c += 32) {
-                        uint32_t o[32];
-                        tmem_load32(t_o[t] + lanes + c, o);
-                        wait_loads();
-                        after_loads32(o);
-#pragma unroll
-                        for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * factor);
-                        tmem_store32(t_o[t] + lanes + c, o);
-                    }
-                }
-                ref = next;
-            }
-            const float minus = ref == -INFINITY ? 0.0f : -ref;
-            float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                uint32_t w[32];
-#pragma unroll
-                for (int c = 0; c < 64; c += 2) {
-                    const float x = exp2_fast(fmaf(__uint_as_float(s[64 * h + c]), a.scale_log2, minus));
-                    const float y = exp2_fast(fmaf(__uint_as_float(s[64 * h + c + 1]), a.scale_log2, minus));
-                    part[c & 2] += x;
-                    part[(c & 2) + 1] += y;
-                    w[c >> 1] = pack2<T>(x, y);
-                }
-                tmem_store32(t_s[t] + lanes + 32 * h, w);
-            }
-            sum += (part[0] + part[1]) + (part[2] + part[3]);
-            wait_stores();
-            fence_before();
-            bar_arrive(bar_p + 8 * t);
+            const int key0 = j * kKeys, last_p = v.p_low + kRows - 1;
+            const uint32_t ts = t_s[t] + lanes, to = t_o[t] + lanes, half = bar_h + 8 * t, full = bar_p + 8 * t;
+            const int above = p - key0, below = p - key0 - a.window, keep = a.sinks - key0;
+            if (v.narrow(j, a.sinks))
+                softmax_tile<T, DP, kNarrow, true>(row, ts, to, done > 0, a.scale_log2, above, below, keep, half, full);
+            else if (key0 + kKeys - 1 > v.p_low || (key0 <= last_p - a.window && key0 + kKeys > a.sinks))
+                softmax_tile<T, DP, kKeys, true>(row, ts, to, done > 0, a.scale_log2, above, below, keep, half, full);
+            else
+                softmax_tile<T, DP, kKeys, false>(row, ts, to, done > 0, a.scale_log2, 0, 0, 0, half, full);
             ++done;
         }
         // ---- epilogue
@@ -339,11 +403,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             failed = !bar_wait_warp(bar_o + 8 * t, 0, a.limit);
             fence_after();
         }
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        const int64_t row = (int64_t)sq.q0 + row0 + t * kRows + r;
+        const float inv = row.sum == 0.0f ? 0.0f : 1.0f / row.sum;
+        const int64_t token = (int64_t)sq.q0 + row0 + t * kRows + r;
         if (a.lse != nullptr && r < v.rows)
-            a.lse[(int64_t)head * a.total_q + row] = sum == 0.0f ? -INFINITY : ref * a.scale_ln + logf(sum);
-        T* out = static_cast<T*>(a.o) + row * a.o_token + (int64_t)head * a.o_head;
+            a.lse[(int64_t)head * a.total_q + token] = row.sum == 0.0f ? -INFINITY : row.ref * a.scale_ln + logf(row.sum);
+        T* out = static_cast<T*>(a.o) + token * a.o_token + (int64_t)head * a.o_head;
 #pragma unroll 1
         for (int c = 0; c < DP; c += 32) {
             uint32_t o[32];
@@ -357,7 +421,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int x = 0; x < 32; x += 8) {
                     if (c + x < a.dim) {
                         uint4 w = make_uint4(0, 0, 0, 0);
-                        if (sum != 0.0f) {
+                        if (row.sum != 0.0f) {
                             w.x = pack2<T>(__uint_as_float(o[x]) * inv, __uint_as_float(o[x + 1]) * inv);
                             w.y = pack2<T>(__uint_as_float(o[x + 2]) * inv, __uint_as_float(o[x + 3]) * inv);
                             w.z = pack2<T>(__uint_as_float(o[x + 4]) * inv, __uint_as_float(o[x + 5]) * inv);
