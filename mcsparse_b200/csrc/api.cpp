@@ -173,14 +173,8 @@ WaitCfg wait_cfg(const mcsparseContext* h) {
     return w;
 }
 
-// A tile kernel of an earlier call on this handle gave up its bounded wait: reported once, by the
-// next compute call, as an execution failure (the word lives in pinned host memory the kernels can
-// write, so reading it needs no synchronisation).
 bool take_device_fault(mcsparseContext* h) {
-    if (h->fault_word_host == nullptr || *reinterpret_cast<volatile int*>(h->fault_word_host) == 0) return false;
-    *reinterpret_cast<volatile int*>(h->fault_word_host) = 0;
-    log_error("an earlier SpMV on this handle gave up a bounded device-side wait; its result is incomplete");
-    return true;
+    return api::take_device_fault(h, "an earlier call on this handle gave up a bounded device-side wait; its result is incomplete");
 }
 
 struct PushArgs {

@@ -22,6 +22,10 @@ ScalarArg<float> scalar(const mcsparseContext* h, const void* p) {
     return a;
 }
 
+bool gave_up(mcsparseContext* h) {
+    return take_device_fault(h, "an earlier call on this handle gave up a bounded device-side wait; its result is incomplete");
+}
+
 // ----------------------------------------------------------------------------- embedding
 
 // table: E or dE (rows x width); tokens: Y or dY (count x width).
@@ -222,6 +226,7 @@ mcsparseStatus_t mcsparseB200WindowAttention(mcsparseHandle_t handle, mcsparseB2
     if (st != OK) return pub(st);
     if (misaligned(lse, 4)) return pub(BAD_VALUE);
     a.q = tensor(q), a.k = tensor(k), a.v = tensor(v), a.o = tensor(o), a.lse = lse;
+    if (gave_up(handle)) return pub(EXEC_FAILED);
     DeviceGuard guard(handle->device);
     return pub(from_cuda(window_attention(handle->stream, a)));
 }
@@ -254,6 +259,7 @@ mcsparseStatus_t mcsparseB200WindowAttentionBackward(
     if (misaligned(lse, 4)) return pub(BAD_VALUE);
     a.q = tensor(q), a.k = tensor(k), a.v = tensor(v), a.o = tensor(o), a.lse = const_cast<float*>(lse);
     a.d_o = tensor(dO), a.dq = tensor(dQ), a.dk = tensor(dK), a.dv = tensor(dV);
+    if (gave_up(handle)) return pub(EXEC_FAILED);
     DeviceGuard guard(handle->device);
     return pub(from_cuda(window_attention_backward(handle->stream, a, externalBuffer)));
 }

@@ -27,6 +27,12 @@ __device__ __forceinline__ bool elect() {
     return one != 0;
 }
 
+// A value that is the same in all lanes of a converged warp, in a form that lets the compiler know it: tcgen05.mma takes its
+// operands from uniform registers, and values it cannot prove uniform (loaded ones, and counters of loops whose ends depend on
+// them) were moved there anew for every instruction, 75 to 100 clocks each.
+__device__ __forceinline__ int uniform(int x) { return __reduce_max_sync(0xffffffffu, x); }
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __reduce_max_sync(0xffffffffu, x); }
+
 // ---- mbarriers
 
 __device__ __forceinline__ void bar_init(uint32_t bar, int arrivals) {
@@ -57,6 +63,8 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, long lon
     return true;
 }
 
+// Limit (SM clocks, about a second) of the waits with which a block that gave up lets its copies and products end.
+constexpr long long kDrain = 2000000000;
 // The same for a whole warp: one answer for all lanes.
 __device__ __forceinline__ bool bar_wait_warp(uint32_t bar, uint32_t parity, long long limit) {
     return __all_sync(0xffffffffu, bar_wait(bar, parity, limit));
@@ -106,6 +114,15 @@ __device__ __forceinline__ void after_loads32(uint32_t* r) {
     asm volatile("" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
                  "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]),
                  "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]));
+}
+__device__ __forceinline__ void tmem_load16(uint32_t addr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(addr));
+}
+__device__ __forceinline__ void after_loads16(uint32_t* r) {
+    asm volatile("" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]));
 }
 __device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t* r) {
     asm volatile(
@@ -198,13 +215,6 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
 }
 // Bits 0 .. n - 1 (none for n <= 0, all for n >= 32).
 __device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
-
-// ---- registers of a warpgroup (all its warps call it): `N` per thread from here on
-
-template <int N>
-__device__ __forceinline__ void registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N>
-__device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
 }  // namespace tc
 }  // namespace mcsp_b200

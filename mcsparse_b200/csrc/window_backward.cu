@@ -287,8 +287,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 issued = i + 1;
             }
             if (failed) {  // nothing of this block's memory is given back while a copy is on its way
-                bar_wait(bar_fixed, 0, a.limit);
-                for (int i = max(0, issued - kStages); i < issued; ++i) bar_wait(bar_full + 8 * (i % kStages), (i / kStages) & 1, a.limit);
+                bar_wait(bar_fixed, 0, kDrain);
+                for (int i = max(0, issued - kStages); i < issued; ++i) bar_wait(bar_full + 8 * (i % kStages), (i / kStages) & 1, kDrain);
             }
         }
         __syncwarp();
@@ -362,7 +362,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (failed && elect()) {  // the tensor memory is given back only when no product uses it any more
             mma_commit(bar_fixed);
-            bar_wait(bar_fixed, 1, a.limit);
+            bar_wait(bar_fixed, 1, kDrain);
         }
         __syncwarp();
     } else {

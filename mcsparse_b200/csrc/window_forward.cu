@@ -1,13 +1,14 @@
 // Windowed attention forward on the tensor cores (fp16 / bf16, rows of 16-byte multiples).
 //
 // One thread block takes 256 consecutive queries of a sequence and one query head: two tiles of 128 rows that share every
-// key tile of 128. S = Q K^T and O += P V are tcgen05.mma with S, P and O in tensor memory (P overwrites its S, half as
-// wide); the tensor cores work on one tile's products while the other tile's 128 threads, one row each, take the row's
-// maximum, exponentials and sum in registers. Key tiles outside window and first tokens are never loaded; a tile needs its
-// mask only at an edge of the pattern.
+// key tile of 64. S = Q K^T and O += P V are tcgen05.mma with S, P and O in tensor memory (P overwrites its S, half as
+// wide); 128 threads per row tile, one row each, take maximum, exponentials and sum in registers. S has two buffers per row
+// tile: the next scores are there when a tile's weights are done, so the chain scores -> weights -> O -> next scores of a
+// single buffer (3300 clocks per 128 keys of both row tiles) is cut. Key tiles outside window and first tokens are never
+// loaded; a tile needs its mask only at an edge of the pattern.
 //
-// Bound by the tensor cores and, about equally at headDim 128, by the exponentials (16 per clock and SM): 128 x 128 x 128
-// takes 512 clocks twice and 1024 clocks of exponentials.
+// Bounds at headDim 128, clocks per 128 keys and both row tiles: products 2560 (Q K^T with 64 keys reads 6 KB of shared memory
+// per 32 clocks of arithmetic and takes 48; P V reads P from tensor memory: 64), exponentials 2048 (16 per clock).
 #include <type_traits>
 
 #include "tensor_core.h"
@@ -21,13 +22,10 @@ using namespace window;
 using namespace tc;
 
 constexpr int kRows = 128;           // query rows of a tile
-constexpr int kKeys = 128;           // keys of a tile
-constexpr int kSoftmaxThreads = 256;             // two tiles
-constexpr int kThreads = kSoftmaxThreads + 128;  // + a warpgroup of which one warp loads and one issues the products
-// Registers: 384 threads start with 168 each (64512); the softmax threads hold a row of 128 scores.
-constexpr int kSoftmaxRegisters = 208, kOtherRegisters = 80;
-static_assert(kSoftmaxThreads * kSoftmaxRegisters + 128 * kOtherRegisters <= kThreads * 168, "no more than the block was launched with");
-constexpr int kNarrow = 32;  // a tile of first tokens that holds no more than these is computed 32 columns wide
+constexpr int kKeys = 64;            // keys of a tile
+constexpr int kSoftmaxWarps = 8;     // two row tiles
+constexpr int kLoadWarp = kSoftmaxWarps, kScoreWarp = kSoftmaxWarps + 1, kValueWarp = kSoftmaxWarps + 2, kClearWarp = kSoftmaxWarps + 3;
+constexpr int kThreads = 32 * (kSoftmaxWarps + 4);
 constexpr float kLog2e = 1.4426950408889634f;
 // The running reference of a row's exponentials is only moved when its maximum has grown past it by more than 2^8: until
 // then the weights are at most 256 (exact in fp32 sums, far from fp16's 65504) and O needs no rescaling.
@@ -35,12 +33,14 @@ constexpr float kSlack = 8.0f;
 
 template <int DP>
 struct Smem {
-    static constexpr int kTile = 128 * DP * 2;          // bytes of a 128-row operand
-    static constexpr int kStages = DP == 128 ? 5 : 8;   // key and value tiles in turn
+    static constexpr int kQuery = kRows * DP * 2;        // bytes of a query tile
+    static constexpr int kTile = kKeys * DP * 2;          // of a tile of keys, or of values
+    static constexpr int kStages = DP == 128 ? 5 : 8;     // of a key tile and a value tile each
     static constexpr int kQ = 0;
-    static constexpr int kRing = 2 * kTile;
-    static constexpr int kBars = kRing + kStages * kTile;
-    static constexpr int kTotal = kBars + 256 + 1024;   // (the start is aligned to 1024)
+    static constexpr int kRing = 2 * kQuery;
+    static constexpr int kBars = kRing + kStages * 2 * kTile;
+    static constexpr int kTotal = kBars + 512 + 1024;     // (the start is aligned to 1024)
+    static_assert(kTotal <= 227 * 1024, "shared memory of a block");
 };
 
 struct Params {
@@ -59,8 +59,8 @@ struct Params {
 // What one tile of 128 rows has to visit: key tiles [0, first) and [low, high].
 struct Visit {
     int rows, p_low, first, low, high;
+    __device__ __forceinline__ Visit same() const { return Visit{uniform(rows), uniform(p_low), uniform(first), uniform(low), uniform(high)}; }
     __device__ __forceinline__ bool has(int j) const { return j < first || (j >= low && j <= high); }
-    __device__ __forceinline__ bool narrow(int j, int sinks) const { return j < first && sinks - j * kKeys <= kNarrow; }
 };
 __device__ __forceinline__ Visit visit_of(const Sequence& s, int row0, int window, int sinks) {
     Visit v;
@@ -80,6 +80,7 @@ __device__ __forceinline__ Visit visit_of(const Sequence& s, int row0, int windo
 // The key tiles of a block in the order they are visited: [0, first), then [low, high].
 struct Order {
     int first, low, n;
+    __device__ __forceinline__ Order same() const { return Order{uniform(first), uniform(low), uniform(n)}; }
     __device__ __forceinline__ int tile(int i) const { return i < first ? i : low + (i - first); }
 };
 __device__ __forceinline__ Order order_of(const Visit& a, const Visit& b) {
@@ -112,38 +113,30 @@ struct Row {
     float ref = -INFINITY, sum = 0.0f;
 };
 
-// One tile of NC columns for one thread: scores from tensor memory, maximum, weights back (16 bits, half the columns), O
-// rescaled if the reference moves. EDGE: column c is seen iff c <= above and (c > below or c < keep).
-// half / full: barriers that get this thread's arrival when the first half / all of the weights are in place.
-template <typename T, int DP, int NC, bool EDGE>
-__device__ __forceinline__ void softmax_tile(Row& row, uint32_t t_s, uint32_t t_o, bool rescale, float scale_log2, int above, int below, int keep,
-                                             uint32_t half, uint32_t full) {
-    uint32_t s[NC];
+// One tile for one thread: scores from tensor memory, maximum, weights back (16 bits, half the columns). EDGE: column c is seen
+// iff c <= above and (c > below or c < keep). `before` waits for the products with the tiles before this one; then O is
+// rescaled if the reference moves. False: that wait ran out.
+template <typename T, int DP, bool EDGE, typename Before>
+__device__ __forceinline__ bool softmax_tile(Row& row, uint32_t t_s, uint32_t t_o, bool rescale, float scale_log2, int above, int below, int keep,
+                                             uint32_t ready, Before before) {
+    uint32_t s[kKeys];
     float top[2] = {-INFINITY, -INFINITY};
+    tmem_load32(t_s, s);
+    tmem_load32(t_s + 32, s + 32);
+    wait_loads();
 #pragma unroll
-    for (int c = 0; c < NC && c < 64; c += 32) tmem_load32(t_s + c, s + c);
-#pragma unroll
-    for (int h = 0; h < NC; h += 64) {
-        wait_loads();
-#pragma unroll
-        for (int c = h; c < h + 64 && c < NC; c += 32) after_loads32(s + c);
-        if (h + 64 < NC) {
-#pragma unroll
-            for (int c = h + 64; c < h + 128; c += 32) tmem_load32(t_s + c, s + c);
-        }
+    for (int c = 0; c < kKeys; c += 32) {
+        after_loads32(s + c);
         if (EDGE) {
+            // (bits, not comparisons: those became a branch per column, 9000 clocks for 128 of them)
+            const uint32_t seen = low_bits(above + 1 - c) & (~low_bits(below + 1 - c) | low_bits(keep - c));
 #pragma unroll
-            for (int c = h; c < h + 64 && c < NC; c += 32) {
-                // (bits, not comparisons: those became a branch per column, 9000 clocks a tile)
-                const uint32_t seen = low_bits(above + 1 - c) & (~low_bits(below + 1 - c) | low_bits(keep - c));
-#pragma unroll
-                for (int x = 0; x < 32; ++x) s[c + x] = seen >> x & 1 ? s[c + x] : 0xff800000u;
-            }
+            for (int x = 0; x < 32; ++x) s[c + x] = seen >> x & 1 ? s[c + x] : 0xff800000u;
         }
 #pragma unroll
-        for (int c = h; c < h + 64 && c < NC; c += 4) {
-            top[0] = max3(top[0], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
-            top[1] = max3(top[1], __uint_as_float(s[c + 2]), __uint_as_float(s[c + 3]));
+        for (int x = 0; x < 32; x += 4) {
+            top[0] = max3(top[0], __uint_as_float(s[c + x]), __uint_as_float(s[c + x + 1]));
+            top[1] = max3(top[1], __uint_as_float(s[c + x + 2]), __uint_as_float(s[c + x + 3]));
         }
     }
     float m = max3(top[0], top[1], -INFINITY) * scale_log2;
@@ -154,6 +147,7 @@ __device__ __forceinline__ void softmax_tile(Row& row, uint32_t t_s, uint32_t t_
         const float factor = row.ref == -INFINITY ? 0.0f : exp2_fast(row.ref - next);
         row.sum *= factor;
         if (rescale) {
+            if (!before()) return false;
 #pragma unroll 1
             for (int c = 0; c < DP; c += 32) {
                 uint32_t o[32];
@@ -170,31 +164,24 @@ __device__ __forceinline__ void softmax_tile(Row& row, uint32_t t_s, uint32_t t_
     const float minus = row.ref == -INFINITY ? 0.0f : -row.ref;
     const uint64_t minus2 = pair(minus, minus), scale2 = pair(scale_log2, scale_log2);
     uint64_t part[2] = {pair(0.0f, 0.0f), pair(0.0f, 0.0f)};
+    uint32_t w[32];
 #pragma unroll
-    for (int h = 0; h < NC; h += 64) {
-        uint32_t w[32];
-#pragma unroll
-        for (int c = 0; c < 64 && h + c < NC; c += 2) {
-            const uint64_t x = fma2(pair(__uint_as_float(s[h + c]), __uint_as_float(s[h + c + 1])), scale2, minus2);
-            float e0, e1;
-            unpair(x, e0, e1);
-            e0 = exp2_fast(e0), e1 = exp2_fast(e1);
-            part[(c / 2) & 1] = add2(part[(c / 2) & 1], pair(e0, e1));
-            w[c / 2] = pack2<T>(e0, e1);
-        }
-        if (NC - h >= 64)
-            tmem_store32(t_s + h / 2, w);
-        else
-            tmem_store16(t_s + h / 2, w);
-        wait_stores();
-        fence_before();
-        if (h == 0) bar_arrive(half);
+    for (int c = 0; c < kKeys; c += 2) {
+        float e0, e1;
+        unpair(fma2(pair(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), scale2, minus2), e0, e1);
+        e0 = exp2_fast(e0), e1 = exp2_fast(e1);
+        part[(c / 2) & 1] = add2(part[(c / 2) & 1], pair(e0, e1));
+        w[c / 2] = pack2<T>(e0, e1);
     }
-    bar_arrive(full);
+    tmem_store32(t_s, w);
+    wait_stores();
+    fence_before();
+    bar_arrive(ready);
     float a, b, c, d;
     unpair(part[0], a, b);
     unpair(part[1], c, d);
     row.sum += (a + b) + (c + d);
+    return true;
 }
 
 template <typename T, int DP>
@@ -206,11 +193,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr int kBlocks = DP / 64;  // 64-value column blocks of an operand
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem = (smem_u32(smem_raw) + 1023) & ~1023u;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    // barriers: Q, full[stages], empty[stages], S ready[2], half of P ready[2], P ready[2], O ready[2]
+    const int warp = uniform((int)(threadIdx.x >> 5)), lane = threadIdx.x & 31;
+    // barriers: Q; of every stage: keys there, values there, values clear, stage done with; of the row tiles' two buffers each:
+    // S ready, P ready, product with the values done; the ends of the two issuing warps
     const uint32_t bars = smem + S::kBars;
-    const uint32_t bar_q = bars, bar_full = bars + 8, bar_empty = bar_full + 8 * S::kStages, bar_s = bar_empty + 8 * S::kStages,
-                   bar_h = bar_s + 16, bar_p = bar_h + 16, bar_o = bar_p + 16, slot = bar_o + 16;
+    const uint32_t bar_q = bars, bar_k = bars + 8, bar_v = bar_k + 8 * S::kStages, bar_clear = bar_v + 8 * S::kStages,
+                   bar_done = bar_clear + 8 * S::kStages, bar_s = bar_done + 8 * S::kStages, bar_p = bar_s + 32, bar_o = bar_p + 32,
+                   bar_end = bar_o + 32, slot = bar_end + 16;
 
     const int head = blockIdx.x % a.q_heads;
     const int block = a.slots - 1 - (int)(blockIdx.x / a.q_heads);  // the later rows of a sequence have more to do: first
@@ -218,15 +207,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     const Sequence sq = rb.b < 0 ? Sequence{0, 0, 0, 0} : sequence_of(a.r, rb.b);
     if (rb.b < 0 || (int64_t)rb.index * 2 * kRows >= sq.lq) return;  // (the same for the whole block)
     const int row0 = rb.index * 2 * kRows;
-    const Visit va = visit_of(sq, row0, a.window, a.sinks), vb = visit_of(sq, row0 + kRows, a.window, a.sinks);
-    const Order order = order_of(va, vb);
+    const Visit va = visit_of(sq, row0, a.window, a.sinks).same(), vb = visit_of(sq, row0 + kRows, a.window, a.sinks).same();
+    const Order order = order_of(va, vb).same();
 
-    if (warp == 9) {
+    if (warp == kValueWarp) {
         tmem_alloc(slot, 512);
-    } else if (threadIdx.x == kSoftmaxThreads) {
+    } else if (threadIdx.x == 32 * kLoadWarp) {
         bar_init(bar_q, 1);
-        for (int i = 0; i < S::kStages; ++i) bar_init(bar_full + 8 * i, 1), bar_init(bar_empty + 8 * i, 1);
-        for (int i = 0; i < 2; ++i) bar_init(bar_s + 8 * i, 1), bar_init(bar_h + 8 * i, kRows), bar_init(bar_p + 8 * i, kRows), bar_init(bar_o + 8 * i, 1);
+        for (int i = 0; i < 4 * S::kStages; ++i) bar_init(bar_k + 8 * i, 1);
+        for (int i = 0; i < 4; ++i) bar_init(bar_s + 8 * i, 1), bar_init(bar_p + 8 * i, kRows), bar_init(bar_o + 8 * i, 1);
+        for (int i = 0; i < 2; ++i) bar_init(bar_end + 8 * i, 1);
         bar_init_fence();
     }
     fence_before();
@@ -234,174 +224,187 @@ __global__ void __launch_bounds__(kThreads, 1)
     fence_after();
     uint32_t tmem;
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(slot));
-    // tensor memory: S (and P) of the two tiles, O of the two tiles
-    const uint32_t t_s[2] = {tmem, tmem + 128}, t_o[2] = {tmem + 256, tmem + 256 + DP};
+    tmem = uniform(tmem);
+    // tensor memory: S (and P) of the two row tiles, two buffers each; O of the two row tiles
+    const uint32_t t_s = tmem, t_o = tmem + 4 * kKeys;
     bool failed = false;
 
-    if (warp >= kSoftmaxThreads / 32) {
-      registers_down<kOtherRegisters>();
-      if (warp == 8) {
+    if (warp == kLoadWarp) {
         // ---- loads
         if (order.n > 0 && elect()) {
             const int hk = head / a.group;
-            bar_expect(bar_q, 2 * S::kTile);
+            bar_expect(bar_q, 2 * S::kQuery);
             for (int t = 0; t < 2; ++t)
                 for (int c = 0; c < kBlocks; ++c)
-                    tma_load_3d(smem + S::kQ + t * S::kTile + c * (kRows * 128), &map_q, 64 * c, head * a.q_mul,
-                                sq.q0 + row0 + t * kRows, bar_q);
+                    tma_load_3d(smem + S::kQ + t * S::kQuery + c * (kRows * 128), &map_q, 64 * c, head * a.q_mul, sq.q0 + row0 + t * kRows, bar_q);
             int issued = 0;
-            for (int i = 0; i < 2 * order.n; ++i) {
+            for (int i = 0; i < order.n; ++i) {
                 const int st = i % S::kStages;
-                if (i >= S::kStages && !bar_wait(bar_empty + 8 * st, (i / S::kStages - 1) & 1, a.limit)) {
+                if (i >= S::kStages && !bar_wait(bar_done + 8 * st, (i / S::kStages - 1) & 1, a.limit)) {
                     failed = true;
                     break;
                 }
-                bar_expect(bar_full + 8 * st, S::kTile);
-                const int key = sq.k0 + order.tile(i >> 1) * kKeys;
-                for (int c = 0; c < kBlocks; ++c)
-                    tma_load_3d(smem + S::kRing + st * S::kTile + c * (kKeys * 128), (i & 1) ? &map_v : &map_k, 64 * c,
-                                hk * ((i & 1) ? a.v_mul : a.k_mul), key, bar_full + 8 * st);
+                const uint32_t to = smem + S::kRing + st * 2 * S::kTile;
+                const int key = sq.k0 + order.tile(i) * kKeys;
+                bar_expect(bar_k + 8 * st, S::kTile);
+                for (int c = 0; c < kBlocks; ++c) tma_load_3d(to + c * (kKeys * 128), &map_k, 64 * c, hk * a.k_mul, key, bar_k + 8 * st);
+                bar_expect(bar_v + 8 * st, S::kTile);
+                for (int c = 0; c < kBlocks; ++c) tma_load_3d(to + S::kTile + c * (kKeys * 128), &map_v, 64 * c, hk * a.v_mul, key, bar_v + 8 * st);
                 issued = i + 1;
             }
             // nothing of this block's memory is given back while a copy is on its way
             if (failed) {
-                bar_wait(bar_q, 0, a.limit);
-                for (int i = max(0, issued - S::kStages); i < issued; ++i)
-                    bar_wait(bar_full + 8 * (i % S::kStages), (i / S::kStages) & 1, a.limit);
+                bar_wait(bar_q, 0, kDrain);
+                for (int i = max(0, issued - S::kStages); i < issued; ++i) {
+                    bar_wait(bar_k + 8 * (i % S::kStages), (i / S::kStages) & 1, kDrain);
+                    bar_wait(bar_v + 8 * (i % S::kStages), (i / S::kStages) & 1, kDrain);
+                }
             }
         }
         __syncwarp();
-      } else if (warp == 9) {
-        // ---- products
-        constexpr uint32_t kDescS = mma_desc(kBf16, kKeys, false), kDescNarrow = mma_desc(kBf16, kNarrow, false), kDescO = mma_desc(kBf16, DP, true);
-        const int first_seen = max(va.rows > 0 ? va.p_low - a.window + 1 : 0, 0);
-        const int last_seen = min(sq.lk, sq.lk - sq.lq + min(row0 + 2 * kRows, sq.lq)) - 1;
-        int n_p[2] = {0, 0};  // P tiles taken
-        const int n = order.n;
-        if (n > 0) {
-            failed = !bar_wait_warp(bar_q, 0, a.limit);
-            for (int i = 0; i <= n && !failed; ++i) {
-                const int j = i < n ? order.tile(i) : 0, before = i > 0 ? order.tile(i - 1) : 0;
-                const int st_k = (2 * i) % S::kStages, st_v = (2 * i - 1 + S::kStages) % S::kStages;
-                if (i > 0) {
-                    if (!bar_wait_warp(bar_full + 8 * st_v, ((2 * i - 1) / S::kStages) & 1, a.limit)) {
-                        failed = true;
-                        break;
-                    }
-                    // Values nobody here sees (behind the last query, before the first window) have weight zero, but zero
-                    // times a NaN that lies there would not be zero: such rows are cleared first.
-                    const int key0 = before * kKeys;
-                    const int clear_low = min(max(first_seen - key0, 0), kKeys);
-                    const int clear_high = min(max(last_seen + 1 - key0, 0), kKeys);
-                    const int keep = min(max(a.sinks - key0, 0), kKeys);  // first tokens stay
-                    if (clear_low > keep || clear_high < kKeys) {
-                        for (int x = lane; x < kKeys * 8 * kBlocks; x += 32) {
-                            const int row = (x >> 3) & (kKeys - 1);
-                            if ((row < clear_low && row >= keep) || row >= clear_high)
-                                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(smem + S::kRing + st_v * S::kTile + x * 16),
-                                             "r"(0)
-                                             : "memory");
-                        }
-                        fence_async();
-                        __syncwarp();
-                    }
-                }
-                if (i < n && !bar_wait_warp(bar_full + 8 * st_k, ((2 * i) / S::kStages) & 1, a.limit)) {
+    } else if (warp == kScoreWarp) {
+        // ---- scores, issued by one thread: a tile's once the weights that were in its buffer are used up. (Products
+        // with the values have a warp of their own: a commit or a wait costs the issuing thread 100 clocks and more, and one
+        // thread for both took 2100 clocks a step against 1280 of work.)
+        constexpr uint32_t kDesc = mma_desc(kBf16, kKeys, false);
+        if (order.n > 0 && elect()) {
+            int n_s[2] = {0, 0};
+            failed = !bar_wait(bar_q, 0, a.limit);
+            for (int i = 0; i < order.n && !failed; ++i) {
+                const int j = order.tile(i), st = i % S::kStages;
+                if (!bar_wait(bar_k + 8 * st, (i / S::kStages) & 1, a.limit)) {
                     failed = true;
                     break;
                 }
+                const uint64_t k = smem_desc(smem + S::kRing + st * 2 * S::kTile);
+#pragma unroll
                 for (int t = 0; t < 2; ++t) {
-                    const Visit& v = t == 0 ? va : vb;
-                    if (i > 0 && v.has(before)) {
-                        if (!bar_wait_warp(bar_h + 8 * t, n_p[t] & 1, a.limit)) {
-                            failed = true;
-                            break;
-                        }
-                        fence_after();
-                        const bool narrow = v.narrow(before, a.sinks);
-                        const uint64_t values = smem_desc(smem + S::kRing + st_v * S::kTile, kKeys * 128);
-                        if (elect()) {
-#pragma unroll
-                            for (int k = 0; k < kKeys / 32; ++k)
-                                if (k < kNarrow / 16 || !narrow)
-                                    mma_ts(t_o[t], t_s[t] + 8 * k, desc_at(values, k * 2048), kDescO, n_p[t] > 0 || k > 0);
-                        }
-                        if (!bar_wait_warp(bar_p + 8 * t, n_p[t] & 1, a.limit)) {
-                            failed = true;
-                            break;
-                        }
-                        fence_after();
-                        if (elect()) {
-                            if (!narrow) {
-#pragma unroll
-                                for (int k = kKeys / 32; k < kKeys / 16; ++k)
-                                    mma_ts(t_o[t], t_s[t] + 8 * k, desc_at(values, k * 2048), kDescO, true);
-                            }
-                            if (before == v.high) mma_commit(bar_o + 8 * t);
-                        }
-                        ++n_p[t];
-                        __syncwarp();
+                    if (failed || !(t == 0 ? va : vb).has(j)) continue;
+                    const uint64_t q = smem_desc(smem + S::kQ + t * S::kQuery);
+                    const int buffer = 2 * t + (n_s[t] & 1);
+                    // (each row tile on its own: waiting for both made them run in step, their products in one burst)
+                    if (n_s[t] >= 2 && !bar_wait(bar_o + 8 * buffer, ((n_s[t] >> 1) - 1) & 1, a.limit)) {
+                        failed = true;
+                        continue;
                     }
-                    if (i < n && v.has(j)) {
-                        if (elect()) {
-                            const uint32_t desc = (v.narrow(j, a.sinks) ? kDescNarrow : kDescS) | a.negate;
-                            const uint64_t q = smem_desc(smem + S::kQ + t * S::kTile), k = smem_desc(smem + S::kRing + st_k * S::kTile);
+                    fence_after();
 #pragma unroll
-                            for (int x = 0; x < DP / 16; ++x) {
-                                const uint32_t off = (x >> 2) * (kRows * 128) + (x & 3) * 32;
-                                mma_ss(t_s[t], desc_at(q, off), desc_at(k, off), desc, x > 0);
-                            }
-                            mma_commit(bar_s + 8 * t);
-                        }
-                        __syncwarp();
-                    }
+                    for (int x = 0; x < DP / 16; ++x)
+                        mma_ss(t_s + kKeys * buffer, desc_at(q, (x >> 2) * (kRows * 128) + (x & 3) * 32),
+                               desc_at(k, (x >> 2) * (kKeys * 128) + (x & 3) * 32), kDesc | a.negate, x > 0);
+                    mma_commit(bar_s + 8 * buffer);
+                    ++n_s[t];
                 }
-                if (!failed && elect()) {
-                    if (i > 0) mma_commit(bar_empty + 8 * st_v);
-                    if (i < n) mma_commit(bar_empty + 8 * st_k);
-                }
-                __syncwarp();
+            }
+            if (failed) {  // the tensor memory is given back only when no product uses it any more
+                mma_commit(bar_end);
+                bar_wait(bar_end, 0, kDrain);
             }
         }
-        if (failed && elect()) {  // the tensor memory is given back only when no product uses it any more
-            mma_commit(bar_q);
-            bar_wait(bar_q, 1, a.limit);
+        __syncwarp();
+    } else if (warp == kValueWarp) {
+        // ---- products of the weights with the values, issued by one thread
+        constexpr uint32_t kDesc = mma_desc(kBf16, DP, true);
+        if (order.n > 0 && elect()) {
+            int n_p[2] = {0, 0};
+            for (int i = 0; i < order.n && !failed; ++i) {
+                const int j = order.tile(i), st = i % S::kStages;
+                if (!bar_wait(bar_clear + 8 * st, (i / S::kStages) & 1, a.limit)) {
+                    failed = true;
+                    break;
+                }
+                const uint64_t values = smem_desc(smem + S::kRing + st * 2 * S::kTile + S::kTile, kKeys * 128);
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    if (failed || !(t == 0 ? va : vb).has(j)) continue;
+                    const int buffer = 2 * t + (n_p[t] & 1);
+                    if (!bar_wait(bar_p + 8 * buffer, (n_p[t] >> 1) & 1, a.limit)) {
+                        failed = true;
+                        continue;
+                    }
+                    fence_after();
+#pragma unroll
+                    for (int x = 0; x < kKeys / 16; ++x)
+                        mma_ts(t_o + DP * t, t_s + kKeys * buffer + 8 * x, desc_at(values, x * 2048), kDesc, n_p[t] > 0 || x > 0);
+                    mma_commit(bar_o + 8 * buffer);
+                    ++n_p[t];
+                }
+                if (!failed) mma_commit(bar_done + 8 * st);
+            }
+            if (failed) {
+                mma_commit(bar_end + 8);
+                bar_wait(bar_end + 8, 0, kDrain);
+            }
         }
         __syncwarp();
-      }
+    } else if (warp == kClearWarp) {
+        // ---- values nobody here sees (behind the last query, before the first window) have weight zero, but zero times a NaN
+        // that lies there would not be zero: such rows are cleared before the products may read the tile.
+        const int first_seen = max(va.p_low - a.window + 1, 0);
+        const int last_seen = sq.lk - sq.lq + min(row0 + 2 * kRows, sq.lq) - 1;
+        for (int i = 0; i < order.n; ++i) {
+            const int st = i % S::kStages, key0 = order.tile(i) * kKeys;
+            if (!bar_wait_warp(bar_v + 8 * st, (i / S::kStages) & 1, a.limit)) {
+                failed = true;
+                break;
+            }
+            const int clear_low = min(max(first_seen - key0, 0), kKeys);
+            const int clear_high = min(max(last_seen + 1 - key0, 0), kKeys);
+            const int keep = min(max(a.sinks - key0, 0), kKeys);  // first tokens stay
+            if (clear_low > keep || clear_high < kKeys) {
+                for (int x = lane; x < kKeys * 8 * kBlocks; x += 32) {
+                    const int row = (x >> 3) & (kKeys - 1);
+                    if ((row < clear_low && row >= keep) || row >= clear_high)
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(smem + S::kRing + st * 2 * S::kTile + S::kTile + x * 16), "r"(0)
+                                     : "memory");
+                }
+                fence_async();
+                __syncwarp();
+            }
+            if (elect()) bar_arrive(bar_clear + 8 * st);
+            __syncwarp();
+        }
     } else {
         // ---- softmax: thread = row
-        registers_up<kSoftmaxRegisters>();
         const int t = warp >> 2;
         const Visit v = t == 0 ? va : vb;
         const int r = threadIdx.x & (kRows - 1);
         const int p = v.p_low + r;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // tensor-memory lane of the warp's first row
+        const uint32_t to = t_o + DP * t + lanes;
         Row row;
         int done = 0;
+        // Waits for the product of the last tile's weights. Scores of a tile are issued when the product of the last but one is
+        // complete: of the two barriers that the products arrive on in turn, the phase before is over.
+        const auto before = [&] {
+            const int last = done - 1;
+            const bool ok = bar_wait_warp(bar_o + 8 * (2 * t + (last & 1)), (last >> 1) & 1, a.limit);
+            fence_after();
+            return ok;
+        };
         for (int i = 0; i < order.n; ++i) {
             const int j = order.tile(i);
             if (!v.has(j)) continue;
-            if (!bar_wait_warp(bar_s + 8 * t, done & 1, a.limit)) {
+            const int buffer = 2 * t + (done & 1);
+            if (!bar_wait_warp(bar_s + 8 * buffer, (done >> 1) & 1, a.limit)) {
                 failed = true;
                 break;
             }
             fence_after();
             const int key0 = j * kKeys, last_p = v.p_low + kRows - 1;
-            const uint32_t ts = t_s[t] + lanes, to = t_o[t] + lanes, half = bar_h + 8 * t, full = bar_p + 8 * t;
-            const int above = p - key0, below = p - key0 - a.window, keep = a.sinks - key0;
-            if (v.narrow(j, a.sinks))
-                softmax_tile<T, DP, kNarrow, true>(row, ts, to, done > 0, a.scale_log2, above, below, keep, half, full);
-            else if (key0 + kKeys - 1 > v.p_low || (key0 <= last_p - a.window && key0 + kKeys > a.sinks))
-                softmax_tile<T, DP, kKeys, true>(row, ts, to, done > 0, a.scale_log2, above, below, keep, half, full);
-            else
-                softmax_tile<T, DP, kKeys, false>(row, ts, to, done > 0, a.scale_log2, 0, 0, 0, half, full);
+            const uint32_t ts = t_s + kKeys * buffer + lanes, ready = bar_p + 8 * buffer;
+            const bool edge = key0 + kKeys - 1 > v.p_low || (key0 <= last_p - a.window && key0 + kKeys > a.sinks);
+            const bool ok = edge ? softmax_tile<T, DP, true>(row, ts, to, done > 0, a.scale_log2, p - key0, p - key0 - a.window, a.sinks - key0, ready, before)
+                                 : softmax_tile<T, DP, false>(row, ts, to, done > 0, a.scale_log2, 0, 0, 0, ready, before);
+            if (!ok) {
+                failed = true;
+                break;
+            }
             ++done;
         }
         // ---- epilogue
         if (done > 0 && !failed) {
-            failed = !bar_wait_warp(bar_o + 8 * t, 0, a.limit);
-            fence_after();
+            failed = !before();
         }
         const float inv = row.sum == 0.0f ? 0.0f : 1.0f / row.sum;
         const int64_t token = (int64_t)sq.q0 + row0 + t * kRows + r;
@@ -412,7 +415,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int c = 0; c < DP; c += 32) {
             uint32_t o[32];
             if (done > 0 && !failed) {
-                tmem_load32(t_o[t] + lanes + c, o);
+                tmem_load32(to + c, o);
                 wait_loads();
                 after_loads32(o);
             }
@@ -436,7 +439,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (failed && a.fault != nullptr) *reinterpret_cast<volatile int*>(a.fault) = 1;
     __syncthreads();
-    if (warp == 9) {
+    if (warp == kValueWarp) {
         fence_after();
         tmem_free(tmem, 512);
     }
