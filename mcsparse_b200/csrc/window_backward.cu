@@ -26,7 +26,9 @@ using namespace tc;
 constexpr int kRows = 128;  // stationary rows of a block
 constexpr int kTile = 64;   // rows of a streamed tile
 constexpr int kStages = 4;
-constexpr int kThreads = 320;  // 2 x 128 for the element-wise part, the loading warp, the warp that issues the products
+constexpr int kElementWarps = 8;  // two buffers x 128 rows
+constexpr int kLoadWarp = kElementWarps, kScoreWarp = kElementWarps + 1, kSumWarp = kElementWarps + 2, kClearWarp = kElementWarps + 3;
+constexpr int kThreads = 32 * (kElementWarps + 4);
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <int DP>
@@ -129,6 +131,48 @@ __global__ void __launch_bounds__(256) delta_kernel(AttentionArgs a, float* __re
     if (live && part == 0) delta[h * a.total_q + t] = sum;
 }
 
+// One row of 64 scores s and 64 dP d -> P and dS in 16 bits, into the first half of their columns of tensor memory. -lse and
+// -delta (scaled) of the columns lie at `vec` in shared memory (keys kernel) or are the row's own. MASK: bit c of `seen`.
+template <typename T, bool KEYS, bool MASK>
+__device__ __forceinline__ void weights(const uint32_t* s, const uint32_t* d, uint32_t ts, uint32_t td, uint64_t seen, uint32_t vec, float own_l,
+                                        float own_d, float scale_log2) {
+    constexpr float kLower = std::is_same<T, __half>::value ? 1.0f / 256.0f : 1.0f;
+    const uint64_t scale2 = pair(scale_log2, scale_log2), lower2 = pair(kLower, kLower);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        uint32_t wp[16], wd[16];
+        const uint32_t bits = (uint32_t)(seen >> (32 * h));
+#pragma unroll
+        for (int c = 0; c < 32; c += 4) {
+            float l[4] = {own_l, own_l, own_l, own_l}, e[4] = {own_d, own_d, own_d, own_d};
+            if (KEYS) {
+                asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                             : "=f"(l[0]), "=f"(l[1]), "=f"(l[2]), "=f"(l[3])
+                             : "r"(vec + 4 * (32 * h + c)));
+                asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                             : "=f"(e[0]), "=f"(e[1]), "=f"(e[2]), "=f"(e[3])
+                             : "r"(vec + 4 * (kTile + 32 * h + c)));
+            }
+#pragma unroll
+            for (int x = 0; x < 4; x += 2) {
+                const int at = 32 * h + c + x;
+                float p0, p1, g0, g1;
+                unpair(fma2(pair(__uint_as_float(s[at]), __uint_as_float(s[at + 1])), scale2, pair(l[x], l[x + 1])), p0, p1);
+                p0 = exp2_fast(p0), p1 = exp2_fast(p1);
+                unpair(mul2(pair(p0, p1), fma2(pair(__uint_as_float(d[at]), __uint_as_float(d[at + 1])), lower2, pair(e[x], e[x + 1]))), g0, g1);
+                if (MASK) {
+                    if (!(bits >> (c + x) & 1)) p0 = 0.0f, g0 = 0.0f;
+                    if (!(bits >> (c + x + 1) & 1)) p1 = 0.0f, g1 = 0.0f;
+                }
+                wp[(c + x) >> 1] = pack2<T>(p0, p1);
+                wd[(c + x) >> 1] = pack2<T>(g0, g1);
+            }
+        }
+        if (KEYS) tmem_store16(ts + 16 * h, wp);
+        tmem_store16(td + 16 * h, wd);
+    }
+}
+
 // KEYS: stationary K, V; streamed Q, dO. Otherwise: stationary Q, dO; streamed K, V.
 template <typename T, int DP, bool KEYS>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -143,11 +187,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr float kLift = kHalf ? 8.0f : 0.0f, kLower = kHalf ? 1.0f / 256.0f : 1.0f;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem = (smem_u32(smem_raw) + 1023) & ~1023u;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = uniform((int)(threadIdx.x >> 5)), lane = threadIdx.x & 31;
+    // barriers: stationary operands; of every stage: there, clear, done with; of the two buffers: S and dP ready, P and dS ready,
+    // the sums' products done; the last of them done; the ends of the two issuing warps
     const uint32_t bars = smem + S::kBars;
-    // barriers: stationary operands, full[stages], empty[stages], S and dP ready[2], P and dS ready[2], sums ready
-    const uint32_t bar_fixed = bars, bar_full = bars + 8, bar_empty = bar_full + 8 * kStages, bar_s = bar_empty + 8 * kStages,
-                   bar_p = bar_s + 16, bar_out = bar_p + 16, slot = bar_out + 8;
+    const uint32_t bar_fixed = bars, bar_full = bars + 8, bar_clear = bar_full + 8 * kStages, bar_empty = bar_clear + 8 * kStages,
+                   bar_s = bar_empty + 8 * kStages, bar_p = bar_s + 16, bar_out = bar_p + 16, bar_last = bar_out + 16, bar_end = bar_last + 8, slot = bar_end + 16;
 
     // ---- the block's rows and its stream
     const int heads = KEYS ? a.kv_heads : a.q_heads;
@@ -203,6 +248,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         first = min((min(a.sinks, p_high + 1) + kTile - 1) / kTile, low);
         tiles = first + p_high / kTile - low + 1;
     }
+    tiles = uniform(tiles), first = uniform(first), low = uniform(low), begin = uniform(begin);
     const int n = tiles * hops;
     // first streamed row of tile i, relative to the sequence
     const auto tile_row = [&](int i) {
@@ -210,13 +256,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         return (i < first ? i : low + (i - first)) * kTile;
     };
 
-    if (warp == 9) {
+    if (warp == kSumWarp) {
         tmem_alloc(slot, 512);
-    } else if (threadIdx.x == 256) {
+    } else if (threadIdx.x == 32 * kLoadWarp) {
         bar_init(bar_fixed, 1);
-        for (int i = 0; i < kStages; ++i) bar_init(bar_full + 8 * i, 1), bar_init(bar_empty + 8 * i, 1);
-        for (int i = 0; i < 2; ++i) bar_init(bar_s + 8 * i, 1), bar_init(bar_p + 8 * i, kRows);
-        bar_init(bar_out, 1);
+        for (int i = 0; i < 3 * kStages; ++i) bar_init(bar_full + 8 * i, 1);
+        for (int i = 0; i < 2; ++i) bar_init(bar_s + 8 * i, 1), bar_init(bar_p + 8 * i, kRows), bar_init(bar_out + 8 * i, 1), bar_init(bar_end + 8 * i, 1);
+        bar_init(bar_last, 1);
         bar_init_fence();
     }
     fence_before();
@@ -224,11 +270,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     fence_after();
     uint32_t tmem;
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(slot));
+    tmem = uniform(tmem);
     // tensor memory: S[2] and dP[2] of 64 columns, then the sums (dV and dK, or dQ)
     const uint32_t t_s = tmem, t_dp = tmem + 2 * kTile, t_out1 = tmem + 4 * kTile, t_out2 = t_out1 + DP;
     bool failed = false;
 
-    if (warp == 8) {
+    if (warp == kLoadWarp) {
         // ---- loads
         if (n > 0) {
             const int hk = KEYS ? head : head / a.group;
@@ -292,79 +339,92 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
         __syncwarp();
-    } else if (warp == 9) {
-        // ---- products
-        constexpr uint32_t kDescS = mma_desc(!kHalf, kTile, false), kDescOut = mma_desc(!kHalf, DP, true);
-        const int first_seen = max(p_low - a.window + 1, 0);  // queries kernel: keys that some row here sees
-        if (n > 0) failed = !bar_wait_warp(bar_fixed, 0, a.limit);
-        for (int i = 0; i <= n && n > 0 && !failed; ++i) {
-            if (i < n) {
+    } else if (warp == kScoreWarp) {
+        // ---- S and dP, issued by one thread: a tile's once what was in their buffer is used up
+        constexpr uint32_t kDesc = mma_desc(!kHalf, kTile, false);
+        if (n > 0 && elect()) {
+            failed = !bar_wait(bar_fixed, 0, a.limit);
+            const uint64_t f1 = smem_desc(smem), f2 = smem_desc(smem + S::kFixed);
+            for (int i = 0; i < n && !failed; ++i) {
                 const int st = i % kStages, b = i & 1;
-                if (!bar_wait_warp(bar_full + 8 * st, (i / kStages) & 1, a.limit)) {
-                    failed = true;
-                    break;
-                }
-                const uint32_t s1 = smem + S::kRing + st * 2 * S::kStream, s2 = s1 + S::kStream;
-                // Rows whose weight is zero for every row here are cleared before they enter a sum: zero times a NaN that
-                // lies there would not be zero. Keys kernel: queries behind the last one; queries kernel: keys nobody sees.
-                const int row = tile_row(i);
-                const int clear_low = KEYS ? 0 : min(max(first_seen - row, 0), kTile);
-                const int keep = KEYS ? 0 : min(max(a.sinks - row, 0), kTile);
-                const int clear_high = min(max((KEYS ? end : p_high + 1) - row, 0), kTile);
-                if (clear_low > keep || clear_high < kTile) {
-                    for (int x = lane; x < (KEYS ? 2 : 1) * kTile * 8 * kBlocks; x += 32) {  // (stream 2 lies behind stream 1)
-                        const int at = (x >> 3) & (kTile - 1);
-                        if ((at < clear_low && at >= keep) || at >= clear_high)
-                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(s1 + x * 16), "r"(0) : "memory");
-                    }
-                    fence_async();
-                    __syncwarp();
-                }
-                if (elect()) {
-                    const uint64_t f1 = smem_desc(smem), f2 = smem_desc(smem + S::kFixed), m1 = smem_desc(s1), m2 = smem_desc(s2);
-#pragma unroll
-                    for (int k = 0; k < DP / 16; ++k) {
-                        const uint32_t fixed = (k >> 2) * (kRows * 128) + (k & 3) * 32, stream = (k >> 2) * (kTile * 128) + (k & 3) * 32;
-                        mma_ss(t_s + kTile * b, desc_at(f1, fixed), desc_at(m1, stream), kDescS | a.negate, k > 0);
-                    }
-#pragma unroll
-                    for (int k = 0; k < DP / 16; ++k) {
-                        const uint32_t fixed = (k >> 2) * (kRows * 128) + (k & 3) * 32, stream = (k >> 2) * (kTile * 128) + (k & 3) * 32;
-                        mma_ss(t_dp + kTile * b, desc_at(f2, fixed), desc_at(m2, stream), kDescS, k > 0);
-                    }
-                    mma_commit(bar_s + 8 * b);
-                }
-                __syncwarp();
-            }
-            if (i > 0) {
-                const int st = (i - 1) % kStages, b = (i - 1) & 1;
-                if (!bar_wait_warp(bar_p + 8 * b, ((i - 1) >> 1) & 1, a.limit)) {
+                if (!bar_wait(bar_clear + 8 * st, (i / kStages) & 1, a.limit) || (i >= 2 && !bar_wait(bar_out + 8 * b, ((i >> 1) - 1) & 1, a.limit))) {
                     failed = true;
                     break;
                 }
                 fence_after();
-                if (elect()) {
-                    const uint32_t s1 = smem + S::kRing + st * 2 * S::kStream;
-                    const uint64_t m1 = smem_desc(s1, kTile * 128), m2 = smem_desc(s1 + S::kStream, kTile * 128);
-                    if (KEYS) {
+                const uint32_t s1 = smem + S::kRing + st * 2 * S::kStream;
+                const uint64_t m1 = smem_desc(s1), m2 = smem_desc(s1 + S::kStream);
 #pragma unroll
-                        for (int k = 0; k < kTile / 16; ++k)
-                            mma_ts(t_out1, t_s + kTile * b + 8 * k, desc_at(m2, k * 2048), kDescOut, i > 1 || k > 0);
-                    }
+                for (int k = 0; k < DP / 16; ++k)
+                    mma_ss(t_s + kTile * b, desc_at(f1, (k >> 2) * (kRows * 128) + (k & 3) * 32), desc_at(m1, (k >> 2) * (kTile * 128) + (k & 3) * 32),
+                           kDesc | a.negate, k > 0);
 #pragma unroll
-                    for (int k = 0; k < kTile / 16; ++k)
-                        mma_ts(KEYS ? t_out2 : t_out1, t_dp + kTile * b + 8 * k, desc_at(m1, k * 2048), kDescOut, i > 1 || k > 0);
-                    mma_commit(bar_empty + 8 * st);
-                    if (i == n) mma_commit(bar_out);
-                }
-                __syncwarp();
+                for (int k = 0; k < DP / 16; ++k)
+                    mma_ss(t_dp + kTile * b, desc_at(f2, (k >> 2) * (kRows * 128) + (k & 3) * 32), desc_at(m2, (k >> 2) * (kTile * 128) + (k & 3) * 32),
+                           kDesc, k > 0);
+                mma_commit(bar_s + 8 * b);
+            }
+            if (failed) {  // the tensor memory is given back only when no product uses it any more
+                mma_commit(bar_end);
+                bar_wait(bar_end, 0, kDrain);
             }
         }
-        if (failed && elect()) {  // the tensor memory is given back only when no product uses it any more
-            mma_commit(bar_fixed);
-            bar_wait(bar_fixed, 1, kDrain);
+        __syncwarp();
+    } else if (warp == kSumWarp) {
+        // ---- dV and dK, or dQ, issued by one thread
+        constexpr uint32_t kDesc = mma_desc(!kHalf, DP, true);
+        if (n > 0 && elect()) {
+            for (int i = 0; i < n; ++i) {
+                const int st = i % kStages, b = i & 1;
+                if (!bar_wait(bar_p + 8 * b, (i >> 1) & 1, a.limit) || !bar_wait(bar_clear + 8 * st, (i / kStages) & 1, a.limit)) {
+                    failed = true;
+                    break;
+                }
+                fence_after();
+                const uint32_t s1 = smem + S::kRing + st * 2 * S::kStream;
+                const uint64_t m1 = smem_desc(s1, kTile * 128), m2 = smem_desc(s1 + S::kStream, kTile * 128);
+                if (KEYS) {
+#pragma unroll
+                    for (int k = 0; k < kTile / 16; ++k) mma_ts(t_out1, t_s + kTile * b + 8 * k, desc_at(m2, k * 2048), kDesc, i > 0 || k > 0);
+                }
+#pragma unroll
+                for (int k = 0; k < kTile / 16; ++k)
+                    mma_ts(KEYS ? t_out2 : t_out1, t_dp + kTile * b + 8 * k, desc_at(m1, k * 2048), kDesc, i > 0 || k > 0);
+                mma_commit(bar_out + 8 * b);
+                mma_commit(bar_empty + 8 * st);
+                if (i == n - 1) mma_commit(bar_last);
+            }
+            if (failed) {
+                mma_commit(bar_end + 8);
+                bar_wait(bar_end + 8, 0, kDrain);
+            }
         }
         __syncwarp();
+    } else if (warp == kClearWarp) {
+        // ---- rows whose weight is zero for every row here are cleared before they enter a sum: zero times a NaN that lies there
+        // would not be zero. Keys kernel: queries behind the last one; queries kernel: keys nobody sees.
+        const int first_seen = max(p_low - a.window + 1, 0);  // queries kernel: the first key in reach of some row here
+        for (int i = 0; i < n; ++i) {
+            const int st = i % kStages, row = tile_row(i);
+            if (!bar_wait_warp(bar_full + 8 * st, (i / kStages) & 1, a.limit)) {
+                failed = true;
+                break;
+            }
+            const int clear_low = KEYS ? 0 : min(max(first_seen - row, 0), kTile);
+            const int keep = KEYS ? 0 : min(max(a.sinks - row, 0), kTile);
+            const int clear_high = min(max((KEYS ? end : p_high + 1) - row, 0), kTile);
+            if (clear_low > keep || clear_high < kTile) {
+                for (int x = lane; x < (KEYS ? 2 : 1) * kTile * 8 * kBlocks; x += 32) {  // (stream 2 lies behind stream 1)
+                    const int at = (x >> 3) & (kTile - 1);
+                    if ((at < clear_low && at >= keep) || at >= clear_high)
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(smem + S::kRing + st * 2 * S::kStream + x * 16), "r"(0) : "memory");
+                }
+                fence_async();
+                __syncwarp();
+            }
+            if (elect()) bar_arrive(bar_clear + 8 * st);
+            __syncwarp();
+        }
     } else {
         // ---- P and dS: thread = stationary row, buffer b = its warpgroup
         const int b = warp >> 2;
@@ -415,36 +475,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
             const uint32_t vec = smem + S::kVec + (i % kStages) * S::kVectors;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                uint32_t wp[16], wd[16];
-                const uint32_t bits = (uint32_t)(seen >> (32 * h));
-#pragma unroll
-                for (int c = 0; c < 32; c += 4) {
-                    float l[4], e[4], p[4], g[4];
-                    if (KEYS) {
-                        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-                                     : "=f"(l[0]), "=f"(l[1]), "=f"(l[2]), "=f"(l[3])
-                                     : "r"(vec + 4 * (32 * h + c)));
-                        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-                                     : "=f"(e[0]), "=f"(e[1]), "=f"(e[2]), "=f"(e[3])
-                                     : "r"(vec + 4 * (kTile + 32 * h + c)));
-                    }
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        const int at = 32 * h + c + x;
-                        p[x] = exp2_fast(fmaf(__uint_as_float(s[at]), a.scale_log2, KEYS ? l[x] : own_l));
-                        g[x] = p[x] * fmaf(__uint_as_float(d[at]), kLower, KEYS ? e[x] : own_d);
-                        if (!(bits >> (c + x) & 1)) p[x] = 0.0f, g[x] = 0.0f;
-                    }
-                    wp[c >> 1] = pack2<T>(p[0], p[1]);
-                    wp[(c >> 1) + 1] = pack2<T>(p[2], p[3]);
-                    wd[c >> 1] = pack2<T>(g[0], g[1]);
-                    wd[(c >> 1) + 1] = pack2<T>(g[2], g[3]);
-                }
-                if (KEYS) tmem_store16(t_s + kTile * b + lanes + 16 * h, wp);
-                tmem_store16(t_dp + kTile * b + lanes + 16 * h, wd);
-            }
+            const uint32_t ts = t_s + kTile * b + lanes, td = t_dp + kTile * b + lanes;
+            if (__all_sync(0xffffffffu, seen == ~0ull))
+                weights<T, KEYS, false>(s, d, ts, td, 0, vec, own_l, own_d, a.scale_log2);
+            else
+                weights<T, KEYS, true>(s, d, ts, td, seen, vec, own_l, own_d, a.scale_log2);
             wait_stores();
             fence_before();
             bar_arrive(bar_p + 8 * b);
@@ -452,7 +487,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         // ---- outputs: keys kernel: one warpgroup writes dV, the other dK; queries kernel: each half of dQ's columns
         if (n > 0 && !failed) {
-            failed = !bar_wait_warp(bar_out, 0, a.limit);
+            failed = !bar_wait_warp(bar_last, 0, a.limit);
             fence_after();
         }
         const uint32_t t_out = KEYS && b == 1 ? t_out2 : t_out1;
@@ -494,7 +529,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (failed && a.fault != nullptr) *reinterpret_cast<volatile int*>(a.fault) = 1;
     __syncthreads();
-    if (warp == 9) {
+    if (warp == kSumWarp) {
         fence_after();
         tmem_free(tmem, 512);
     }
