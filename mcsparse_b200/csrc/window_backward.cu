@@ -4,8 +4,9 @@
 //                   tiles of 64 that see them, for all query heads that share the keys (their sum stays in tensor memory);
 //   queries kernel  one block per 128 queries and query head: S = Q K^T, dP = dO V^T, dQ += dS K over the key tiles of 64.
 // Both are one kernel template: 128 stationary rows against a stream of 64-row tiles. S and dP have two buffers in tensor
-// memory, each with 128 threads (one row each) that turn them into P and dS in place, in 16 bits, while the tensor cores work
-// on the other buffer; P and dS enter the second products from tensor memory. Two kernels compute S and dP twice (7 products
+// memory (three where dV, dK or dQ leave room); two groups of 128 threads, one row each, take the tiles in turn and make P
+// and dS of them in place, in 16 bits, while the tensor cores work on the other buffers; P and dS enter the second products
+// from tensor memory, P as soon as it is there. Two kernels compute S and dP twice (7 products
 // instead of 5), which buys sums without atomics: equal inputs give equal bits, and nothing is kept in fp32 in HBM.
 //
 // The first tokens of a sequence are seen by all its queries. Their key tiles would run far longer than the others: what
@@ -39,7 +40,8 @@ struct Smem {
     static constexpr int kRing = 2 * kFixed;
     static constexpr int kVec = kRing + kStages * 2 * kStream;
     static constexpr int kBars = kVec + kStages * kVectors;
-    static constexpr int kTotal = kBars + 256 + 1024;
+    static constexpr int kTotal = kBars + 512 + 1024;  // (the start is aligned to 1024)
+    static_assert(kTotal <= 227 * 1024, "shared memory of a block");
 };
 
 struct Params {
@@ -131,45 +133,73 @@ __global__ void __launch_bounds__(256) delta_kernel(AttentionArgs a, float* __re
     if (live && part == 0) delta[h * a.total_q + t] = sum;
 }
 
-// One row of 64 scores s and 64 dP d -> P and dS in 16 bits, into the first half of their columns of tensor memory. -lse and
-// -delta (scaled) of the columns lie at `vec` in shared memory (keys kernel) or are the row's own. MASK: bit c of `seen`.
+// Four values of the tile's columns: from shared memory (keys kernel), or the row's own.
+template <bool KEYS>
+__device__ __forceinline__ void column_values(uint32_t vec, int c, float own, float* v) {
+    if (KEYS)
+        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(vec + 4 * c));
+    else
+        v[0] = v[1] = v[2] = v[3] = own;
+}
+
+// 64 scores of a row -> its weights, in place; keys kernel: also, in 16 bits, into the first half of the scores' columns. `vec` /
+// own_l: -lse (base 2) of the columns / the row. MASK: column c counts iff bit c of `seen` is set.
 template <typename T, bool KEYS, bool MASK>
-__device__ __forceinline__ void weights(const uint32_t* s, const uint32_t* d, uint32_t ts, uint32_t td, uint64_t seen, uint32_t vec, float own_l,
-                                        float own_d, float scale_log2) {
-    constexpr float kLower = std::is_same<T, __half>::value ? 1.0f / 256.0f : 1.0f;
-    const uint64_t scale2 = pair(scale_log2, scale_log2), lower2 = pair(kLower, kLower);
+__device__ __forceinline__ void weights(uint32_t* p, uint32_t ts, uint64_t seen, uint32_t vec, float own_l, float scale_log2) {
+    const uint64_t scale2 = pair(scale_log2, scale_log2);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        uint32_t wp[16], wd[16];
+        uint32_t w[16];
         const uint32_t bits = (uint32_t)(seen >> (32 * h));
 #pragma unroll
         for (int c = 0; c < 32; c += 4) {
-            float l[4] = {own_l, own_l, own_l, own_l}, e[4] = {own_d, own_d, own_d, own_d};
-            if (KEYS) {
-                asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-                             : "=f"(l[0]), "=f"(l[1]), "=f"(l[2]), "=f"(l[3])
-                             : "r"(vec + 4 * (32 * h + c)));
-                asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-                             : "=f"(e[0]), "=f"(e[1]), "=f"(e[2]), "=f"(e[3])
-                             : "r"(vec + 4 * (kTile + 32 * h + c)));
-            }
+            float l[4];
+            column_values<KEYS>(vec, 32 * h + c, own_l, l);
 #pragma unroll
             for (int x = 0; x < 4; x += 2) {
                 const int at = 32 * h + c + x;
-                float p0, p1, g0, g1;
-                unpair(fma2(pair(__uint_as_float(s[at]), __uint_as_float(s[at + 1])), scale2, pair(l[x], l[x + 1])), p0, p1);
+                float p0, p1;
+                unpair(fma2(pair(__uint_as_float(p[at]), __uint_as_float(p[at + 1])), scale2, pair(l[x], l[x + 1])), p0, p1);
                 p0 = exp2_fast(p0), p1 = exp2_fast(p1);
-                unpair(mul2(pair(p0, p1), fma2(pair(__uint_as_float(d[at]), __uint_as_float(d[at + 1])), lower2, pair(e[x], e[x + 1]))), g0, g1);
                 if (MASK) {
-                    if (!(bits >> (c + x) & 1)) p0 = 0.0f, g0 = 0.0f;
-                    if (!(bits >> (c + x + 1) & 1)) p1 = 0.0f, g1 = 0.0f;
+                    p0 = bits >> (c + x) & 1 ? p0 : 0.0f;
+                    p1 = bits >> (c + x + 1) & 1 ? p1 : 0.0f;
                 }
-                wp[(c + x) >> 1] = pack2<T>(p0, p1);
-                wd[(c + x) >> 1] = pack2<T>(g0, g1);
+                if (KEYS) w[(c + x) >> 1] = pack2<T>(p0, p1);
+                p[at] = __float_as_uint(p0), p[at + 1] = __float_as_uint(p1);
             }
         }
-        if (KEYS) tmem_store16(ts + 16 * h, wp);
-        tmem_store16(td + 16 * h, wd);
+        if (KEYS) tmem_store16(ts + 16 * h, w);
+    }
+}
+
+// dS = P * (dP - delta) of a row, in 16 bits into the first half of dP's columns. (An unseen pair is 0 also where dP is NaN.)
+template <typename T, bool KEYS, bool MASK>
+__device__ __forceinline__ void weight_gradients(const uint32_t* p, const uint32_t* d, uint32_t td, uint64_t seen, uint32_t vec, float own_d) {
+    constexpr float kLower = std::is_same<T, __half>::value ? 1.0f / 256.0f : 1.0f;
+    const uint64_t lower2 = pair(kLower, kLower);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        uint32_t w[16];
+        const uint32_t bits = (uint32_t)(seen >> (32 * h));
+#pragma unroll
+        for (int c = 0; c < 32; c += 4) {
+            float e[4];
+            column_values<KEYS>(vec, 32 * h + c, own_d, e);
+#pragma unroll
+            for (int x = 0; x < 4; x += 2) {
+                const int at = 32 * h + c + x;
+                float g0, g1;
+                unpair(mul2(pair(__uint_as_float(p[at]), __uint_as_float(p[at + 1])),
+                            fma2(pair(__uint_as_float(d[at]), __uint_as_float(d[at + 1])), lower2, pair(e[x], e[x + 1]))), g0, g1);
+                if (MASK) {
+                    g0 = bits >> (c + x) & 1 ? g0 : 0.0f;
+                    g1 = bits >> (c + x + 1) & 1 ? g1 : 0.0f;
+                }
+                w[(c + x) >> 1] = pack2<T>(g0, g1);
+            }
+        }
+        tmem_store16(td + 16 * h, w);
     }
 }
 
@@ -182,17 +212,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     using S = Smem<DP>;
     constexpr bool kHalf = std::is_same<T, __half>::value;
     constexpr int kBlocks = DP / 64;
+    constexpr int kBuffers = KEYS && DP == 128 ? 2 : 3;
+    static_assert(kBuffers * 2 * kTile + (KEYS ? 2 : 1) * DP <= 512, "columns of tensor memory");
     // fp16 P is held 2^8 times too large (at most 256): weights below 2^-14 would lose bits to fp16's subnormal numbers. The
     // factor leaves dS through the other factor of its product and dV at the end.
     constexpr float kLift = kHalf ? 8.0f : 0.0f, kLower = kHalf ? 1.0f / 256.0f : 1.0f;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem = (smem_u32(smem_raw) + 1023) & ~1023u;
     const int warp = uniform((int)(threadIdx.x >> 5)), lane = threadIdx.x & 31;
-    // barriers: stationary operands; of every stage: there, clear, done with; of the two buffers: S and dP ready, P and dS ready,
-    // the sums' products done; the last of them done; the ends of the two issuing warps
+    // barriers: stationary operands; of every stage: there, clear, done with; of the buffers: S ready, dP ready, P ready, dS ready,
+    // S's columns free, dP's columns free; the last product done; the ends of the two issuing warps
     const uint32_t bars = smem + S::kBars;
     const uint32_t bar_fixed = bars, bar_full = bars + 8, bar_clear = bar_full + 8 * kStages, bar_empty = bar_clear + 8 * kStages,
-                   bar_s = bar_empty + 8 * kStages, bar_p = bar_s + 16, bar_out = bar_p + 16, bar_last = bar_out + 16, bar_end = bar_last + 8, slot = bar_end + 16;
+                   bar_s = bar_empty + 8 * kStages, bar_dp = bar_s + 8 * kBuffers, bar_p = bar_dp + 8 * kBuffers, bar_ds = bar_p + 8 * kBuffers,
+                   bar_free_s = bar_ds + 8 * kBuffers, bar_free_dp = bar_free_s + 8 * kBuffers, bar_last = bar_free_dp + 8 * kBuffers,
+                   bar_end = bar_last + 8, slot = bar_end + 16;
 
     // ---- the block's rows and its stream
     const int heads = KEYS ? a.kv_heads : a.q_heads;
@@ -261,8 +295,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (threadIdx.x == 32 * kLoadWarp) {
         bar_init(bar_fixed, 1);
         for (int i = 0; i < 3 * kStages; ++i) bar_init(bar_full + 8 * i, 1);
-        for (int i = 0; i < 2; ++i) bar_init(bar_s + 8 * i, 1), bar_init(bar_p + 8 * i, kRows), bar_init(bar_out + 8 * i, 1), bar_init(bar_end + 8 * i, 1);
-        bar_init(bar_last, 1);
+        for (int i = 0; i < kBuffers; ++i) {
+            bar_init(bar_s + 8 * i, 1), bar_init(bar_dp + 8 * i, 1), bar_init(bar_p + 8 * i, kRows), bar_init(bar_ds + 8 * i, kRows);
+            bar_init(bar_free_s + 8 * i, 1), bar_init(bar_free_dp + 8 * i, 1);
+        }
+        bar_init(bar_last, 1), bar_init(bar_end, 1), bar_init(bar_end + 8, 1);
         bar_init_fence();
     }
     fence_before();
@@ -271,8 +308,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t tmem;
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(slot));
     tmem = uniform(tmem);
-    // tensor memory: S[2] and dP[2] of 64 columns, then the sums (dV and dK, or dQ)
-    const uint32_t t_s = tmem, t_dp = tmem + 2 * kTile, t_out1 = tmem + 4 * kTile, t_out2 = t_out1 + DP;
+    // tensor memory: the buffers of S and dP, 64 columns each, then the sums (dV and dK, or dQ)
+    const uint32_t t_s = tmem, t_dp = tmem + kBuffers * kTile, t_out1 = tmem + 2 * kBuffers * kTile, t_out2 = t_out1 + DP;
     bool failed = false;
 
     if (warp == kLoadWarp) {
@@ -340,29 +377,38 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
     } else if (warp == kScoreWarp) {
-        // ---- S and dP, issued by one thread: a tile's once what was in their buffer is used up
+        // ---- S and dP, issued by one thread, each once its columns are free
         constexpr uint32_t kDesc = mma_desc(!kHalf, kTile, false);
         if (n > 0 && elect()) {
             failed = !bar_wait(bar_fixed, 0, a.limit);
             const uint64_t f1 = smem_desc(smem), f2 = smem_desc(smem + S::kFixed);
             for (int i = 0; i < n && !failed; ++i) {
-                const int st = i % kStages, b = i & 1;
-                if (!bar_wait(bar_clear + 8 * st, (i / kStages) & 1, a.limit) || (i >= 2 && !bar_wait(bar_out + 8 * b, ((i >> 1) - 1) & 1, a.limit))) {
+                const int st = i % kStages, b = i % kBuffers;
+                const uint32_t before = (i / kBuffers - 1) & 1;  // the phase of the buffer's last use
+                const uint32_t s1 = smem + S::kRing + st * 2 * S::kStream;
+                const uint64_t m1 = smem_desc(s1), m2 = smem_desc(s1 + S::kStream);
+                if (!bar_wait(bar_clear + 8 * st, (i / kStages) & 1, a.limit) || (i >= kBuffers && !bar_wait(bar_free_s + 8 * b, before, a.limit))) {
                     failed = true;
                     break;
                 }
                 fence_after();
-                const uint32_t s1 = smem + S::kRing + st * 2 * S::kStream;
-                const uint64_t m1 = smem_desc(s1), m2 = smem_desc(s1 + S::kStream);
 #pragma unroll
                 for (int k = 0; k < DP / 16; ++k)
                     mma_ss(t_s + kTile * b, desc_at(f1, (k >> 2) * (kRows * 128) + (k & 3) * 32), desc_at(m1, (k >> 2) * (kTile * 128) + (k & 3) * 32),
                            kDesc | a.negate, k > 0);
+                mma_commit(bar_s + 8 * b);
+                if (KEYS && i >= kBuffers) {  // (queries kernel: S and dP are free together)
+                    if (!bar_wait(bar_free_dp + 8 * b, before, a.limit)) {
+                        failed = true;
+                        break;
+                    }
+                    fence_after();
+                }
 #pragma unroll
                 for (int k = 0; k < DP / 16; ++k)
                     mma_ss(t_dp + kTile * b, desc_at(f2, (k >> 2) * (kRows * 128) + (k & 3) * 32), desc_at(m2, (k >> 2) * (kTile * 128) + (k & 3) * 32),
                            kDesc, k > 0);
-                mma_commit(bar_s + 8 * b);
+                mma_commit(bar_dp + 8 * b);
             }
             if (failed) {  // the tensor memory is given back only when no product uses it any more
                 mma_commit(bar_end);
@@ -375,22 +421,33 @@ __global__ void __launch_bounds__(kThreads, 1)
         constexpr uint32_t kDesc = mma_desc(!kHalf, DP, true);
         if (n > 0 && elect()) {
             for (int i = 0; i < n; ++i) {
-                const int st = i % kStages, b = i & 1;
-                if (!bar_wait(bar_p + 8 * b, (i >> 1) & 1, a.limit) || !bar_wait(bar_clear + 8 * st, (i / kStages) & 1, a.limit)) {
+                const int st = i % kStages, b = i % kBuffers;
+                const uint32_t phase = (i / kBuffers) & 1;
+                const uint32_t s1 = smem + S::kRing + st * 2 * S::kStream;
+                const uint64_t m1 = smem_desc(s1, kTile * 128), m2 = smem_desc(s1 + S::kStream, kTile * 128);
+                if (!bar_wait(bar_clear + 8 * st, (i / kStages) & 1, a.limit)) {
+                    failed = true;
+                    break;
+                }
+                if (KEYS) {
+                    if (!bar_wait(bar_p + 8 * b, phase, a.limit)) {
+                        failed = true;
+                        break;
+                    }
+                    fence_after();
+#pragma unroll
+                    for (int k = 0; k < kTile / 16; ++k) mma_ts(t_out1, t_s + kTile * b + 8 * k, desc_at(m2, k * 2048), kDesc, i > 0 || k > 0);
+                    mma_commit(bar_free_s + 8 * b);
+                }
+                if (!bar_wait(bar_ds + 8 * b, phase, a.limit)) {
                     failed = true;
                     break;
                 }
                 fence_after();
-                const uint32_t s1 = smem + S::kRing + st * 2 * S::kStream;
-                const uint64_t m1 = smem_desc(s1, kTile * 128), m2 = smem_desc(s1 + S::kStream, kTile * 128);
-                if (KEYS) {
-#pragma unroll
-                    for (int k = 0; k < kTile / 16; ++k) mma_ts(t_out1, t_s + kTile * b + 8 * k, desc_at(m2, k * 2048), kDesc, i > 0 || k > 0);
-                }
 #pragma unroll
                 for (int k = 0; k < kTile / 16; ++k)
                     mma_ts(KEYS ? t_out2 : t_out1, t_dp + kTile * b + 8 * k, desc_at(m1, k * 2048), kDesc, i > 0 || k > 0);
-                mma_commit(bar_out + 8 * b);
+                mma_commit(KEYS ? bar_free_dp + 8 * b : bar_free_s + 8 * b);
                 mma_commit(bar_empty + 8 * st);
                 if (i == n - 1) mma_commit(bar_last);
             }
@@ -426,8 +483,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
         }
     } else {
-        // ---- P and dS: thread = stationary row, buffer b = its warpgroup
-        const int b = warp >> 2;
+        // ---- P and dS: thread = stationary row; the two groups take the tiles in turn
+        const int group = warp >> 2;
         const int r = threadIdx.x & (kRows - 1);
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;
         const int64_t token = (int64_t)(KEYS ? sq.k0 : sq.q0) + row0 + r;
@@ -438,27 +495,24 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (v != -INFINITY) own_l = kLift - v * kLog2e;
             own_d = -kLower * __ldg(a.delta + at);
         }
-        int done = 0;
-        for (int i = b; i < n; i += 2) {
+        for (int i = group; i < n; i += 2) {
+            const int b = i % kBuffers;
+            const uint32_t phase = (i / kBuffers) & 1;
+            const uint32_t ts = t_s + kTile * b + lanes, td = t_dp + kTile * b + lanes;
             // (the second wait is over by then; it is there for the vectors, which ordinary stores wrote)
-            if (!bar_wait_warp(bar_s + 8 * b, done & 1, a.limit) ||
-                (KEYS && !bar_wait_warp(bar_full + 8 * (i % kStages), (i / kStages) & 1, a.limit))) {
+            if (!bar_wait_warp(bar_s + 8 * b, phase, a.limit) || (KEYS && !bar_wait_warp(bar_full + 8 * (i % kStages), (i / kStages) & 1, a.limit))) {
                 failed = true;
                 break;
             }
             fence_after();
-            uint32_t s[kTile], d[kTile];
-            tmem_load32(t_s + kTile * b + lanes, s);
-            tmem_load32(t_s + kTile * b + lanes + 32, s + 32);
-            tmem_load32(t_dp + kTile * b + lanes, d);
-            tmem_load32(t_dp + kTile * b + lanes + 32, d + 32);
-            wait_loads();
-            after_loads32(s), after_loads32(s + 32), after_loads32(d), after_loads32(d + 32);
+            uint32_t p[kTile];
+            tmem_load32(ts, p);
+            tmem_load32(ts + 32, p + 32);
             const int row = tile_row(i);
             uint64_t seen = ~0ull;
             if (KEYS) {
                 // key j = row0 + r, query at position p = shift + row + c: seen iff p >= j and (p < j + window or j < sinks)
-                const int p0 = shift + row, j = row0 + r;
+                const int p0 = shift + row, j = row0 + r;  // (positions)
                 if (p0 < row0 + kRows - 1 || (p0 + kTile - 1 >= row0 + a.window && row0 + kRows > a.sinks)) {
                     const int from = min(max(j - p0, 0), 64);
                     const int upto = j < a.sinks ? 64 : min(max(j + a.window - p0, 0), 64);
@@ -466,36 +520,56 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             } else {
                 // query at p, key j = row + c: seen iff j <= p and (j > p - window or j < sinks)
-                const int p = p_low + r;
+                const int at = p_low + r;
                 if (row + kTile - 1 > p_low || (row <= p_low + kRows - 1 - a.window && row + kTile > a.sinks)) {
-                    const int upto = min(max(p + 1 - row, 0), 64), from = min(max(p - a.window + 1 - row, 0), 64);
+                    const int upto = min(max(at + 1 - row, 0), 64), from = min(max(at - a.window + 1 - row, 0), 64);
                     const int keep = min(max(a.sinks - row, 0), 64);
                     const uint64_t near = from < 64 ? ~0ull << from : 0ull, kept = keep < 64 ? (1ull << keep) - 1 : ~0ull;
                     seen = (near | kept) & (upto < 64 ? (1ull << upto) - 1 : ~0ull);
                 }
             }
             const uint32_t vec = smem + S::kVec + (i % kStages) * S::kVectors;
-            const uint32_t ts = t_s + kTile * b + lanes, td = t_dp + kTile * b + lanes;
-            if (__all_sync(0xffffffffu, seen == ~0ull))
-                weights<T, KEYS, false>(s, d, ts, td, 0, vec, own_l, own_d, a.scale_log2);
+            const bool masked = !__all_sync(0xffffffffu, seen == ~0ull);
+            wait_loads();
+            after_loads32(p), after_loads32(p + 32);
+            if (masked)
+                weights<T, KEYS, true>(p, ts, seen, vec, own_l, a.scale_log2);
             else
-                weights<T, KEYS, true>(s, d, ts, td, seen, vec, own_l, own_d, a.scale_log2);
+                weights<T, KEYS, false>(p, ts, seen, vec, own_l, a.scale_log2);
+            if (KEYS) {
+                wait_stores();
+                fence_before();
+                bar_arrive(bar_p + 8 * b);
+            }
+            if (!bar_wait_warp(bar_dp + 8 * b, phase, a.limit)) {
+                failed = true;
+                break;
+            }
+            fence_after();
+            uint32_t d[kTile];
+            tmem_load32(td, d);
+            tmem_load32(td + 32, d + 32);
+            wait_loads();
+            after_loads32(d), after_loads32(d + 32);
+            if (masked)
+                weight_gradients<T, KEYS, true>(p, d, td, seen, vec + 4 * kTile, own_d);
+            else
+                weight_gradients<T, KEYS, false>(p, d, td, seen, vec + 4 * kTile, own_d);
             wait_stores();
             fence_before();
-            bar_arrive(bar_p + 8 * b);
-            ++done;
+            bar_arrive(bar_ds + 8 * b);
         }
         // ---- outputs: keys kernel: one warpgroup writes dV, the other dK; queries kernel: each half of dQ's columns
         if (n > 0 && !failed) {
             failed = !bar_wait_warp(bar_last, 0, a.limit);
             fence_after();
         }
-        const uint32_t t_out = KEYS && b == 1 ? t_out2 : t_out1;
-        const float factor = KEYS && b == 0 ? kLower : a.scale;
-        T* out = b == 1 && KEYS ? static_cast<T*>(a.out2) + token * a.out2_token + (int64_t)head * a.out2_head
+        const uint32_t t_out = KEYS && group == 1 ? t_out2 : t_out1;
+        const float factor = KEYS && group == 0 ? kLower : a.scale;
+        T* out = group == 1 && KEYS ? static_cast<T*>(a.out2) + token * a.out2_token + (int64_t)head * a.out2_head
                                 : static_cast<T*>(a.out1) + token * a.out1_token + (int64_t)head * a.out1_head;
-        float* part = partial < 0 ? nullptr : a.partial + ((partial * 2 + b) * kRows + r) * DP;
-        const int c0 = KEYS ? 0 : b * (DP / 2), c1 = KEYS ? DP : c0 + DP / 2;
+        float* part = partial < 0 ? nullptr : a.partial + ((partial * 2 + group) * kRows + r) * DP;
+        const int c0 = KEYS ? 0 : group * (DP / 2), c1 = KEYS ? DP : c0 + DP / 2;
 #pragma unroll 1
         for (int c = c0; c < c1; c += 32) {
             uint32_t o[32];
@@ -536,13 +610,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // The sums of a first-tokens tile: what its own window holds, then its far pieces in order. One block per (sequence by its
-// first far slot, key tile, key head, which of dV and dK); thread = 4 values.
+// first far slot, key tile, key head, which of dV and dK, slice of 16 rows); thread = 4 values.
+constexpr int kJoinSlices = 8;
 template <typename T, int DP>
 __global__ void __launch_bounds__(256) window_backward_join_kernel(const Params a) {
     const int lane = threadIdx.x & 31;
     int64_t x = blockIdx.x;
-    const int which = (int)(x & 1), head = (int)((x >> 1) % a.kv_heads);
-    x = (x >> 1) / a.kv_heads;
+    const int slice = (int)(x % kJoinSlices), which = (int)(x / kJoinSlices & 1), head = (int)((x / kJoinSlices >> 1) % a.kv_heads);
+    x = (x / kJoinSlices >> 1) / a.kv_heads;
     const int tile = (int)(x % a.far_tiles), far = (int)(x / a.far_tiles);
     const RaggedBlock fb = far_block(a.r, far, a.chunk, lane);
     if (fb.b < 0 || fb.index != 0) return;
@@ -553,7 +628,8 @@ __global__ void __launch_bounds__(256) window_backward_join_kernel(const Params 
     if (v.pieces == 0) return;
     const float factor = which == 0 ? (std::is_same<T, __half>::value ? 1.0f / 256.0f : 1.0f) : a.scale;
     const auto part = [&](int64_t f) { return a.partial + ((((f * a.far_tiles + tile) * a.kv_heads + head) * 2 + which) * (int64_t)kRows) * DP; };
-    for (int i = threadIdx.x * 4; i < kRows * DP; i += 256 * 4) {
+    constexpr int kSlice = kRows / kJoinSlices * DP;
+    for (int i = slice * kSlice + threadIdx.x * 4; i < (slice + 1) * kSlice; i += 256 * 4) {
         const int r = i / DP, c = i % DP;
         if (row0 + r >= sq.lk || c >= a.dim) continue;
         float4 s = *reinterpret_cast<const float4*>(part((int64_t)a.far_slots + far) + i);
@@ -618,7 +694,7 @@ cudaError_t launch(cudaStream_t s, const AttentionArgs& a, void* buffer) {
     const int64_t key_blocks = ragged_slots(a.total_k, a.batch, a.k_offsets != nullptr, kRows) + (int64_t)p.far_slots * p.far_tiles;
     window_backward_kernel<T, DP, true><<<(unsigned)(key_blocks * a.kv_heads), kThreads, S::kTotal, s>>>(k_rows, v_rows, q_tile, go_tile, pk);
     if (p.far_tiles > 0)
-        window_backward_join_kernel<T, DP><<<(unsigned)((int64_t)p.far_slots * p.far_tiles * a.kv_heads * 2), 256, 0, s>>>(pk);
+        window_backward_join_kernel<T, DP><<<(unsigned)((int64_t)p.far_slots * p.far_tiles * a.kv_heads * 2 * kJoinSlices), 256, 0, s>>>(pk);
     p.out1 = a.dq.p, p.out1_token = a.dq.token, p.out1_head = a.dq.head;
     p.slots = ragged_slots(a.total_q, a.batch, a.q_offsets != nullptr, kRows);
     window_backward_kernel<T, DP, false><<<(unsigned)((int64_t)p.slots * a.q_heads), kThreads, S::kTotal, s>>>(q_rows, go_rows, k_tile, v_tile, p);
