@@ -152,19 +152,6 @@ __global__ void __launch_bounds__(kThreads) window_decode_kernel(const Params a)
     const int tile0 = (int)((int64_t)tiles * split / a.splits), tile1 = (int)((int64_t)tiles * (split + 1) / a.splits);
     const int mine = tile0 + warp < tile1 ? (tile1 - tile0 - warp + kWarps - 1) / kWarps : 0;
 
-    // the query heads as the left operand: lane holds rows lane / 4 and + 8, columns 2 * (lane % 4) and + 8 of every step
-    uint32_t q[kSteps][4];
-    {
-        const T* base = static_cast<const T*>(a.q) + (int64_t)b * a.q_token;
-#pragma unroll
-        for (int k = 0; k < kSteps; ++k)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const int row = (lane >> 2) + 8 * (x & 1), c = 16 * k + 2 * (lane & 3) + 8 * (x >> 1);
-                q[k][x] = row < rows && c < a.dim ? __ldg(reinterpret_cast<const unsigned*>(base + (int64_t)(head0 + row) * a.q_head + c)) : 0u;
-            }
-    }
-
     // Lanes 0 .. 15 look up the place of the tile's key `lane`: page (-1: not seen) and token of the page.
     const auto lookup = [&](int i, int& page, int& at) {
         page = -1, at = 0;
@@ -213,6 +200,19 @@ __global__ void __launch_bounds__(kThreads) window_decode_kernel(const Params a)
         commit_copies();
     }
     lookup(R::kStages - 1, page, at);
+    // the query heads as the left operand: lane holds rows lane / 4 and + 8, columns 2 * (lane % 4) and + 8 of every step
+    uint32_t q[kSteps][4];
+    {
+        const T* base = static_cast<const T*>(a.q) + (int64_t)b * a.q_token;
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const int row = (lane >> 2) + 8 * (x & 1), c = 16 * k + 2 * (lane & 3) + 8 * (x >> 1);
+                q[k][x] = row < rows && c < a.dim ? __ldg(reinterpret_cast<const unsigned*>(base + (int64_t)(head0 + row) * a.q_head + c)) : 0u;
+            }
+    }
+
     for (int i0 = 0; i0 < mine; i0 += R::kStages) {
 #pragma unroll
         for (int s = 0; s < R::kStages; ++s) {
@@ -371,16 +371,22 @@ int64_t decode_items(const DecodeArgs& a) {
     return (int64_t)a.batch * a.kv_heads * ((group + kHeads - 1) / kHeads);
 }
 
-// Parts per sequence and key head: as many as fill the GPU four times over (two blocks per SM), of at least 64 keys (a tile
-// per warp) each.
+// Parts per sequence and key head. A part costs its keys and about 250 more (its start, its first loads, the join: fitted to
+// 64 sequences x 8 key heads x 4100 keys, where 1, 2, 3 parts took 196, 206, 217 us); two blocks run per SM, so the launch costs
+// its whole rounds of blocks. At least 64 keys (a tile per warp) each. Up to 8 parts join as a cluster; more take the work buffer
+// and a second launch (200 keys' worth) and only come into question when an eighth is still long.
 int decode_splits(const DecodeArgs& a) {
-    const int64_t room = a.max_pages * a.page_size;
+    const int64_t room = a.max_pages * a.page_size, items = decode_items(a);
     const int64_t most = (int64_t)a.window + a.sinks < room ? (int64_t)a.window + a.sinks : room;
-    const int64_t by_work = (most + 63) / 64, by_fill = (8LL * a.sm_count + decode_items(a) - 1) / (decode_items(a) > 0 ? decode_items(a) : 1);
-    int64_t s = by_work < by_fill ? by_work : by_fill;
-    // a cluster's blocks start together and need no second launch: more only pay when a part is still long (1024 keys)
-    if (s > kCluster && most / kCluster < 1024) s = kCluster;
-    return (int)(s < 1 ? 1 : s);
+    const int64_t slots = 2LL * a.sm_count;
+    int best = 1;
+    int64_t least = INT64_MAX;
+    for (int s = 1; s <= 64; s = s < kCluster ? s + 1 : 2 * s) {
+        if (s > 1 && (most < 64LL * s || (s > kCluster && most / kCluster < 1024))) break;
+        const int64_t cost = (items * s + slots - 1) / slots * (most / s + 250) + (s > kCluster ? 200 : 0);
+        if (cost < least) least = cost, best = s;
+    }
+    return best;
 }
 
 template <typename T, int DP>
