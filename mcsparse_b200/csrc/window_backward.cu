@@ -2,9 +2,13 @@
 // dS = P * (dP - delta), delta = rowsum(dO * O):
 //   keys kernel     one block per 128 keys and key head: S^T = K Q^T, dP^T = V dO^T, dV += P^T dO, dK += dS^T Q over the query
 //                   tiles of 64 that see them, for all query heads that share the keys (their sum stays in tensor memory);
-//   queries kernel  one block per 128 queries and query head: S = Q K^T, dP = dO V^T, dQ += dS K over the key tiles of 64.
+//   queries kernel  one block per 128 queries and query head: S = Q K^T, dP = dO V^T, dQ += dS K over the key tiles of 64, and
+//                   M += P K, the mean of the keys.
+// delta from the rounded O is off by up to half a step of O's type times |dO|, which reaches dQ and dK as much as the rounding of
+// dS does. The sum of a row of dS would be 0 with the exact delta; with the other one it is the difference. So the queries kernel,
+// which runs first, takes the sum e of its rows of dS (fp32), returns scale * (dQ - e M), and leaves delta + e for the keys kernel.
 // Both are one kernel template: 128 stationary rows against a stream of 64-row tiles. S and dP have two buffers in tensor
-// memory (three where dV, dK or dQ leave room); two groups of 128 threads, one row each, take the tiles in turn and make P
+// memory (three where the sums leave room); two groups of 128 threads, one row each, take the tiles in turn and make P
 // and dS of them in place, in 16 bits, while the tensor cores work on the other buffers; P and dS enter the second products
 // from tensor memory, P as soon as it is there. Two kernels compute S and dP twice (7 products
 // instead of 5), which buys sums without atomics: equal inputs give equal bits, and nothing is kept in fp32 in HBM.
@@ -56,6 +60,7 @@ struct Params {
     int64_t out1_token, out1_head, out2_token, out2_head;
     // the first tokens' far queries
     int chunk, far_slots, far_tiles;
+    float* delta_out;  // queries kernel: the exact delta, may be the same array
     float* partial;  // [2 * far_slots][far_tiles][kv_heads][2][kRows][DP]: far pieces, then what their own windows hold
     long long limit;
     int* fault;
@@ -142,7 +147,7 @@ __device__ __forceinline__ void column_values(uint32_t vec, int c, float own, fl
         v[0] = v[1] = v[2] = v[3] = own;
 }
 
-// 64 scores of a row -> its weights, in place; keys kernel: also, in 16 bits, into the first half of the scores' columns. `vec` /
+// 64 scores of a row -> its weights, in place, and in 16 bits into the first half of the scores' columns. `vec` /
 // own_l: -lse (base 2) of the columns / the row. MASK: column c counts iff bit c of `seen` is set.
 template <typename T, bool KEYS, bool MASK>
 __device__ __forceinline__ void weights(uint32_t* p, uint32_t ts, uint64_t seen, uint32_t vec, float own_l, float scale_log2) {
@@ -165,19 +170,21 @@ __device__ __forceinline__ void weights(uint32_t* p, uint32_t ts, uint64_t seen,
                     p0 = bits >> (c + x) & 1 ? p0 : 0.0f;
                     p1 = bits >> (c + x + 1) & 1 ? p1 : 0.0f;
                 }
-                if (KEYS) w[(c + x) >> 1] = pack2<T>(p0, p1);
+                w[(c + x) >> 1] = pack2<T>(p0, p1);
                 p[at] = __float_as_uint(p0), p[at + 1] = __float_as_uint(p1);
             }
         }
-        if (KEYS) tmem_store16(ts + 16 * h, w);
+        tmem_store16(ts + 16 * h, w);
     }
 }
 
 // dS = P * (dP - delta) of a row, in 16 bits into the first half of dP's columns. (An unseen pair is 0 also where dP is NaN.)
+// Returns the sum of the row's dS in fp32.
 template <typename T, bool KEYS, bool MASK>
-__device__ __forceinline__ void weight_gradients(const uint32_t* p, const uint32_t* d, uint32_t td, uint64_t seen, uint32_t vec, float own_d) {
+__device__ __forceinline__ float weight_gradients(const uint32_t* p, const uint32_t* d, uint32_t td, uint64_t seen, uint32_t vec, float own_d) {
     constexpr float kLower = std::is_same<T, __half>::value ? 1.0f / 256.0f : 1.0f;
     const uint64_t lower2 = pair(kLower, kLower);
+    uint64_t sum = pair(0.0f, 0.0f);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         uint32_t w[16];
@@ -196,11 +203,15 @@ __device__ __forceinline__ void weight_gradients(const uint32_t* p, const uint32
                     g0 = bits >> (c + x) & 1 ? g0 : 0.0f;
                     g1 = bits >> (c + x + 1) & 1 ? g1 : 0.0f;
                 }
+                if (!KEYS) sum = add2(sum, pair(g0, g1));
                 w[(c + x) >> 1] = pack2<T>(g0, g1);
             }
         }
         tmem_store16(td + 16 * h, w);
     }
+    float a, b;
+    unpair(sum, a, b);
+    return a + b;
 }
 
 // KEYS: stationary K, V; streamed Q, dO. Otherwise: stationary Q, dO; streamed K, V.
@@ -212,8 +223,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     using S = Smem<DP>;
     constexpr bool kHalf = std::is_same<T, __half>::value;
     constexpr int kBlocks = DP / 64;
-    constexpr int kBuffers = KEYS && DP == 128 ? 2 : 3;
-    static_assert(kBuffers * 2 * kTile + (KEYS ? 2 : 1) * DP <= 512, "columns of tensor memory");
+    constexpr int kBuffers = DP == 128 ? 2 : 3;
+    static_assert(kBuffers * 2 * kTile + 2 * DP <= 512, "columns of tensor memory");
     // fp16 P is held 2^8 times too large (at most 256): weights below 2^-14 would lose bits to fp16's subnormal numbers. The
     // factor leaves dS through the other factor of its product and dV at the end.
     constexpr float kLift = kHalf ? 8.0f : 0.0f, kLower = kHalf ? 1.0f / 256.0f : 1.0f;
@@ -221,12 +232,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t smem = (smem_u32(smem_raw) + 1023) & ~1023u;
     const int warp = uniform((int)(threadIdx.x >> 5)), lane = threadIdx.x & 31;
     // barriers: stationary operands; of every stage: there, clear, done with; of the buffers: S ready, dP ready, P ready, dS ready,
-    // S's columns free, dP's columns free; the last product done; the ends of the two issuing warps
+    // S's columns free, dP's columns free; the last product done; the groups' exchange; the ends of the two issuing warps
     const uint32_t bars = smem + S::kBars;
     const uint32_t bar_fixed = bars, bar_full = bars + 8, bar_clear = bar_full + 8 * kStages, bar_empty = bar_clear + 8 * kStages,
                    bar_s = bar_empty + 8 * kStages, bar_dp = bar_s + 8 * kBuffers, bar_p = bar_dp + 8 * kBuffers, bar_ds = bar_p + 8 * kBuffers,
                    bar_free_s = bar_ds + 8 * kBuffers, bar_free_dp = bar_free_s + 8 * kBuffers, bar_last = bar_free_dp + 8 * kBuffers,
-                   bar_end = bar_last + 8, slot = bar_end + 16;
+                   bar_x = bar_last + 8, bar_end = bar_x + 8, slot = bar_end + 16;
 
     // ---- the block's rows and its stream
     const int heads = KEYS ? a.kv_heads : a.q_heads;
@@ -299,7 +310,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             bar_init(bar_s + 8 * i, 1), bar_init(bar_dp + 8 * i, 1), bar_init(bar_p + 8 * i, kRows), bar_init(bar_ds + 8 * i, kRows);
             bar_init(bar_free_s + 8 * i, 1), bar_init(bar_free_dp + 8 * i, 1);
         }
-        bar_init(bar_last, 1), bar_init(bar_end, 1), bar_init(bar_end + 8, 1);
+        bar_init(bar_last, 1), bar_init(bar_x, 2 * kRows), bar_init(bar_end, 1), bar_init(bar_end + 8, 1);
         bar_init_fence();
     }
     fence_before();
@@ -308,7 +319,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t tmem;
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(slot));
     tmem = uniform(tmem);
-    // tensor memory: the buffers of S and dP, 64 columns each, then the sums (dV and dK, or dQ)
+    // tensor memory: the buffers of S and dP, 64 columns each, then the sums (dV and dK, or M and dQ)
     const uint32_t t_s = tmem, t_dp = tmem + kBuffers * kTile, t_out1 = tmem + 2 * kBuffers * kTile, t_out2 = t_out1 + DP;
     bool failed = false;
 
@@ -397,13 +408,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                     mma_ss(t_s + kTile * b, desc_at(f1, (k >> 2) * (kRows * 128) + (k & 3) * 32), desc_at(m1, (k >> 2) * (kTile * 128) + (k & 3) * 32),
                            kDesc | a.negate, k > 0);
                 mma_commit(bar_s + 8 * b);
-                if (KEYS && i >= kBuffers) {  // (queries kernel: S and dP are free together)
-                    if (!bar_wait(bar_free_dp + 8 * b, before, a.limit)) {
-                        failed = true;
-                        break;
-                    }
-                    fence_after();
+                if (i >= kBuffers && !bar_wait(bar_free_dp + 8 * b, before, a.limit)) {
+                    failed = true;
+                    break;
                 }
+                fence_after();
 #pragma unroll
                 for (int k = 0; k < DP / 16; ++k)
                     mma_ss(t_dp + kTile * b, desc_at(f2, (k >> 2) * (kRows * 128) + (k & 3) * 32), desc_at(m2, (k >> 2) * (kTile * 128) + (k & 3) * 32),
@@ -417,7 +426,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
     } else if (warp == kSumWarp) {
-        // ---- dV and dK, or dQ, issued by one thread
+        // ---- dV and dK, or M and dQ, issued by one thread
         constexpr uint32_t kDesc = mma_desc(!kHalf, DP, true);
         if (n > 0 && elect()) {
             for (int i = 0; i < n; ++i) {
@@ -425,20 +434,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const uint32_t phase = (i / kBuffers) & 1;
                 const uint32_t s1 = smem + S::kRing + st * 2 * S::kStream;
                 const uint64_t m1 = smem_desc(s1, kTile * 128), m2 = smem_desc(s1 + S::kStream, kTile * 128);
-                if (!bar_wait(bar_clear + 8 * st, (i / kStages) & 1, a.limit)) {
+                if (!bar_wait(bar_clear + 8 * st, (i / kStages) & 1, a.limit) || !bar_wait(bar_p + 8 * b, phase, a.limit)) {
                     failed = true;
                     break;
                 }
-                if (KEYS) {
-                    if (!bar_wait(bar_p + 8 * b, phase, a.limit)) {
-                        failed = true;
-                        break;
-                    }
-                    fence_after();
+                fence_after();
 #pragma unroll
-                    for (int k = 0; k < kTile / 16; ++k) mma_ts(t_out1, t_s + kTile * b + 8 * k, desc_at(m2, k * 2048), kDesc, i > 0 || k > 0);
-                    mma_commit(bar_free_s + 8 * b);
-                }
+                for (int k = 0; k < kTile / 16; ++k)
+                    mma_ts(t_out1, t_s + kTile * b + 8 * k, desc_at(KEYS ? m2 : m1, k * 2048), kDesc, i > 0 || k > 0);
+                mma_commit(bar_free_s + 8 * b);
                 if (!bar_wait(bar_ds + 8 * b, phase, a.limit)) {
                     failed = true;
                     break;
@@ -446,8 +450,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 fence_after();
 #pragma unroll
                 for (int k = 0; k < kTile / 16; ++k)
-                    mma_ts(KEYS ? t_out2 : t_out1, t_dp + kTile * b + 8 * k, desc_at(m1, k * 2048), kDesc, i > 0 || k > 0);
-                mma_commit(KEYS ? bar_free_dp + 8 * b : bar_free_s + 8 * b);
+                    mma_ts(t_out2, t_dp + kTile * b + 8 * k, desc_at(m1, k * 2048), kDesc, i > 0 || k > 0);
+                mma_commit(bar_free_dp + 8 * b);
                 mma_commit(bar_empty + 8 * st);
                 if (i == n - 1) mma_commit(bar_last);
             }
@@ -495,6 +499,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (v != -INFINITY) own_l = kLift - v * kLog2e;
             own_d = -kLower * __ldg(a.delta + at);
         }
+        float e = 0.0f;  // queries kernel: the sum of the row's dS
         for (int i = group; i < n; i += 2) {
             const int b = i % kBuffers;
             const uint32_t phase = (i / kBuffers) & 1;
@@ -536,11 +541,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 weights<T, KEYS, true>(p, ts, seen, vec, own_l, a.scale_log2);
             else
                 weights<T, KEYS, false>(p, ts, seen, vec, own_l, a.scale_log2);
-            if (KEYS) {
-                wait_stores();
-                fence_before();
-                bar_arrive(bar_p + 8 * b);
-            }
+            wait_stores();
+            fence_before();
+            bar_arrive(bar_p + 8 * b);
             if (!bar_wait_warp(bar_dp + 8 * b, phase, a.limit)) {
                 failed = true;
                 break;
@@ -552,31 +555,51 @@ __global__ void __launch_bounds__(kThreads, 1)
             wait_loads();
             after_loads32(d), after_loads32(d + 32);
             if (masked)
-                weight_gradients<T, KEYS, true>(p, d, td, seen, vec + 4 * kTile, own_d);
+                e += weight_gradients<T, KEYS, true>(p, d, td, seen, vec + 4 * kTile, own_d);
             else
-                weight_gradients<T, KEYS, false>(p, d, td, seen, vec + 4 * kTile, own_d);
+                e += weight_gradients<T, KEYS, false>(p, d, td, seen, vec + 4 * kTile, own_d);
             wait_stores();
             fence_before();
             bar_arrive(bar_ds + 8 * b);
         }
-        // ---- outputs: keys kernel: one warpgroup writes dV, the other dK; queries kernel: each half of dQ's columns
+        // ---- outputs: keys kernel: one group writes dV, the other dK; queries kernel: each half of dQ's columns
         if (n > 0 && !failed) {
-            failed = !bar_wait_warp(bar_last, 0, a.limit);
+            if (!KEYS) {  // the row's sum over the tiles of both groups
+                const uint32_t words = smem + S::kVec;
+                asm volatile("st.shared.f32 [%0], %1;" ::"r"(words + 4 * (kRows * group + r)), "f"(e) : "memory");
+                bar_arrive(bar_x);
+                failed = !bar_wait_warp(bar_x, 0, a.limit);
+                float e0, e1;
+                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(e0) : "r"(words + 4 * r) : "memory");
+                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(e1) : "r"(words + 4 * (kRows + r)) : "memory");
+                e = e0 + e1;
+                if (group == 0 && r < rows && !failed) a.delta_out[(int64_t)head * a.r.total_q + token] = e - own_d / kLower;
+            }
+            failed = !bar_wait_warp(bar_last, 0, a.limit) || failed;
             fence_after();
         }
-        const uint32_t t_out = KEYS && group == 1 ? t_out2 : t_out1;
+        const float less = -e * kLower;
         const float factor = KEYS && group == 0 ? kLower : a.scale;
         T* out = group == 1 && KEYS ? static_cast<T*>(a.out2) + token * a.out2_token + (int64_t)head * a.out2_head
-                                : static_cast<T*>(a.out1) + token * a.out1_token + (int64_t)head * a.out1_head;
+                                    : static_cast<T*>(a.out1) + token * a.out1_token + (int64_t)head * a.out1_head;
         float* part = partial < 0 ? nullptr : a.partial + ((partial * 2 + group) * kRows + r) * DP;
         const int c0 = KEYS ? 0 : group * (DP / 2), c1 = KEYS ? DP : c0 + DP / 2;
 #pragma unroll 1
         for (int c = c0; c < c1; c += 32) {
             uint32_t o[32];
             if (n > 0 && !failed) {
-                tmem_load32(t_out + lanes + c, o);
-                wait_loads();
-                after_loads32(o);
+                tmem_load32((KEYS && group == 0 ? t_out1 : t_out2) + lanes + c, o);
+                if (!KEYS) {
+                    uint32_t m[32];
+                    tmem_load32(t_out1 + lanes + c, m);
+                    wait_loads();
+                    after_loads32(o), after_loads32(m);
+#pragma unroll
+                    for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(fmaf(less, __uint_as_float(m[x]), __uint_as_float(o[x])));
+                } else {
+                    wait_loads();
+                    after_loads32(o);
+                }
             } else {
 #pragma unroll
                 for (int x = 0; x < 32; ++x) o[x] = 0u;
@@ -691,13 +714,14 @@ cudaError_t launch(cudaStream_t s, const AttentionArgs& a, void* buffer) {
     Params pk = p;
     pk.out1 = a.dv.p, pk.out1_token = a.dv.token, pk.out1_head = a.dv.head;
     pk.out2 = a.dk.p, pk.out2_token = a.dk.token, pk.out2_head = a.dk.head;
+    p.out1 = a.dq.p, p.out1_token = a.dq.token, p.out1_head = a.dq.head;
+    p.slots = ragged_slots(a.total_q, a.batch, a.q_offsets != nullptr, kRows);
+    p.delta_out = delta;
+    window_backward_kernel<T, DP, false><<<(unsigned)((int64_t)p.slots * a.q_heads), kThreads, S::kTotal, s>>>(q_rows, go_rows, k_tile, v_tile, p);
     const int64_t key_blocks = ragged_slots(a.total_k, a.batch, a.k_offsets != nullptr, kRows) + (int64_t)p.far_slots * p.far_tiles;
     window_backward_kernel<T, DP, true><<<(unsigned)(key_blocks * a.kv_heads), kThreads, S::kTotal, s>>>(k_rows, v_rows, q_tile, go_tile, pk);
     if (p.far_tiles > 0)
         window_backward_join_kernel<T, DP><<<(unsigned)((int64_t)p.far_slots * p.far_tiles * a.kv_heads * 2 * kJoinSlices), 256, 0, s>>>(pk);
-    p.out1 = a.dq.p, p.out1_token = a.dq.token, p.out1_head = a.dq.head;
-    p.slots = ragged_slots(a.total_q, a.batch, a.q_offsets != nullptr, kRows);
-    window_backward_kernel<T, DP, false><<<(unsigned)((int64_t)p.slots * a.q_heads), kThreads, S::kTotal, s>>>(q_rows, go_rows, k_tile, v_tile, p);
     return cudaGetLastError();
 }
 
