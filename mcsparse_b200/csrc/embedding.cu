@@ -323,17 +323,15 @@ __global__ void __launch_bounds__(256)
         finish_row<E, V>(table, a, row, first, lane, alpha, beta, sum);
 }
 
-// One block per chunk: if a sum starts in this chunk and goes on, its partials are added. The warps share out the slabs of
-// columns, kWays of them a slab's chunks (each adds its own in order, then the kWays sums are added in order).
-constexpr int kWays = 2;
-constexpr int kJoinThreads = 512;
+// One block per chunk: if a sum starts in this chunk and goes on, its partials are added in chunk order; a warp takes a slab of
+// columns at a time, eight partials on their way. (Few partials each, mostly: small blocks, of which many run at once.)
+constexpr int kJoinThreads = 256;
 
 template <typename E, int V>
 __global__ void __launch_bounds__(kJoinThreads)
     embedding_join_kernel(GradientArgs a, E* __restrict__ table, ScalarArg<float> alpha_arg, ScalarArg<float> beta_arg) {
-    constexpr int kPer = Columns<V>::kPer, kSlab = Columns<V>::kSlab, kDepth = 8, kSlabs = kJoinThreads / 32 / kWays;
-    __shared__ float s_sum[kJoinThreads / 32][kPer][32];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, way = warp % kWays;
+    constexpr int kPer = Columns<V>::kPer, kSlab = Columns<V>::kSlab, kDepth = 8;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t c = blockIdx.x;
     const int64_t k0 = c * a.chunk, k1 = k0 + a.chunk;
     grid_wait();  // the sums
@@ -350,36 +348,26 @@ __global__ void __launch_bounds__(kJoinThreads)
         beyond = min(last + step, beyond);
     }
     const float alpha = alpha_arg.get(), beta = beta_arg.get();
-    for (int slab0 = 0; slab0 < a.slabs; slab0 += kSlabs) {  // block-uniform
-        const int64_t first = (int64_t)(slab0 + warp / kWays) * kSlab;
+    for (int slab = warp; slab < a.slabs; slab += kJoinThreads / 32) {
+        const int64_t first = (int64_t)slab * kSlab;
         float sum[kPer];
 #pragma unroll
         for (int i = 0; i < kPer; ++i) sum[i] = 0.0f;
-        if (way == 0) load_columns<float, V>(a.partial + (2 * c + 1) * a.width, first, a.width, lane, sum);
-        for (int64_t d = c + 1 + way; d <= last; d += kWays * kDepth) {
+        load_columns<float, V>(a.partial + (2 * c + 1) * a.width, first, a.width, lane, sum);
+        for (int64_t d = c + 1; d <= last; d += kDepth) {
             float v[kDepth][kPer];
 #pragma unroll
             for (int j = 0; j < kDepth; ++j) {
 #pragma unroll
                 for (int i = 0; i < kPer; ++i) v[j][i] = 0.0f;
-                if (d + kWays * j <= last) load_columns<float, V>(a.partial + (2 * (d + kWays * j)) * a.width, first, a.width, lane, v[j]);
+                if (d + j <= last) load_columns<float, V>(a.partial + (2 * (d + j)) * a.width, first, a.width, lane, v[j]);
             }
 #pragma unroll
             for (int j = 0; j < kDepth; ++j)
 #pragma unroll
                 for (int i = 0; i < kPer; ++i) sum[i] += v[j][i];
         }
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) s_sum[warp][i][lane] = sum[i];
-        __syncthreads();
-        if (way == 0) {
-#pragma unroll
-            for (int w = 1; w < kWays; ++w)
-#pragma unroll
-                for (int i = 0; i < kPer; ++i) sum[i] += s_sum[warp + w][i][lane];
-            finish_row<E, V>(table, a, row, first, lane, alpha, beta, sum);
-        }
-        __syncthreads();
+        finish_row<E, V>(table, a, row, first, lane, alpha, beta, sum);
     }
 }
 
@@ -387,7 +375,8 @@ __global__ void __launch_bounds__(kJoinThreads)
 
 constexpr int kSortCluster = 8;
 constexpr int kSortThreads = 1024;
-constexpr int kSortRounds = 16;  // items per thread
+constexpr int kSortRounds = 16;  // items per thread, at most
+constexpr int kFewRounds = 2;    // the same, of the kernel for few tokens (registers and predicated code for 16 cost it 3 us)
 constexpr int64_t kSortMost = (int64_t)kSortCluster * kSortThreads * kSortRounds;
 constexpr int kMostDigits = 512;
 
@@ -432,7 +421,22 @@ struct SortShared {
     unsigned part[32];
 };
 
-// Items are owned in ascending order by (block, warp, round, lane), so that equal keys keep their order.
+// Lanes with the same digit as the calling one (a lane that is not live: nobody's). One vote per bit: __match_any_sync visits the
+// distinct digits one after the other, up to 32 of them (four times as long on ids as text has them).
+__device__ __forceinline__ unsigned same_digit(unsigned d, bool live, int bits) {
+    unsigned peers = __ballot_sync(0xffffffffu, live);
+#pragma unroll
+    for (int b = 0; b < 9; ++b) {
+        if (b < bits) {
+            const unsigned votes = __ballot_sync(0xffffffffu, d >> b & 1);
+            peers &= d >> b & 1 ? votes : ~votes;
+        }
+    }
+    return peers;
+}
+
+// Items are owned in ascending order by (block, warp, round, lane), so that equal keys keep their order. At most R rounds.
+template <int R>
 __device__ __forceinline__ void sort_block(const SortArgs& a, SortShared& s, int rank) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rounds = (int)((a.count + (int64_t)a.sorters * kSortThreads - 1) / ((int64_t)a.sorters * kSortThreads));
@@ -440,12 +444,13 @@ __device__ __forceinline__ void sort_block(const SortArgs& a, SortShared& s, int
     const int digits = 1 << a.bits;
     for (int pass = 0; pass < a.passes; ++pass) {
         const int shift = pass * a.bits, to = pass & 1;
-        const uint2* in = a.sorted[to ^ 1];
+        const uint2* in = to ? a.sorted[0] : a.sorted[1];
+        uint2* const out = to ? a.sorted[1] : a.sorted[0];
         for (int i = threadIdx.x; i < 32 * kMostDigits / 2; i += kSortThreads) reinterpret_cast<unsigned*>(s.warp)[i] = 0u;
-        uint2 pair[kSortRounds];
-        unsigned ranks[kSortRounds / 2];  // place of an item among its warp's items with the same digit, two to a word
+        uint2 pair[R];
+        unsigned ranks[(R + 1) / 2];  // place of an item among its warp's items with the same digit, two to a word
 #pragma unroll
-        for (int r = 0; r < kSortRounds; ++r) {
+        for (int r = 0; r < R; ++r) {
             const int64_t t = begin + 32 * r;
             pair[r] = make_uint2(0u, 0u);
             // (the previous pass's output was written by other blocks of the cluster: read past L1)
@@ -453,11 +458,11 @@ __device__ __forceinline__ void sort_block(const SortArgs& a, SortShared& s, int
         }
         __syncthreads();
 #pragma unroll
-        for (int r = 0; r < kSortRounds; ++r) {
+        for (int r = 0; r < R; ++r) {
             if (r < rounds) {
                 const bool live = begin + 32 * r < a.count;
-                const unsigned d = live ? (pair[r].x >> shift) & (digits - 1) : 0xffffu;
-                const unsigned peers = __match_any_sync(0xffffffffu, d);
+                const unsigned d = (pair[r].x >> shift) & (digits - 1);
+                const unsigned peers = same_digit(d, live, a.bits);
                 const unsigned before = live ? s.warp[warp][d] : 0;
                 __syncwarp();
                 if (live && lane == __ffs(peers) - 1) s.warp[warp][d] = (unsigned short)(before + __popc(peers));
@@ -494,10 +499,13 @@ __device__ __forceinline__ void sort_block(const SortArgs& a, SortShared& s, int
         // places: all smaller digits of the cluster, then the same digit in the blocks before this one
         unsigned all = 0, before = 0;
         if ((int)threadIdx.x < digits) {
-            for (int r = 0; r < a.sorters; ++r) {
-                const unsigned c = load_remote(&s.total[threadIdx.x], r);
-                all += c;
-                if (r < rank) before += c;
+            unsigned c[kSortCluster];
+#pragma unroll
+            for (int r = 0; r < kSortCluster; ++r) c[r] = r < a.sorters ? load_remote(&s.total[threadIdx.x], r) : 0u;
+#pragma unroll
+            for (int r = 0; r < kSortCluster; ++r) {
+                all += c[r];
+                if (r < rank) before += c[r];
             }
         }
         unsigned inc = all;
@@ -513,11 +521,11 @@ __device__ __forceinline__ void sort_block(const SortArgs& a, SortShared& s, int
         if ((int)threadIdx.x < digits) s.base[threadIdx.x] = ahead + inc - all + before;
         __syncthreads();
 #pragma unroll
-        for (int r = 0; r < kSortRounds; ++r) {
+        for (int r = 0; r < R; ++r) {
             if (r < rounds && begin + 32 * r < a.count) {
                 const unsigned d = (pair[r].x >> shift) & (digits - 1);
                 const unsigned at = s.base[d] + s.warp[warp][d] + (r & 1 ? ranks[r / 2] >> 16 : ranks[r / 2] & 0xffffu);
-                a.sorted[to][at] = pair[r];
+                out[at] = pair[r];
             }
         }
         cluster_sync();  // the pass is in memory, and nobody reads this block's counts any more
@@ -586,10 +594,11 @@ __device__ __forceinline__ void fill_block(const SortArgs& a, float beta, uint8_
     if (bulk) asm volatile("cp.async.bulk.commit_group;\ncp.async.bulk.wait_group 0;" ::: "memory");
 }
 
+template <int R>
 __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(const SortArgs a) {
     __shared__ SortShared s;
     grid_release();
-    sort_block(a, s, (int)blockIdx.x);
+    sort_block<R>(a, s, (int)blockIdx.x);
 }
 
 // Runs beside the sort, which lets it start at once; it ends no earlier than the sort does, so that what waits for this launch
@@ -600,7 +609,7 @@ __global__ void __launch_bounds__(kSortThreads) embedding_fill_kernel(const Sort
     __shared__ __align__(16) uint8_t smem[kShared];
     grid_release();
     if ((int)blockIdx.x == 1 << a.fill_shift) {
-        sort_block(a, *reinterpret_cast<SortShared*>(smem), 0);
+        sort_block<kFewRounds>(a, *reinterpret_cast<SortShared*>(smem), 0);
         return;
     }
     const float beta = beta_arg.get();
@@ -727,7 +736,7 @@ cudaError_t launch_gradient(cudaStream_t s, const EmbeddingArgs& a, char* b) {
     const bool fill = a.beta.dev != nullptr || a.beta.host != 1.0f;
     int last = (so.passes - 1) & 1;
     // few tokens: one block sorts them in two rounds, as a further block of the other launch where there is one
-    so.sorters = a.count == 0 || !l.one_cluster ? 0 : a.count > 2 * kSortThreads ? kSortCluster : 1;
+    so.sorters = a.count == 0 || !l.one_cluster ? 0 : a.count > kFewRounds * kSortThreads ? kSortCluster : 1;
     const bool together = fill && so.sorters == 1;
     if (so.sorters > 0 && !together) {
         cudaLaunchConfig_t cfg = {};
@@ -739,7 +748,9 @@ cudaError_t launch_gradient(cudaStream_t s, const EmbeddingArgs& a, char* b) {
         attr.val.clusterDim.x = (unsigned)so.sorters, attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
         cfg.attrs = &attr;
         cfg.numAttrs = 1;
-        const cudaError_t e = cudaLaunchKernelEx(&cfg, embedding_sort_kernel, static_cast<const SortArgs>(so));
+        const bool few = a.count <= (int64_t)so.sorters * kSortThreads * kFewRounds;
+        const cudaError_t e = few ? cudaLaunchKernelEx(&cfg, embedding_sort_kernel<kFewRounds>, static_cast<const SortArgs>(so))
+                                  : cudaLaunchKernelEx(&cfg, embedding_sort_kernel<kSortRounds>, static_cast<const SortArgs>(so));
         if (e != cudaSuccess) return e;
     }
     if (!l.one_cluster) {
