@@ -304,7 +304,7 @@ typedef struct mcsparseB200Heads {
  * sequence sees; a value that is not finite in a key that some query sees may reach the sequence's other queries.
  * fp32 scores, softmax statistics and sums; 16-bit inputs: the softmax weights are rounded to the inputs' type for the
  * product with V, and O is rounded once. Asynchronous, no buffer, no allocation. The tensor-core kernels' waits are bounded by
- * the handle's device wait limit (mcsparseB200SetDeviceWaitLimit): a block that gives up leaves its rows unwritten, and the
+ * 64 times the handle's device wait limit (mcsparseB200SetDeviceWaitLimit): a block that gives up leaves its rows unwritten, and the
  * next forward or backward call on the handle returns MCSPARSE_STATUS_EXECUTION_FAILED once.
  */
 mcsparseStatus_t mcsparseB200WindowAttention(mcsparseHandle_t handle, mcsparseB200WindowDescr_t descr, int64_t batch,

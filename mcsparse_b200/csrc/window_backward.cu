@@ -16,6 +16,7 @@
 // The first tokens of a sequence are seen by all its queries. Their key tiles would run far longer than the others: what
 // lies past their window is cut into pieces of `chunk` queries, blocks of their own, whose partial sums (fp32) a last kernel
 // adds in order.
+#include <climits>
 #include <type_traits>
 
 #include "tensor_core.h"
@@ -381,10 +382,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 issued = i + 1;
             }
-            if (failed) {  // nothing of this block's memory is given back while a copy is on its way
-                bar_wait(bar_fixed, 0, kDrain);
-                for (int i = max(0, issued - kStages); i < issued; ++i) bar_wait(bar_full + 8 * (i % kStages), (i / kStages) & 1, kDrain);
-            }
+            // nothing of this block's memory is given back while a copy is on its way, whoever gave up
+            bar_wait(bar_fixed, 0, kDrain);
+            for (int i = max(0, issued - kStages); i < issued; ++i) bar_wait(bar_full + 8 * (i % kStages), (i / kStages) & 1, kDrain);
         }
         __syncwarp();
     } else if (warp == kScoreWarp) {
@@ -419,10 +419,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                            kDesc, k > 0);
                 mma_commit(bar_dp + 8 * b);
             }
-            if (failed) {  // the tensor memory is given back only when no product uses it any more
-                mma_commit(bar_end);
-                bar_wait(bar_end, 0, kDrain);
-            }
+            mma_commit(bar_end);  // the tensor memory is given back only when no product uses it any more
+            bar_wait(bar_end, 0, kDrain);
         }
         __syncwarp();
     } else if (warp == kSumWarp) {
@@ -455,10 +453,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 mma_commit(bar_empty + 8 * st);
                 if (i == n - 1) mma_commit(bar_last);
             }
-            if (failed) {
-                mma_commit(bar_end + 8);
-                bar_wait(bar_end + 8, 0, kDrain);
-            }
+            mma_commit(bar_end + 8);
+            bar_wait(bar_end + 8, 0, kDrain);
         }
         __syncwarp();
     } else if (warp == kClearWarp) {
@@ -672,16 +668,23 @@ __global__ void __launch_bounds__(256) window_backward_join_kernel(const Params 
 
 size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
 
-// Queries of one far piece: about what a key tile's own window holds, so that the blocks are alike.
+// Key tiles whose far queries are cut into pieces: those of up to 1024 first tokens. (With more of them there are blocks enough,
+// and the pieces' partial sums would grow with their square.)
+constexpr int kMostFarTiles = 8;
+constexpr int kMostPartials = 2048;  // of 128 rows of dV and dK each, for a whole call
+// Queries of one piece: about what a key tile's own window holds, so that the blocks are alike; at least 1024, and no fewer than
+// keep the partial sums in bounds. INT_MAX: nothing is cut.
 int far_chunk(const AttentionArgs& a) {
-    const int64_t c = (int64_t)a.window + kRows;
-    return (int)(c < 1024 ? 1024 : c);
-}
-int far_tiles(const AttentionArgs& a) {
     const int seen = a.sinks < a.total_k ? a.sinks : a.total_k;
-    // no sequence reaches past its window by a whole piece when all keys together do not
-    return a.total_k < far_chunk(a) ? 0 : (seen + kRows - 1) / kRows;
+    const int64_t tiles = (seen + kRows - 1) / kRows;
+    if (tiles == 0 || tiles > kMostFarTiles) return INT_MAX;
+    int64_t c = (int64_t)a.window + kRows;
+    if (c < 1024) c = 1024;
+    const int64_t bound = (int64_t)a.total_k * tiles * a.kv_heads * 2 / kMostPartials + 1;
+    if (c < bound) c = bound;
+    return c > a.total_k ? INT_MAX : (int)c;  // no sequence reaches past its window by a whole piece when all keys together do not
 }
+int far_tiles(const AttentionArgs& a) { return far_chunk(a) == INT_MAX ? 0 : ((a.sinks < a.total_k ? a.sinks : a.total_k) + kRows - 1) / kRows; }
 int far_slots(const AttentionArgs& a) { return a.total_k / far_chunk(a) + 1; }
 
 template <typename T, int DP>
@@ -704,7 +707,7 @@ cudaError_t launch(cudaStream_t s, const AttentionArgs& a, void* buffer) {
     p.lse = a.lse, p.delta = delta;
     p.chunk = far_chunk(a), p.far_tiles = far_tiles(a), p.far_slots = p.far_tiles > 0 ? far_slots(a) : 0;
     p.partial = reinterpret_cast<float*>(b + align256(size_t(a.q_heads) * a.total_q * 4));
-    p.limit = a.wait.limit_cycles, p.fault = a.wait.fault_word;
+    p.limit = window_wait_limit(a), p.fault = a.wait.fault_word;
     delta_kernel<T><<<(unsigned)(((int64_t)a.total_q * a.q_heads + 15) / 16), 256, 0, s>>>(a, delta);
     cudaError_t e = cudaGetLastError();
     static SharedMemoryOnce once_keys, once_queries;

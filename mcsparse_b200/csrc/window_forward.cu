@@ -252,13 +252,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int c = 0; c < kBlocks; ++c) tma_load_3d(to + S::kTile + c * (kKeys * 128), &map_v, 64 * c, hk * a.v_mul, key, bar_v + 8 * st);
                 issued = i + 1;
             }
-            // nothing of this block's memory is given back while a copy is on its way
-            if (failed) {
-                bar_wait(bar_q, 0, kDrain);
-                for (int i = max(0, issued - S::kStages); i < issued; ++i) {
-                    bar_wait(bar_k + 8 * (i % S::kStages), (i / S::kStages) & 1, kDrain);
-                    bar_wait(bar_v + 8 * (i % S::kStages), (i / S::kStages) & 1, kDrain);
-                }
+            // nothing of this block's memory is given back while a copy is on its way, whoever gave up
+            bar_wait(bar_q, 0, kDrain);
+            for (int i = max(0, issued - S::kStages); i < issued; ++i) {
+                bar_wait(bar_k + 8 * (i % S::kStages), (i / S::kStages) & 1, kDrain);
+                bar_wait(bar_v + 8 * (i % S::kStages), (i / S::kStages) & 1, kDrain);
             }
         }
         __syncwarp();
@@ -296,10 +294,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     ++n_s[t];
                 }
             }
-            if (failed) {  // the tensor memory is given back only when no product uses it any more
-                mma_commit(bar_end);
-                bar_wait(bar_end, 0, kDrain);
-            }
+            mma_commit(bar_end);  // the tensor memory is given back only when no product uses it any more
+            bar_wait(bar_end, 0, kDrain);
         }
         __syncwarp();
     } else if (warp == kValueWarp) {
@@ -331,10 +327,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 if (!failed) mma_commit(bar_done + 8 * st);
             }
-            if (failed) {
-                mma_commit(bar_end + 8);
-                bar_wait(bar_end + 8, 0, kDrain);
-            }
+            mma_commit(bar_end + 8);
+            bar_wait(bar_end + 8, 0, kDrain);
         }
         __syncwarp();
     } else if (warp == kClearWarp) {
@@ -408,7 +402,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         const float inv = row.sum == 0.0f ? 0.0f : 1.0f / row.sum;
         const int64_t token = (int64_t)sq.q0 + row0 + t * kRows + r;
-        if (a.lse != nullptr && r < v.rows)
+        if (a.lse != nullptr && r < v.rows && !failed)
             a.lse[(int64_t)head * a.total_q + token] = row.sum == 0.0f ? -INFINITY : row.ref * a.scale_ln + logf(row.sum);
         T* out = static_cast<T*>(a.o) + token * a.o_token + (int64_t)head * a.o_head;
 #pragma unroll 1
@@ -461,7 +455,7 @@ cudaError_t launch(cudaStream_t s, const AttentionArgs& a) {
     p.negate = a.scale < 0.0f ? kNegateA : 0;
     p.scale_log2 = fabsf(a.scale) * kLog2e, p.scale_ln = 1.0f / kLog2e;
     p.o = a.o.p, p.o_token = a.o.token, p.o_head = a.o.head, p.lse = a.lse;
-    p.limit = a.wait.limit_cycles, p.fault = a.wait.fault_word;
+    p.limit = window_wait_limit(a), p.fault = a.wait.fault_word;
     static SharedMemoryOnce once;
     const cudaError_t e = once.allow(reinterpret_cast<const void*>(window_forward_kernel<T, DP>), S::kTotal);
     if (e != cudaSuccess) return e;

@@ -17,6 +17,10 @@ bool head_map(CUtensorMap* map, const AttentionTensor& t, int64_t tokens, int he
 // [offset[b] / size + b, offset[b + 1] / size + b + 1), which are at least as many as its blocks; the surplus does nothing.
 inline int ragged_slots(int total, int batch, bool offsets, int size) { return offsets ? total / size + batch : (total + size - 1) / size; }
 
+// SM clocks a wait may take: 64 times the handle's limit (20 ms), so that a process that was switched off the GPU for a while
+// does not look like one whose copies never arrive.
+inline long long window_wait_limit(const AttentionArgs& a) { return a.wait.limit_cycles > (1LL << 50) ? (1LL << 56) : a.wait.limit_cycles * 64; }
+
 struct RaggedBlock {
     int b, index;  // sequence (-1: none), block inside it
 };

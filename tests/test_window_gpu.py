@@ -254,6 +254,46 @@ def test_two_calls_at_once(device):
         handle.close()
 
 
+@pytest.mark.parametrize("sinks", [900, 1024, 1025, 5000])
+def test_many_first_tokens_of_a_long_sequence(handle, device, sinks):
+    """First tokens on either side of the number whose far queries are cut into pieces, two sequences of different length."""
+    gen = torch.Generator(device=device).manual_seed(51)
+    lengths = [3300, 1500]
+    q, k, v, g = (normal((sum(lengths), h, 64), torch.bfloat16, device, gen) for h in (2, 1, 1, 2))
+    check(handle, q, k, v, lengths, lengths, 100, sinks, dout=g)
+
+
+def test_waits_that_run_out_are_reported(device):
+    """With a wait limit of one clock every block gives up; the call after the next synchronisation says so, once, and with the
+    limit back the same handle computes what it should."""
+    handle = mc.Handle()
+    gen = torch.Generator(device=device).manual_seed(52)
+    n, w = 900, mc.Window(200, 4, 4, 2, 128, torch.bfloat16)
+    q, k, v, g = (normal((n, h, 128), torch.bfloat16, device, gen) for h in (4, 2, 2, 4))
+    out, lse = torch.empty_like(q), torch.empty(4, n, device=device)
+    grads = [torch.empty_like(x) for x in (q, k, v)]
+    buf = torch.empty(mc.window_attention_backward_buffer_size(handle, w, 1, n, n), dtype=torch.uint8, device=device)
+    for step in ("forward", "backward"):
+        mc.window_attention(handle, w, q, k, v, out, lse)
+        torch.cuda.synchronize()
+        capi.check(lib.mcsparseB200SetDeviceWaitLimit(handle.h, 1, 0))
+        if step == "forward":
+            mc.window_attention(handle, w, q, k, v, out, lse)
+        else:
+            mc.window_attention_backward(handle, w, q, k, v, out, lse, g, *grads, buf)
+        torch.cuda.synchronize()
+        capi.check(lib.mcsparseB200SetDeviceWaitLimit(handle.h, 40_000_000, 0))
+        with pytest.raises(mc.McsparseError) as e:
+            mc.window_attention(handle, w, q, k, v, out, lse)
+        assert e.value.status == capi.MCSPARSE_STATUS_EXECUTION_FAILED
+    mc.window_attention(handle, w, q, k, v, out, lse)
+    mc.window_attention_backward(handle, w, q, k, v, out, lse, g, *grads, buf)
+    want = ref.attention(q, k, v, 200, 4, w.scale, g)
+    for name, x in zip(("out", "lse", "dq", "dk", "dv"), (out, lse, *grads)):
+        ref.close(x, want[name], name)
+    handle.close()
+
+
 def test_offsets_that_lie_stay_inside(handle, device):
     """Offsets that do not ascend or leave the tensors: rows of no meaning, but nothing outside the outputs is written."""
     gen = torch.Generator(device=device).manual_seed(53)
