@@ -201,30 +201,35 @@ __global__ void __launch_bounds__(kThreads, 1)
                    bar_done = bar_clear + 8 * S::kStages, bar_s = bar_done + 8 * S::kStages, bar_p = bar_s + 32, bar_o = bar_p + 32,
                    bar_end = bar_o + 32, slot = bar_end + 16;
 
-    const int head = blockIdx.x % a.q_heads;
-    const int block = a.slots - 1 - (int)(blockIdx.x / a.q_heads);  // the later rows of a sequence have more to do: first
-    const RaggedBlock rb = ragged_block(a.r.q_offsets, a.r.batch, a.r.total_q, block, 2 * kRows, lane);
-    const Sequence sq = rb.b < 0 ? Sequence{0, 0, 0, 0} : sequence_of(a.r, rb.b);
-    if (rb.b < 0 || (int64_t)rb.index * 2 * kRows >= sq.lq) return;  // (the same for the whole block)
-    const int row0 = rb.index * 2 * kRows;
-    const Visit va = visit_of(sq, row0, a.window, a.sinks).same(), vb = visit_of(sq, row0 + kRows, a.window, a.sinks).same();
-    const Order order = order_of(va, vb).same();
-
     if (warp == kValueWarp) {
         tmem_alloc(slot, 512);
     } else if (threadIdx.x == 32 * kLoadWarp) {
+        tma_prefetch(&map_q), tma_prefetch(&map_k), tma_prefetch(&map_v);
         bar_init(bar_q, 1);
         for (int i = 0; i < 4 * S::kStages; ++i) bar_init(bar_k + 8 * i, 1);
         for (int i = 0; i < 4; ++i) bar_init(bar_s + 8 * i, 1), bar_init(bar_p + 8 * i, kRows), bar_init(bar_o + 8 * i, 1);
         for (int i = 0; i < 2; ++i) bar_init(bar_end + 8 * i, 1);
         bar_init_fence();
     }
+    const int head = blockIdx.x % a.q_heads;
+    const int block = a.slots - 1 - (int)(blockIdx.x / a.q_heads);  // the later rows of a sequence have more to do: first
+    const RaggedBlock rb = ragged_block(a.r.q_offsets, a.r.batch, a.r.total_q, block, 2 * kRows, lane);
+    const Sequence sq = rb.b < 0 ? Sequence{0, 0, 0, 0} : sequence_of(a.r, rb.b);
+    const bool none = rb.b < 0 || (int64_t)rb.index * 2 * kRows >= sq.lq;  // a surplus number: nothing to do
+    const int row0 = none ? 0 : rb.index * 2 * kRows;
+    const Visit va = visit_of(sq, row0, a.window, a.sinks).same(), vb = visit_of(sq, row0 + kRows, a.window, a.sinks).same();
+    const Order order = order_of(va, vb).same();
+
     fence_before();
     __syncthreads();
     fence_after();
     uint32_t tmem;
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(slot));
     tmem = uniform(tmem);
+    if (none) {  // (the same for the whole block)
+        if (warp == kValueWarp) tmem_free(tmem, 512);
+        return;
+    }
     // tensor memory: S (and P) of the two row tiles, two buffers each; O of the two row tiles
     const uint32_t t_s = tmem, t_o = tmem + 4 * kKeys;
     bool failed = false;
