@@ -232,6 +232,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem = (smem_u32(smem_raw) + 1023) & ~1023u;
     const int warp = uniform((int)(threadIdx.x >> 5)), lane = threadIdx.x & 31;
+    if (threadIdx.x == 32 * kLoadWarp) tma_prefetch(&map_fixed1), tma_prefetch(&map_fixed2), tma_prefetch(&map_stream1), tma_prefetch(&map_stream2);
     // barriers: stationary operands; of every stage: there, clear, done with; of the buffers: S ready, dP ready, P ready, dS ready,
     // S's columns free, dP's columns free; the last product done; the groups' exchange; the ends of the two issuing warps
     const uint32_t bars = smem + S::kBars;
@@ -348,9 +349,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                     l[x] = -INFINITY, d[x] = 0.0f;
                     if (q < end) {
                         const int64_t at = (int64_t)h * a.r.total_q + sq.q0 + q;
-                        const float v = __ldg(a.lse + at);
+                        const float v = __ldg(a.lse + at), w = __ldg(a.delta + at);  // (both on their way before either is looked at)
                         if (v != -INFINITY) l[x] = kLift - v * kLog2e;
-                        d[x] = -kLower * __ldg(a.delta + at);
+                        d[x] = -kLower * w;
                     }
                 }
             };
