@@ -59,10 +59,17 @@ __device__ __forceinline__ Pack<T, V> load_pack(const T* p) {
     }
     return r;
 }
-template <typename T, int V>
+// STREAM: written once and not looked at before it has left L2 anyway.
+template <typename T, int V, bool STREAM = false>
 __device__ __forceinline__ void store_pack(T* p, const Pack<T, V>& r) {
-    if constexpr (sizeof(r) == 32) {
-        const float* f = reinterpret_cast<const float*>(&r);
+    const float* f = reinterpret_cast<const float*>(&r);
+    if constexpr (sizeof(r) == 32 && STREAM) {
+        asm volatile("st.global.cs.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]),
+                     "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7])
+                     : "memory");
+    } else if constexpr (sizeof(r) == 16 && STREAM) {
+        __stcs(reinterpret_cast<float4*>(p), *reinterpret_cast<const float4*>(f));
+    } else if constexpr (sizeof(r) == 32) {
         asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]),
                      "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7])
                      : "memory");
@@ -99,7 +106,7 @@ __device__ __forceinline__ void load_columns(const T* row, int64_t first, int64_
     }
 }
 
-template <typename T, int V>
+template <typename T, int V, bool STREAM = false>
 __device__ __forceinline__ void store_columns(T* row, int64_t first, int64_t width, int lane, const float* in) {
     if (V > 1) {
         const int64_t c = first + lane * V;
@@ -107,7 +114,7 @@ __device__ __forceinline__ void store_columns(T* row, int64_t first, int64_t wid
             Pack<T, V> p;
 #pragma unroll
             for (int i = 0; i < V; ++i) p.v[i] = from_float<T>(in[i]);
-            store_pack<T, V>(row + c, p);
+            store_pack<T, V, STREAM>(row + c, p);
         }
     } else {
 #pragma unroll
@@ -122,7 +129,7 @@ __device__ __forceinline__ void store_columns(T* row, int64_t first, int64_t wid
 
 constexpr int kLookupPieces = 4;  // slabs per warp, all loads in flight together
 
-template <typename E, typename Y, typename I, int V>
+template <typename E, typename Y, typename I, int V, bool STREAM>
 __global__ void __launch_bounds__(256)
     embedding_lookup_kernel(int64_t count, int64_t rows, int64_t width, const I* __restrict__ ids, int base,
                             const E* __restrict__ table, int64_t ld_e, Y* __restrict__ out, int64_t ld_y,
@@ -154,7 +161,7 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
             for (int i = 0; i < kPer; ++i) v[p][i] *= alpha;
         }
-        store_columns<Y, V>(dst, first + p * kSlab, width, lane, v[p]);
+        store_columns<Y, V, STREAM>(dst, first + p * kSlab, width, lane, v[p]);
     }
 }
 
@@ -634,8 +641,11 @@ cudaError_t launch_lookup(cudaStream_t s, const EmbeddingArgs& a, const I* ids) 
     const int64_t pieces = (a.width + span - 1) / span;
     const unsigned blocks = warp_blocks(a.count * pieces);
     if (blocks == 0) return cudaErrorInvalidValue;
-    embedding_lookup_kernel<E, Y, I, V><<<blocks, 256, 0, s>>>(a.count, a.rows, a.width, ids, a.base, static_cast<const E*>(a.table),
-                                                               a.ld_table, static_cast<Y*>(a.tokens), a.ld_tokens, a.alpha, pieces);
+    // Rows of the result that cannot stay in L2 (126 MB) leave it first, so that rows of the table which come again are still there.
+    const bool stream = V > 1 && a.count * a.width * (int64_t)sizeof(Y) > (int64_t(64) << 20);
+    const auto kernel = stream ? embedding_lookup_kernel<E, Y, I, V, (V > 1)> : embedding_lookup_kernel<E, Y, I, V, false>;
+    kernel<<<blocks, 256, 0, s>>>(a.count, a.rows, a.width, ids, a.base, static_cast<const E*>(a.table), a.ld_table, static_cast<Y*>(a.tokens),
+                                  a.ld_tokens, a.alpha, pieces);
     return cudaGetLastError();
 }
 

@@ -82,6 +82,21 @@ def test_lookup_keeps_bits_and_device_alpha(handle, device):
     assert bool((out[::3] == 0).all()), "padding is zero whatever alpha is"
 
 
+@pytest.mark.parametrize("types", TYPES, ids=lambda t: f"{str(t[0])[6:]}-{str(t[1])[6:]}")
+def test_lookup_of_more_rows_than_l2_holds(handle, device, types):
+    """A result of more than 64 MB is written past L2."""
+    te, ty = types
+    gen = torch.Generator(device=device).manual_seed(9)
+    count = (80 << 20) // (2048 * torch.finfo(ty).bits // 8)
+    table = torch.empty(3000, 2048, dtype=te, device=device).normal_(generator=gen)
+    ids = ids_for(count, 3000, "outside", device)
+    out = torch.empty(count, 2048, dtype=ty, device=device)
+    mc.embedding_lookup(handle, ids, mat(table), mat(out), alpha=0.5)
+    ok = (ids >= 0) & (ids < 3000)
+    want = torch.where(ok[:, None], table[ids.clamp(0, 2999)].float() * 0.5, 0.0)  # exact: a power of two
+    assert torch.equal(out, want.to(ty))
+
+
 def run_gradient(handle, ids, dy, table, alpha=1.0, beta=0.0, base=0):
     m_y, m_e = mc.DnMat(dy, dy.shape[0], dy.shape[1], dy.stride(0)), mc.DnMat(table, *table.shape, table.stride(0))
     buf = torch.empty(mc.embedding_gradient_buffer_size(handle, ids, m_y, m_e), dtype=torch.uint8, device=dy.device)
