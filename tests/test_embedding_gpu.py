@@ -156,6 +156,50 @@ def test_gradient_strides_and_untouched_rows(handle, device):
         assert bool(same[~inside].all()), "beta = 1 leaves rows without tokens as they were"
 
 
+@pytest.mark.parametrize("rows", [300_000, 1 << 28])
+@pytest.mark.parametrize("count", [500, 5000])
+def test_gradient_of_a_tall_table(handle, device, rows, count):
+    """Ids of 19 and 29 bits: three and four passes of the sort, an odd and an even number."""
+    gen = torch.Generator(device=device).manual_seed(13)
+    ids = torch.randint(0, rows, (count,), device=device, generator=gen)
+    ids[::3] = ids[0]
+    ids[1::7] = rows - 1
+    dy = torch.empty(count, 2, dtype=torch.float32, device=device).normal_(generator=gen)
+    table = torch.zeros(rows, 2, device=device)
+    run_gradient(handle, ids, dy, table, beta=1.0)
+    touched, inverse = torch.unique(ids, return_inverse=True)
+    value, allowed = ref.gradient(inverse, dy, len(touched), 1.0, 0.0, torch.zeros(len(touched), 2, device=device))
+    ref.close(table[touched], (value, allowed), "gradient")
+    table[touched] = 0
+    assert not bool(table.any()), "wrote a row nobody named"
+
+
+def test_gradient_with_scalars_on_the_device(handle, device):
+    gen = torch.Generator(device=device).manual_seed(14)
+    ids = ids_for(700, 200, "outside", device)
+    dy = torch.empty(700, 64, dtype=torch.bfloat16, device=device).normal_(generator=gen)
+    handle.set_pointer_mode(capi.MCSPARSE_POINTER_MODE_DEVICE)
+    try:
+        for a, b in ((0.75, 0.0), (2.0, 1.0), (-1.0, 0.5)):
+            table = torch.empty(200, 64, device=device).normal_(generator=gen)
+            want = ref.gradient(ids, dy, 200, a, b, table)
+            run_gradient(handle, ids, dy, table, torch.full((1,), a, device=device), torch.full((1,), b, device=device))
+            ref.close(table, want, f"{a} {b}")
+    finally:
+        handle.set_pointer_mode(capi.MCSPARSE_POINTER_MODE_HOST)
+
+
+def test_no_rows(handle, device):
+    """A table without rows: every index lies outside it."""
+    ids = torch.zeros(5, dtype=torch.int32, device=device)
+    table = mc.DnMat(torch.zeros(1, 16, device=device), 0, 16, 16)
+    out = torch.full((5, 16), 7.0, device=device)
+    mc.embedding_lookup(handle, ids, table, mat(out))
+    assert bool((out == 0).all())
+    buf = torch.empty(mc.embedding_gradient_buffer_size(handle, ids, mat(out), table), dtype=torch.uint8, device=device)
+    mc.embedding_gradient(handle, ids, mat(out), table, buf)
+
+
 def test_gradient_empty(handle, device):
     table = torch.randn(5, 8, device=device)
     ids = torch.empty(1, dtype=torch.int64, device=device)[:0]

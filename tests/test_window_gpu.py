@@ -263,6 +263,41 @@ def test_many_first_tokens_of_a_long_sequence(handle, device, sinks):
     check(handle, q, k, v, lengths, lengths, 100, sinks, dout=g)
 
 
+def test_offsets_past_32_bits(handle, device):
+    """2.4e9 values per tensor of queries: the last sequence lies behind 2^31 of them."""
+    gen = torch.Generator(device=device).manual_seed(54)
+    lengths, hq, d, window = [139_800, 300], 136, 128, 40
+    total = sum(lengths)
+    assert lengths[0] * hq * d > 1 << 31
+    q, g = (normal((total, hq, d), torch.bfloat16, device, gen) for _ in range(2))
+    k, v = (normal((total, 1, d), torch.bfloat16, device, gen) for _ in range(2))
+    w, off = mc.Window(window, 2, hq, 1, d, torch.bfloat16), offsets(lengths, device)
+    out, dq, dk, dv = torch.empty_like(q), torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+    lse = torch.empty(hq, total, device=device)
+    mc.window_attention(handle, w, q, k, v, out, lse, q_offsets=off)
+    buf = torch.empty(mc.window_attention_backward_buffer_size(handle, w, 2, total, total), dtype=torch.uint8, device=device)
+    mc.window_attention_backward(handle, w, q, k, v, out, lse, g, dq, dk, dv, buf, q_offsets=off)
+    last = slice(lengths[0], total)
+    want = ref.attention(q[last], k[last], v[last], window, 2, w.scale, g[last])
+    for name, x in (("out", out[last]), ("lse", lse[:, last]), ("dq", dq[last]), ("dk", dk[last]), ("dv", dv[last])):
+        ref.close(x, want[name], name)
+
+
+def test_infinite_and_nan_scores_stay_in_their_row(handle, device):
+    """A query with an infinite or a NaN value gives a row of NaN, as a softmax does, and no other row notices."""
+    gen = torch.Generator(device=device).manual_seed(55)
+    for dtype in (torch.bfloat16, torch.float16, torch.float32):
+        q, k, v = (normal((400, 2, 64), dtype, device, gen) for _ in range(3))
+        w = mc.Window(90, 2, 2, 2, 64, dtype)
+        plain, bad = torch.empty_like(q), torch.empty_like(q)
+        mc.window_attention(handle, w, q, k, v, plain)
+        q[37, 0, 5], q[200, 1, 9] = float("nan"), float("inf")
+        mc.window_attention(handle, w, q, k, v, bad)
+        assert bool(bad[37, 0].isnan().all()) and bool(bad[200, 1].isnan().all())
+        bad[37, 0], bad[200, 1] = plain[37, 0], plain[200, 1]
+        assert torch.equal(bad, plain)
+
+
 def test_waits_that_run_out_are_reported(device):
     """With a wait limit of one clock every block gives up; the call after the next synchronisation says so, once, and with the
     limit back the same handle computes what it should."""
