@@ -7,6 +7,8 @@ handle's, or that have another type or shape than the call needs, are refused wi
 
 import ctypes as C
 import math
+import struct
+import threading
 
 import torch
 
@@ -15,13 +17,20 @@ from .capi import check, lib
 from .host import _DTYPE
 
 _INDEX = {torch.int32: capi.MCSPARSE_INDEX_32I, torch.int64: capi.MCSPARSE_INDEX_64I}
-# Several mcsparseB200Heads_t / mcsparseB200Cache_t side by side: one allocation per call, addressed by its parts.
-_Tensors4, _Tensors8 = C.c_int64 * 12, C.c_int64 * 24
-_Decode = C.c_int64 * 14
-_HEADS = C.sizeof(capi.Heads)
-_CACHE = C.sizeof(capi.Cache)
+_HEADS, _CACHE = C.sizeof(capi.Heads), C.sizeof(capi.Cache)
+_pack4, _pack8, _pack_decode = (struct.Struct(f"{n}q").pack_into for n in (12, 24, 14))
 
 
+class _Block(threading.local):
+    """Room for the mcsparseB200Heads_t / mcsparseB200Cache_t of one call, side by side and addressed by their parts: the library
+    copies them before the call returns."""
+
+    def __init__(self):
+        self.memory = (C.c_int64 * 24)()
+        self.at = C.addressof(self.memory)
+
+
+_block = _Block()
 _GRADIENT_SIZES = {}  # buffer sizes asked for so far, by device, tokens and table
 
 
@@ -142,12 +151,13 @@ def _offsets(device, q_offsets, k_offsets):
         return 1, None, None
     if k_offsets is None:
         k_offsets = q_offsets
-    for t in (q_offsets, k_offsets):
+    for t in (q_offsets, k_offsets) if k_offsets is not q_offsets else (q_offsets,):
         if t.dtype is not torch.int32 or t.dim() != 1 or t.shape[0] < 1 or not t.is_contiguous() or t.get_device() != device:
             raise ValueError("offsets must be a contiguous int32 row of sequences + 1 entries on the handle's device")
-    if q_offsets.shape != k_offsets.shape:
+    n = q_offsets.shape[0]
+    if k_offsets.shape[0] != n:
         raise ValueError("q_offsets and k_offsets must describe the same number of sequences")
-    return q_offsets.shape[0] - 1, q_offsets.data_ptr(), k_offsets.data_ptr()
+    return n - 1, q_offsets.data_ptr(), k_offsets.data_ptr()
 
 
 def _lse(device, lse, shape):
@@ -165,10 +175,10 @@ def window_attention(handle, window, q, k, v, out, lse=None, q_offsets=None, k_o
     k_offsets: int32 offsets of the sequences (k_offsets defaults to q_offsets; neither: one sequence). lse: q_heads x queries."""
     device = handle.stream.device_index
     tq, tk, hq, hk = q.shape[0], k.shape[0], window.q_heads, window.kv_heads
-    t = _Tensors4(*_heads(device, q, tq, hq, window, "q"), *_heads(device, k, tk, hk, window, "k"),
-                  *_heads(device, v, tk, hk, window, "v"), *_heads(device, out, tq, hq, window, "out"))
+    _pack4(_block.memory, 0, *_heads(device, q, tq, hq, window, "q"), *_heads(device, k, tk, hk, window, "k"),
+           *_heads(device, v, tk, hk, window, "v"), *_heads(device, out, tq, hq, window, "out"))
     batch, qo, ko = _offsets(device, q_offsets, k_offsets)
-    p = C.addressof(t)
+    p = _block.at
     check(lib.mcsparseB200WindowAttention(handle.h, window.d, batch, qo, ko, tq, tk, p, p + _HEADS, p + 2 * _HEADS, p + 3 * _HEADS,
                                           _lse(device, lse, (hq, tq))), "mcsparseB200WindowAttention")
 
@@ -181,16 +191,16 @@ def window_attention_backward(handle, window, q, k, v, out, lse, dout, dq, dk, d
     """Gradients dq, dk, dv of :func:`window_attention`; ``out`` and ``lse`` are what it wrote."""
     device = handle.stream.device_index
     tq, tk, hq, hk = q.shape[0], k.shape[0], window.q_heads, window.kv_heads
-    t = _Tensors8(*_heads(device, q, tq, hq, window, "q"), *_heads(device, k, tk, hk, window, "k"),
-                  *_heads(device, v, tk, hk, window, "v"), *_heads(device, out, tq, hq, window, "out"),
-                  *_heads(device, dout, tq, hq, window, "dout"), *_heads(device, dq, tq, hq, window, "dq"),
-                  *_heads(device, dk, tk, hk, window, "dk"), *_heads(device, dv, tk, hk, window, "dv"))
+    _pack8(_block.memory, 0, *_heads(device, q, tq, hq, window, "q"), *_heads(device, k, tk, hk, window, "k"),
+           *_heads(device, v, tk, hk, window, "v"), *_heads(device, out, tq, hq, window, "out"),
+           *_heads(device, dout, tq, hq, window, "dout"), *_heads(device, dq, tq, hq, window, "dq"),
+           *_heads(device, dk, tk, hk, window, "dk"), *_heads(device, dv, tk, hk, window, "dv"))
     batch, qo, ko = _offsets(device, q_offsets, k_offsets)
     if lse is None:
         raise ValueError("the backward pass needs lse")
     work = _buffer(buffer, window_attention_backward_buffer_size(handle, window, batch, tq, tk))
     _on_device(handle, buffer)
-    p = C.addressof(t)
+    p = _block.at
     check(lib.mcsparseB200WindowAttentionBackward(
         handle.h, window.d, batch, qo, ko, tq, tk, p, p + _HEADS, p + 2 * _HEADS, p + 3 * _HEADS, _lse(device, lse, (hq, tq)),
         p + 4 * _HEADS, p + 5 * _HEADS, p + 6 * _HEADS, p + 7 * _HEADS, work), "mcsparseB200WindowAttentionBackward")
@@ -220,8 +230,8 @@ def window_attention_decode(handle, window, q, k_cache, v_cache, lengths, out, l
     batch x pages of a sequence (None: page b is all of sequence b); lse: batch x q_heads."""
     device = handle.stream.device_index
     batch, hq = q.shape[0], window.q_heads
-    t = _Decode(*_heads(device, q, batch, hq, window, "q"), *_heads(device, out, batch, hq, window, "out"),
-                *_cache(device, k_cache, window, "k_cache"), *_cache(device, v_cache, window, "v_cache"))
+    _pack_decode(_block.memory, 0, *_heads(device, q, batch, hq, window, "q"), *_heads(device, out, batch, hq, window, "out"),
+                 *_cache(device, k_cache, window, "k_cache"), *_cache(device, v_cache, window, "v_cache"))
     pages, page_size = k_cache.shape[:2]
     if v_cache.shape != k_cache.shape:
         raise ValueError("k_cache and v_cache must hold the same pages")
@@ -238,7 +248,7 @@ def window_attention_decode(handle, window, q, k_cache, v_cache, lengths, out, l
         table, max_pages = page_table.data_ptr(), page_table.shape[1]
     work = _buffer(buffer, window_attention_decode_buffer_size(handle, window, batch, max_pages, page_size))
     _on_device(handle, buffer)
-    p = C.addressof(t)
+    p = _block.at
     check(lib.mcsparseB200WindowAttentionDecode(handle.h, window.d, batch, lengths.data_ptr(), p, p + 2 * _HEADS, p + 2 * _HEADS + _CACHE,
                                                 pages, page_size, table, max_pages, p + _HEADS, _lse(device, lse, (batch, hq)), work),
           "mcsparseB200WindowAttentionDecode")
