@@ -20,6 +20,7 @@
 #include <cuda_fp16.h>
 
 #include "internal.h"
+#include "launch.h"
 
 namespace mcsp_b200 {
 namespace {
@@ -167,11 +168,6 @@ __global__ void __launch_bounds__(256)
 
 // ----------------------------------------------------------------------------- gradient
 
-// Waits until the launch before this one in the stream is done and its writes are seen (programmatic dependent launch).
-__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-// Lets the next launch's blocks come up early; they wait in grid_wait().
-__device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-
 // The rows of a warp's chunk on their way. Vectors: a ring of asynchronous copies in shared memory, a thread reads back what it
 // copied itself; the copies of 16 (8) rows are in flight whatever the warp is doing. (Loads into registers, as many ahead,
 // waited for the newest of them at every row: 52 us against 25 for 16384 rows of 2048 bf16 values.)
@@ -271,7 +267,10 @@ __global__ void __launch_bounds__(256)
     const int lane = threadIdx.x & 31;
     const float alpha = alpha_arg.get(), beta = beta_arg.get();
     grid_release();
-    if (warp >= a.chunks * a.slabs) return;
+    if (warp >= a.chunks * a.slabs) {
+        grid_wait();
+        return;
+    }
     const int64_t c = warp / a.slabs;
     const int64_t first = (warp - c * a.slabs) * kSlab;
     const int64_t k0 = c * a.chunk, k1 = min(k0 + a.chunk, a.count);
@@ -712,23 +711,6 @@ __global__ void __launch_bounds__(256)
     embedding_pairs_kernel(int64_t count, const int* __restrict__ keys, const unsigned* __restrict__ perm, uint2* __restrict__ sorted) {
     const int64_t t = blockIdx.x * (int64_t)blockDim.x + threadIdx.x;
     if (t < count) sorted[t] = make_uint2((unsigned)keys[t], perm[t]);
-}
-
-// A launch whose blocks may come up before the launch ahead of it is done (they wait in grid_wait()); early = false: an
-// ordinary one.
-template <typename... P, typename... A>
-cudaError_t launch_behind(cudaStream_t s, bool early, void (*kernel)(P...), unsigned blocks, int threads, int shared, A... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(blocks);
-    cfg.blockDim = dim3((unsigned)threads);
-    cfg.dynamicSmemBytes = (size_t)shared;
-    cfg.stream = s;
-    cudaLaunchAttribute attr = {};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = early ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
 }
 
 template <typename Y, typename E, int V>

@@ -19,6 +19,7 @@
 #include <climits>
 #include <type_traits>
 
+#include "launch.h"
 #include "tensor_core.h"
 #include "window_common.h"
 #include "window_maps.h"
@@ -122,6 +123,7 @@ __device__ __forceinline__ RaggedBlock far_block(const Ragged& r, int number, in
 // delta = rowsum(dO * O): 16 lanes per row, 8 values each.
 template <typename T>
 __global__ void __launch_bounds__(256) delta_kernel(AttentionArgs a, float* __restrict__ delta) {
+    grid_release();
     const int64_t g = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> 4;
     const int part = threadIdx.x & 15;
     float sum = 0.0f;
@@ -241,7 +243,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                    bar_free_s = bar_ds + 8 * kBuffers, bar_free_dp = bar_free_s + 8 * kBuffers, bar_last = bar_free_dp + 8 * kBuffers,
                    bar_x = bar_last + 8, bar_end = bar_x + 8, slot = bar_end + 16;
 
-    // ---- the block's rows and its stream
+    grid_release();
+    // ---- the block's rows and its stream. (All launches but delta's may come up early: what they read that an earlier one of
+    // them wrote is delta, and the partial sums; every block waits for the launch ahead before it ends.)
     const int heads = KEYS ? a.kv_heads : a.q_heads;
     const int head = blockIdx.x % heads;
     const int number = (int)(blockIdx.x / heads);
@@ -255,20 +259,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (number < far_blocks) {
             const int far = number / a.far_tiles, tile = number % a.far_tiles;
             const RaggedBlock fb = far_block(a.r, far, a.chunk, lane);
-            if (fb.b < 0) return;
+            if (fb.b < 0) return grid_wait();
             sq = sequence_of(a.r, fb.b);
             row0 = tile * kRows;
-            if (row0 >= sq.lk) return;
+            if (row0 >= sq.lk) return grid_wait();
             const Split v = split_of(sq, row0, a.window, a.sinks, a.chunk);
-            if (fb.index >= v.pieces) return;
+            if (fb.index >= v.pieces) return grid_wait();
             begin = v.mid + fb.index * a.chunk;
             end = fb.index + 1 < v.pieces ? begin + a.chunk : sq.lq;
             partial = ((int64_t)far * a.far_tiles + tile) * a.kv_heads + head;
         } else {
             const RaggedBlock rb = ragged_block(a.r.k_offsets, a.r.batch, a.r.total_k, number - far_blocks, kRows, lane);
-            if (rb.b < 0) return;
+            if (rb.b < 0) return grid_wait();
             sq = sequence_of(a.r, rb.b);
-            if ((int64_t)rb.index * kRows >= sq.lk) return;
+            if ((int64_t)rb.index * kRows >= sq.lk) return grid_wait();
             row0 = rb.index * kRows;
             const Split v = split_of(sq, row0, a.window, a.sinks, a.chunk);
             begin = v.begin, end = v.mid;
@@ -279,9 +283,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else {
         const RaggedBlock rb = ragged_block(a.r.q_offsets, a.r.batch, a.r.total_q, a.slots - 1 - number, kRows, lane);
-        if (rb.b < 0) return;
+        if (rb.b < 0) return grid_wait();
         sq = sequence_of(a.r, rb.b);
-        if ((int64_t)rb.index * kRows >= sq.lq) return;
+        if ((int64_t)rb.index * kRows >= sq.lq) return grid_wait();
         row0 = rb.index * kRows;
     }
     const int shift = sq.lk - sq.lq;
@@ -324,6 +328,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // tensor memory: the buffers of S and dP, 64 columns each, then the sums (dV and dK, or M and dQ)
     const uint32_t t_s = tmem, t_dp = tmem + kBuffers * kTile, t_out1 = tmem + 2 * kBuffers * kTile, t_out2 = t_out1 + DP;
     bool failed = false;
+    if (warp != kLoadWarp) grid_wait();  // (before any wait that is timed)
 
     if (warp == kLoadWarp) {
         // ---- loads
@@ -355,6 +360,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
             };
+            grid_wait();  // (the stationary operands are on their way)
             fetch(0);
             int issued = 0;
             for (int i = 0; i < n; ++i) {
@@ -622,6 +628,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         fence_before();
     }
     if (failed && a.fault != nullptr) *reinterpret_cast<volatile int*>(a.fault) = 1;
+    grid_wait();
     __syncthreads();
     if (warp == kSumWarp) {
         fence_after();
@@ -634,6 +641,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 constexpr int kJoinSlices = 8;
 template <typename T, int DP>
 __global__ void __launch_bounds__(256) window_backward_join_kernel(const Params a) {
+    grid_wait();
     const int lane = threadIdx.x & 31;
     int64_t x = blockIdx.x;
     const int slice = (int)(x % kJoinSlices), which = (int)(x / kJoinSlices & 1), head = (int)((x / kJoinSlices >> 1) % a.kv_heads);
@@ -721,12 +729,15 @@ cudaError_t launch(cudaStream_t s, const AttentionArgs& a, void* buffer) {
     p.out1 = a.dq.p, p.out1_token = a.dq.token, p.out1_head = a.dq.head;
     p.slots = ragged_slots(a.total_q, a.batch, a.q_offsets != nullptr, kRows);
     p.delta_out = delta;
-    window_backward_kernel<T, DP, false><<<(unsigned)((int64_t)p.slots * a.q_heads), kThreads, S::kTotal, s>>>(q_rows, go_rows, k_tile, v_tile, p);
+    e = launch_behind(s, true, window_backward_kernel<T, DP, false>, (unsigned)((int64_t)p.slots * a.q_heads), kThreads, S::kTotal, q_rows, go_rows, k_tile,
+                      v_tile, p);
     const int64_t key_blocks = ragged_slots(a.total_k, a.batch, a.k_offsets != nullptr, kRows) + (int64_t)p.far_slots * p.far_tiles;
-    window_backward_kernel<T, DP, true><<<(unsigned)(key_blocks * a.kv_heads), kThreads, S::kTotal, s>>>(k_rows, v_rows, q_tile, go_tile, pk);
-    if (p.far_tiles > 0)
-        window_backward_join_kernel<T, DP><<<(unsigned)((int64_t)p.far_slots * p.far_tiles * a.kv_heads * 2 * kJoinSlices), 256, 0, s>>>(pk);
-    return cudaGetLastError();
+    if (e == cudaSuccess)
+        e = launch_behind(s, true, window_backward_kernel<T, DP, true>, (unsigned)(key_blocks * a.kv_heads), kThreads, S::kTotal, k_rows, v_rows, q_tile,
+                          go_tile, pk);
+    if (e == cudaSuccess && p.far_tiles > 0)
+        e = launch_behind(s, true, window_backward_join_kernel<T, DP>, (unsigned)((int64_t)p.far_slots * p.far_tiles * a.kv_heads * 2 * kJoinSlices), 256, 0, pk);
+    return e;
 }
 
 }  // namespace
