@@ -263,8 +263,8 @@ mcsparseStatus_t mcsparseB200EmbeddingLookup(mcsparseHandle_t handle, const void
  * the rows of dY with one index are summed in fp32 in an order that depends on the indices and sizes alone, so equal
  * inputs give equal bits. Types as in the lookup (matDY in the place of matY). beta == 0: dE is not read, rows without a
  * token become zero. beta == 1: rows without a token are neither read nor written. Indices outside the table contribute
- * nothing. externalBuffer: mcsparseB200EmbeddingGradient_bufferSize bytes, free again when the call's work is done;
- * nothing in it outlives the call.
+ * nothing. dY and dE must not overlap. externalBuffer: mcsparseB200EmbeddingGradient_bufferSize bytes, free again when the
+ * call's work is done; nothing in it outlives the call.
  */
 mcsparseStatus_t mcsparseB200EmbeddingGradient_bufferSize(mcsparseHandle_t handle, int64_t count,
                                                           mcsparseIndexType_t indexType, mcsparseDnMatDescr_t matDY,
@@ -289,7 +289,11 @@ mcsparseStatus_t mcsparseB200CreateWindow(mcsparseB200WindowDescr_t* descr, int6
 mcsparseStatus_t mcsparseB200DestroyWindow(mcsparseB200WindowDescr_t descr);
 
 /* One tensor of tokens x heads x headDim in device memory: element (t, h, d) = values[t * tokenStride + h * headStride + d].
- * Strides in elements. Inputs may overlap themselves (a stride of 0 broadcasts); outputs may not. */
+ * Strides in elements. Inputs may overlap themselves (a stride of 0 broadcasts); outputs may not, and overlap no input.
+ *
+ * Every type, headDim and stride is computed. The fast kernels take 16-bit types whose values are 16-byte aligned, with
+ * headDim and all strides multiples of 8 (forward and backward: token strides above 0, scale other than 0); one call with any
+ * tensor that is not like that runs a row at a time, tens of times slower. */
 typedef struct mcsparseB200Heads {
     void* values;
     int64_t tokenStride;
@@ -300,12 +304,13 @@ typedef struct mcsparseB200Heads {
  * mcsparseB200WindowAttention: forward over a ragged batch. Sequence b holds queries [qOffsets[b], qOffsets[b + 1]) and keys
  * [kOffsets[b], kOffsets[b + 1]) (device arrays of batch + 1 ascending int32; both NULL with batch == 1: one sequence of all
  * tokens). totalQ / totalK: rows of the tensors; rows in no sequence are left as they were. lse: qHeads x totalQ floats
- * (natural logarithm of the softmax sums), may be NULL. totalQ, totalK and a sequence's cache are below 2^30 tokens. A result does not depend on keys and values that no query of its
- * sequence sees; a value that is not finite in a key that some query sees may reach the sequence's other queries.
- * fp32 scores, softmax statistics and sums; 16-bit inputs: the softmax weights are rounded to the inputs' type for the
- * product with V, and O is rounded once. Asynchronous, no buffer, no allocation. The tensor-core kernels' waits are bounded by
- * 64 times the handle's device wait limit (mcsparseB200SetDeviceWaitLimit): a block that gives up leaves its rows unwritten, and the
- * next forward or backward call on the handle returns MCSPARSE_STATUS_EXECUTION_FAILED once.
+ * (natural logarithm of the softmax sums), may be NULL. totalQ, totalK and a sequence's cache are below 2^30 tokens. A result
+ * does not depend on keys and values that no query of its sequence sees; a value that is not finite in a key that some query
+ * sees may reach the sequence's other queries. fp32 scores, softmax statistics and sums; 16-bit inputs: the softmax weights
+ * are rounded to the inputs' type for the product with V, and O is rounded once. Asynchronous, no buffer, no allocation. The
+ * tensor-core kernels' waits are bounded by 64 times the handle's device wait limit (mcsparseB200SetDeviceWaitLimit): a block
+ * that gives up leaves its rows unwritten, and the next forward or backward call on the handle returns
+ * MCSPARSE_STATUS_EXECUTION_FAILED once.
  */
 mcsparseStatus_t mcsparseB200WindowAttention(mcsparseHandle_t handle, mcsparseB200WindowDescr_t descr, int64_t batch,
                                              const int32_t* qOffsets, const int32_t* kOffsets, int64_t totalQ,

@@ -65,7 +65,7 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, long lon
 
 // Limit (SM clocks, about a second) of the waits with which a block that gave up lets its copies and products end.
 constexpr long long kDrain = 2000000000;
-// The same for a whole warp: one answer for all lanes.
+// bar_wait for a whole warp: one answer for all lanes.
 __device__ __forceinline__ bool bar_wait_warp(uint32_t bar, uint32_t parity, long long limit) {
     return __all_sync(0xffffffffu, bar_wait(bar, parity, limit));
 }
@@ -115,15 +115,6 @@ __device__ __forceinline__ void after_loads32(uint32_t* r) {
                  "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]),
                  "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]));
 }
-__device__ __forceinline__ void tmem_load16(uint32_t addr, uint32_t* r) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(addr));
-}
-__device__ __forceinline__ void after_loads16(uint32_t* r) {
-    asm volatile("" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]));
-}
 __device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t* r) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, "
@@ -158,7 +149,7 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t column_blo
 }
 // The descriptor of the operand `bytes` (a multiple of 16) further on.
 __device__ __forceinline__ uint64_t desc_at(uint64_t desc, uint32_t bytes) { return desc + (bytes >> 4); }
-// Instruction descriptor: D (128 x n, fp32) = A * B, bf16 or fp16; b_mn: B is MN-major; negate: A enters with its sign turned.
+// Instruction descriptor: D (128 x n, fp32) = A * B, bf16 or fp16; b_mn: B is MN-major; with kNegateA, A enters with its sign turned.
 __host__ __device__ constexpr uint32_t mma_desc(bool bf16, int n, bool b_mn) {
     return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
 }

@@ -57,12 +57,12 @@ struct Params {
     uint32_t negate;
     float scale, scale_log2;
     const float* lse;
-    const float* delta;  // q_heads x total_q
+    const float* delta;  // q_heads x total_q; read past L1, which may hold what was there before the launch ahead wrote it
     void *out1, *out2;   // dQ, or dV and dK
     int64_t out1_token, out1_head, out2_token, out2_head;
     // the first tokens' far queries
     int chunk, far_slots, far_tiles;
-    float* delta_out;  // queries kernel: the exact delta, may be the same array
+    float* delta_out;  // queries kernel: the exact delta, the same array
     float* partial;  // [2 * far_slots][far_tiles][kv_heads][2][kRows][DP]: far pieces, then what their own windows hold
     long long limit;
     int* fault;
@@ -354,7 +354,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     l[x] = -INFINITY, d[x] = 0.0f;
                     if (q < end) {
                         const int64_t at = (int64_t)h * a.r.total_q + sq.q0 + q;
-                        const float v = __ldg(a.lse + at), w = __ldg(a.delta + at);  // (both on their way before either is looked at)
+                        const float v = __ldg(a.lse + at), w = __ldcg(a.delta + at);  // (both on their way before either is looked at)
                         if (v != -INFINITY) l[x] = kLift - v * kLog2e;
                         d[x] = -kLower * w;
                     }
@@ -500,7 +500,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int64_t at = (int64_t)head * a.r.total_q + token;
             const float v = __ldg(a.lse + at);
             if (v != -INFINITY) own_l = kLift - v * kLog2e;
-            own_d = -kLower * __ldg(a.delta + at);
+            own_d = -kLower * __ldcg(a.delta + at);
         }
         float e = 0.0f;  // queries kernel: the sum of the row's dS
         for (int i = group; i < n; i += 2) {

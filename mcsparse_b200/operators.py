@@ -37,8 +37,9 @@ _GRADIENT_SIZES = {}  # buffer sizes asked for so far, by device, tokens and tab
 def _scalar(handle, value):
     """A float as a C argument: a host scalar, or a one-element fp32 device tensor in device pointer mode."""
     if handle.pointer_mode == capi.MCSPARSE_POINTER_MODE_DEVICE:
-        if not (isinstance(value, torch.Tensor) and value.dtype == torch.float32 and value.numel() == 1 and value.is_cuda):
-            raise ValueError("device pointer mode: alpha and beta are one-element float32 device tensors")
+        if not (isinstance(value, torch.Tensor) and value.dtype == torch.float32 and value.numel() == 1
+                and value.get_device() == handle.stream.device_index):
+            raise ValueError("device pointer mode: alpha and beta are one-element float32 tensors on the handle's device")
         return value.data_ptr()
     return C.byref(C.c_float(value))
 
@@ -89,10 +90,10 @@ def embedding_gradient(handle, indices, dY, dE, buffer, alpha=1.0, beta=0.0, bas
         if len(_GRADIENT_SIZES) >= 1024:
             _GRADIENT_SIZES.clear()
         need = _GRADIENT_SIZES[key] = embedding_gradient_buffer_size(handle, indices, dY, dE)
-    kind = _indices(handle, indices)
+    kind, work = _indices(handle, indices), _buffer(buffer, need)
     _on_device(handle, indices, dY.values, dE.values, buffer)
-    check(lib.mcsparseB200EmbeddingGradient(handle.h, _scalar(handle, alpha), indices.numel(), indices.data_ptr(), kind, base, dY.d, _scalar(handle, beta), dE.d, _buffer(buffer, need)),
-          "mcsparseB200EmbeddingGradient")
+    check(lib.mcsparseB200EmbeddingGradient(handle.h, _scalar(handle, alpha), indices.numel(), indices.data_ptr(), kind, base, dY.d,
+                                            _scalar(handle, beta), dE.d, work), "mcsparseB200EmbeddingGradient")
 
 
 class Window:

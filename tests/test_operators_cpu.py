@@ -81,3 +81,35 @@ def test_tensors_are_checked_before_the_call():
                 lambda: mc.embedding_lookup(Stub, torch.zeros(6, dtype=torch.int64)[::2], table, y)):
         with pytest.raises(ValueError):
             bad()
+    grad = lambda buffer, **kw: mc.embedding_gradient(Stub, ids, y, table, buffer, **kw)
+    with pytest.raises(mc.McsparseError):  # the buffer's size is asked first
+        grad(torch.zeros(64, dtype=torch.uint8))
+
+
+def test_gradient_buffers_and_scalars(monkeypatch):
+    from mcsparse_b200 import operators
+    monkeypatch.setattr(operators, "embedding_gradient_buffer_size", lambda *a: 64)
+    monkeypatch.setattr(operators, "_GRADIENT_SIZES", {})
+
+    class Device(Stub):
+        pointer_mode = capi.MCSPARSE_POINTER_MODE_DEVICE
+
+    ids = torch.zeros(3, dtype=torch.int64)
+    table, y = mc.DnMat(torch.zeros(4, 8), 4, 8, 8), mc.DnMat(torch.zeros(3, 8), 3, 8, 8)
+    room, one = torch.zeros(64, dtype=torch.uint8), torch.ones(1)
+    for handle, scalars in ((Stub, {}), (Device, dict(alpha=one, beta=one))):
+        for buffer in (None, room[:63], room.float(), torch.zeros(128, dtype=torch.uint8)[::2]):
+            with pytest.raises(ValueError):
+                mc.embedding_gradient(handle, ids, y, table, buffer, **scalars)
+        with pytest.raises(mc.McsparseError):  # nothing to object to but the handle
+            mc.embedding_gradient(handle, ids, y, table, room, **scalars)
+    for bad in (1.0, one.double(), torch.ones(2)):  # a scalar of the host, of another type or size
+        with pytest.raises(ValueError):
+            mc.embedding_gradient(Device, ids, y, table, room, alpha=bad, beta=one)
+
+    class Elsewhere(Device):
+        class stream:
+            device_index = 0
+
+    with pytest.raises(ValueError):  # a scalar on another device than the handle's
+        operators._scalar(Elsewhere, one)
