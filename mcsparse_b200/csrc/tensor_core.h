@@ -84,6 +84,24 @@ __device__ __forceinline__ void tma_prefetch(const CUtensorMap* map) {
 // Orders this thread's ordinary shared-memory writes before later reads by TMA or tcgen05.mma.
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+// ---- cluster launch control: a running block takes over a block of the grid that has not started
+
+// Asks for one; the answer (16 bytes) completes on the barrier.
+__device__ __forceinline__ void ask_block(uint32_t answer, uint32_t bar) {
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(answer), "r"(bar) : "memory");
+}
+// Its blockIdx.x, or -1: there is none left (and none may be asked for again).
+__device__ __forceinline__ int asked_block(uint32_t answer) {
+    int x;
+    asm volatile(
+        "{\n .reg .b128 h;\n .reg .pred p;\n ld.shared.b128 h, [%1];\n clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n"
+        " mov.s32 %0, -1;\n @p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %0, h;\n}"
+        : "=r"(x)
+        : "r"(answer)
+        : "memory");
+    return x;
+}
+
 // ---- tensor memory
 
 __device__ __forceinline__ void tmem_alloc(uint32_t smem_slot, int columns) {
