@@ -46,7 +46,7 @@ struct Smem {
     static constexpr int kRing = 2 * kFixed;
     static constexpr int kVec = kRing + kStages * 2 * kStream;
     static constexpr int kBars = kVec + kStages * kVectors;
-    static constexpr int kTotal = kBars + 512 + 1024;  // (the start is aligned to 1024)
+    static constexpr int kTotal = kBars + 1024 + 1024;  // (the start is aligned to 1024)
     static_assert(kTotal <= 227 * 1024, "shared memory of a block");
 };
 
@@ -217,6 +217,50 @@ __device__ __forceinline__ float weight_gradients(const uint32_t* p, const uint3
     return a + b;
 }
 
+// What a block number stands for: 128 stationary rows of a head, and the streamed rows [begin, end) (keys kernel).
+struct Work {
+    Sequence sq;
+    int row0, head, begin, end;  // row0 < 0: nothing
+    int partial;                 // where the sums go instead of the outputs; -1: to the outputs
+};
+template <bool KEYS>
+__device__ __forceinline__ Work work_of(const Params& a, int number, int lane) {
+    const int heads = KEYS ? a.kv_heads : a.q_heads;
+    Work w;
+    w.sq = Sequence{0, 0, 0, 0};
+    w.row0 = -1, w.head = number % heads, w.begin = w.end = 0, w.partial = -1;
+    number /= heads;
+    const int far_blocks = KEYS ? a.far_slots * a.far_tiles : 0;
+    if (KEYS && number < far_blocks) {
+        const int far = number / a.far_tiles, tile = number % a.far_tiles;
+        const RaggedBlock fb = far_block(a.r, far, a.chunk, lane);
+        if (fb.b < 0) return w;
+        w.sq = sequence_of(a.r, fb.b);
+        if (tile * kRows >= w.sq.lk) return w;
+        const Split v = split_of(w.sq, tile * kRows, a.window, a.sinks, a.chunk);
+        if (fb.index >= v.pieces) return w;
+        w.row0 = tile * kRows;
+        w.begin = v.mid + fb.index * a.chunk;
+        w.end = fb.index + 1 < v.pieces ? w.begin + a.chunk : w.sq.lq;
+        w.partial = (far * a.far_tiles + tile) * a.kv_heads + w.head;
+    } else if (KEYS) {
+        const RaggedBlock rb = ragged_block(a.r.k_offsets, a.r.batch, a.r.total_k, number - far_blocks, kRows, lane);
+        if (rb.b < 0) return w;
+        w.sq = sequence_of(a.r, rb.b);
+        if ((int64_t)rb.index * kRows >= w.sq.lk) return w;
+        w.row0 = rb.index * kRows;
+        const Split v = split_of(w.sq, w.row0, a.window, a.sinks, a.chunk);
+        w.begin = v.begin, w.end = v.mid;
+        if (v.pieces > 0) w.partial = (((a.r.k_offsets == nullptr ? 0 : w.sq.k0 / a.chunk) + a.far_slots) * a.far_tiles + rb.index) * a.kv_heads + w.head;
+    } else {
+        const RaggedBlock rb = ragged_block(a.r.q_offsets, a.r.batch, a.r.total_q, a.slots - 1 - number, kRows, lane);
+        if (rb.b < 0) return w;
+        w.sq = sequence_of(a.r, rb.b);
+        if ((int64_t)rb.index * kRows < w.sq.lq) w.row0 = rb.index * kRows;
+    }
+    return w;
+}
+
 // KEYS: stationary K, V; streamed Q, dO. Otherwise: stationary Q, dO; streamed K, V.
 template <typename T, int DP, bool KEYS>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -234,90 +278,40 @@ __global__ void __launch_bounds__(kThreads, 1)
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem = (smem_u32(smem_raw) + 1023) & ~1023u;
     const int warp = uniform((int)(threadIdx.x >> 5)), lane = threadIdx.x & 31;
-    if (threadIdx.x == 32 * kLoadWarp) tma_prefetch(&map_fixed1), tma_prefetch(&map_fixed2), tma_prefetch(&map_stream1), tma_prefetch(&map_stream2);
-    // barriers: stationary operands; of every stage: there, clear, done with; of the buffers: S ready, dP ready, P ready, dS ready,
-    // S's columns free, dP's columns free; the last product done; the groups' exchange; the ends of the two issuing warps
+    // barriers: stationary operands, and their place free again; of every stage: there, clear, done with; of the buffers: S ready, dP
+    // ready, P ready, dS ready, S's columns free, dP's columns free; a work's last product done, its sums read; the groups' exchange;
+    // of the two places for what a block number stands for: written, read by all other warps; the answer to a request; the ends of
+    // the two issuing warps
     const uint32_t bars = smem + S::kBars;
-    const uint32_t bar_fixed = bars, bar_full = bars + 8, bar_clear = bar_full + 8 * kStages, bar_empty = bar_clear + 8 * kStages,
-                   bar_s = bar_empty + 8 * kStages, bar_dp = bar_s + 8 * kBuffers, bar_p = bar_dp + 8 * kBuffers, bar_ds = bar_p + 8 * kBuffers,
-                   bar_free_s = bar_ds + 8 * kBuffers, bar_free_dp = bar_free_s + 8 * kBuffers, bar_last = bar_free_dp + 8 * kBuffers,
-                   bar_x = bar_last + 8, bar_end = bar_x + 8, slot = bar_end + 16;
+    const uint32_t bar_fixed = bars, bar_fixed_free = bars + 8, bar_full = bars + 16, bar_clear = bar_full + 8 * kStages,
+                   bar_empty = bar_clear + 8 * kStages, bar_s = bar_empty + 8 * kStages, bar_dp = bar_s + 8 * kBuffers,
+                   bar_p = bar_dp + 8 * kBuffers, bar_ds = bar_p + 8 * kBuffers, bar_free_s = bar_ds + 8 * kBuffers,
+                   bar_free_dp = bar_free_s + 8 * kBuffers, bar_last = bar_free_dp + 8 * kBuffers, bar_drained = bar_last + 8,
+                   bar_x = bar_drained + 8, bar_work = bar_x + 8, bar_taken = bar_work + 16, bar_asked = bar_taken + 16,
+                   bar_end = bar_asked + 8, slot = bar_end + 16;
+    const uint32_t answer = bars + 512, works = answer + 16;  // 2 x 48 bytes
 
     grid_release();
-    // ---- the block's rows and its stream. (All launches but delta's may come up early: what they read that an earlier one of
-    // them wrote is delta, and the partial sums; every block waits for the launch ahead before it ends.)
-    const int heads = KEYS ? a.kv_heads : a.q_heads;
-    const int head = blockIdx.x % heads;
-    const int number = (int)(blockIdx.x / heads);
-    const int far_blocks = KEYS ? a.far_slots * a.far_tiles : 0;
-    Sequence sq;
-    int row0, begin = 0, end = 0, hops = 1;  // streamed rows [begin, end), once per head that streams
-    int first = 0, low = 0;                  // queries kernel: key tiles [0, first) and from `low` on
-    int64_t partial = -1;                    // where the sums go instead of the outputs
-    if (KEYS) {
-        hops = a.group;
-        if (number < far_blocks) {
-            const int far = number / a.far_tiles, tile = number % a.far_tiles;
-            const RaggedBlock fb = far_block(a.r, far, a.chunk, lane);
-            if (fb.b < 0) return grid_wait();
-            sq = sequence_of(a.r, fb.b);
-            row0 = tile * kRows;
-            if (row0 >= sq.lk) return grid_wait();
-            const Split v = split_of(sq, row0, a.window, a.sinks, a.chunk);
-            if (fb.index >= v.pieces) return grid_wait();
-            begin = v.mid + fb.index * a.chunk;
-            end = fb.index + 1 < v.pieces ? begin + a.chunk : sq.lq;
-            partial = ((int64_t)far * a.far_tiles + tile) * a.kv_heads + head;
-        } else {
-            const RaggedBlock rb = ragged_block(a.r.k_offsets, a.r.batch, a.r.total_k, number - far_blocks, kRows, lane);
-            if (rb.b < 0) return grid_wait();
-            sq = sequence_of(a.r, rb.b);
-            if ((int64_t)rb.index * kRows >= sq.lk) return grid_wait();
-            row0 = rb.index * kRows;
-            const Split v = split_of(sq, row0, a.window, a.sinks, a.chunk);
-            begin = v.begin, end = v.mid;
-            if (v.pieces > 0) {
-                const int far = (a.r.k_offsets == nullptr ? 0 : sq.k0 / a.chunk) + a.far_slots;
-                partial = ((int64_t)far * a.far_tiles + rb.index) * a.kv_heads + head;
-            }
-        }
-    } else {
-        const RaggedBlock rb = ragged_block(a.r.q_offsets, a.r.batch, a.r.total_q, a.slots - 1 - number, kRows, lane);
-        if (rb.b < 0) return grid_wait();
-        sq = sequence_of(a.r, rb.b);
-        if ((int64_t)rb.index * kRows >= sq.lq) return grid_wait();
-        row0 = rb.index * kRows;
-    }
-    const int shift = sq.lk - sq.lq;
-    const int rows = min(kRows, (KEYS ? sq.lk : sq.lq) - row0);
-    const int p_low = shift + row0, p_high = p_low + rows - 1;  // queries kernel: positions of the block
-    int tiles = 0;                                              // of one hop
-    if (KEYS) {
-        tiles = end > begin ? (end - begin + kTile - 1) / kTile : 0;
-    } else if (p_high >= 0) {
-        low = max(p_low - a.window + 1, 0) / kTile;
-        first = min((min(a.sinks, p_high + 1) + kTile - 1) / kTile, low);
-        tiles = first + p_high / kTile - low + 1;
-    }
-    tiles = uniform(tiles), first = uniform(first), low = uniform(low), begin = uniform(begin);
-    const int n = tiles * hops;
-    // first streamed row of tile i, relative to the sequence
-    const auto tile_row = [&](int i) {
-        if (KEYS) return begin + (i % tiles) * kTile;
-        return (i < first ? i : low + (i - first)) * kTile;
-    };
-
+    // (All launches but delta's may come up early: what they read that an earlier one of them wrote is delta, and the partial sums;
+    // every block waits for the launch ahead before it ends.)
+    Work work;
     if (warp == kSumWarp) {
         tmem_alloc(slot, 512);
-    } else if (threadIdx.x == 32 * kLoadWarp) {
-        bar_init(bar_fixed, 1);
-        for (int i = 0; i < 3 * kStages; ++i) bar_init(bar_full + 8 * i, 1);
-        for (int i = 0; i < kBuffers; ++i) {
-            bar_init(bar_s + 8 * i, 1), bar_init(bar_dp + 8 * i, 1), bar_init(bar_p + 8 * i, kRows), bar_init(bar_ds + 8 * i, kRows);
-            bar_init(bar_free_s + 8 * i, 1), bar_init(bar_free_dp + 8 * i, 1);
+    } else if (warp == kLoadWarp) {
+        if (lane == 0) {
+            tma_prefetch(&map_fixed1), tma_prefetch(&map_fixed2), tma_prefetch(&map_stream1), tma_prefetch(&map_stream2);
+            bar_init(bar_fixed, 1), bar_init(bar_fixed_free, 1);
+            for (int i = 0; i < 3 * kStages; ++i) bar_init(bar_full + 8 * i, 1);
+            for (int i = 0; i < kBuffers; ++i) {
+                bar_init(bar_s + 8 * i, 1), bar_init(bar_dp + 8 * i, 1), bar_init(bar_p + 8 * i, kRows), bar_init(bar_ds + 8 * i, kRows);
+                bar_init(bar_free_s + 8 * i, 1), bar_init(bar_free_dp + 8 * i, 1);
+            }
+            bar_init(bar_last, 1), bar_init(bar_drained, 2 * kRows), bar_init(bar_x, 2 * kRows), bar_init(bar_asked, 1);
+            for (int i = 0; i < 2; ++i) bar_init(bar_work + 8 * i, 1), bar_init(bar_taken + 8 * i, kThreads / 32 - 1), bar_init(bar_end + 8 * i, 1);
+            bar_init_fence();
         }
-        bar_init(bar_last, 1), bar_init(bar_x, 2 * kRows), bar_init(bar_end, 1), bar_init(bar_end + 8, 1);
-        bar_init_fence();
+        __syncwarp();
+        work = work_of<KEYS>(a, (int)blockIdx.x, lane);
     }
     fence_before();
     __syncthreads();
@@ -330,102 +324,211 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool failed = false;
     if (warp != kLoadWarp) grid_wait();  // (before any wait that is timed)
 
-    if (warp == kLoadWarp) {
-        // ---- loads
-        if (n > 0) {
-            const int hk = KEYS ? head : head / a.group;
-            if (elect()) {
-                bar_expect(bar_fixed, 2 * S::kFixed);
-                const int h1 = head * (KEYS ? a.k_mul : a.q_mul), h2 = head * (KEYS ? a.v_mul : a.go_mul);
-                const int row = (KEYS ? sq.k0 : sq.q0) + row0;
-                for (int c = 0; c < kBlocks; ++c) {
-                    tma_load_3d(smem + c * (kRows * 128), &map_fixed1, 64 * c, h1, row, bar_fixed);
-                    tma_load_3d(smem + S::kFixed + c * (kRows * 128), &map_fixed2, 64 * c, h2, row, bar_fixed);
-                }
-            }
-            // -lse (base 2) and delta of the tile's queries, fetched one tile ahead; a row that is none has -lse = -inf: P = 0
-            float l[2], d[2];
-            const auto fetch = [&](int i) {
-                if (!KEYS || i >= n) return;
-                const int h = head * a.group + i / tiles, row = tile_row(i);
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const int q = row + 2 * lane + x;
-                    l[x] = -INFINITY, d[x] = 0.0f;
-                    if (q < end) {
-                        const int64_t at = (int64_t)h * a.r.total_q + sq.q0 + q;
-                        const float v = __ldg(a.lse + at), w = __ldcg(a.delta + at);  // (both on their way before either is looked at)
-                        if (v != -INFINITY) l[x] = kLift - v * kLog2e;
-                        d[x] = -kLower * w;
-                    }
-                }
-            };
-            grid_wait();  // (the stationary operands are on their way)
-            fetch(0);
-            int issued = 0;
-            for (int i = 0; i < n; ++i) {
-                const int st = i % kStages;
-                if (i >= kStages && !bar_wait_warp(bar_empty + 8 * st, (i / kStages - 1) & 1, a.limit)) {
-                    failed = true;
-                    break;
-                }
-                if (KEYS) {
-                    const uint32_t vec = smem + S::kVec + st * S::kVectors + 8 * lane;
-                    asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(vec), "f"(l[0]), "f"(l[1]) : "memory");
-                    asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(vec + 4 * kTile), "f"(d[0]), "f"(d[1]) : "memory");
-                    fetch(i + 1);
-                    __syncwarp();
-                }
-                if (elect()) {
-                    bar_expect(bar_full + 8 * st, 2 * S::kStream);
-                    const int h = KEYS ? head * a.group + i / tiles : hk;
-                    const int h1 = h * (KEYS ? a.q_mul : a.k_mul), h2 = h * (KEYS ? a.go_mul : a.v_mul);
-                    const int row = (KEYS ? sq.q0 : sq.k0) + tile_row(i);
-                    const uint32_t to = smem + S::kRing + st * 2 * S::kStream;
-                    for (int c = 0; c < kBlocks; ++c) {
-                        tma_load_3d(to + c * (kTile * 128), &map_stream1, 64 * c, h1, row, bar_full + 8 * st);
-                        tma_load_3d(to + S::kStream + c * (kTile * 128), &map_stream2, 64 * c, h2, row, bar_full + 8 * st);
-                    }
-                }
-                issued = i + 1;
-            }
-            // nothing of this block's memory is given back while a copy is on its way, whoever gave up
-            bar_wait(bar_fixed, 0, kDrain);
-            for (int i = max(0, issued - kStages); i < issued; ++i) bar_wait(bar_full + 8 * (i % kStages), (i / kStages) & 1, kDrain);
+    // All warps run through the same work, each with running counts of the barriers' phases: `total` tiles, `turns` works with tiles.
+    int turn = 0, total = 0, turns = 0;
+    int shift, rows, p_low, p_high;       // (positions: queries kernel)
+    int tiles, n, first, low, begin;      // tiles of one head that streams, and of all; queries kernel: key tiles [0, first) and from `low` on
+    const auto plan = [&] {
+        const int hops = KEYS ? a.group : 1;
+        shift = work.sq.lk - work.sq.lq;
+        rows = min(kRows, (KEYS ? work.sq.lk : work.sq.lq) - work.row0);
+        p_low = shift + work.row0, p_high = p_low + rows - 1;
+        tiles = first = low = 0, begin = uniform(work.begin);
+        if (KEYS) {
+            tiles = work.end > work.begin ? (work.end - work.begin + kTile - 1) / kTile : 0;
+        } else if (p_high >= 0) {
+            low = max(p_low - a.window + 1, 0) / kTile;
+            first = min((min(a.sinks, p_high + 1) + kTile - 1) / kTile, low);
+            tiles = first + p_high / kTile - low + 1;
         }
+        tiles = uniform(tiles), first = uniform(first), low = uniform(low);
+        n = tiles * hops;
+        total = uniform(total), turns = uniform(turns);
+    };
+    // first streamed row of tile i, relative to the sequence
+    const auto tile_row = [&](int i) {
+        if (KEYS) return begin + (i % tiles) * kTile;
+        return (i < first ? i : low + (i - first)) * kTile;
+    };
+    // Whole warps; false: no more, or `failed`.
+    const auto next_work = [&] {
+        const int at = turn & 1;
+        if (!bar_wait_warp(bar_work + 8 * at, (turn >> 1) & 1, a.limit)) {
+            failed = true;
+            return false;
+        }
+        const uint32_t from = works + 48 * at;
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(work.sq.q0), "=r"(work.sq.lq), "=r"(work.sq.k0), "=r"(work.sq.lk) : "r"(from) : "memory");
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(work.row0), "=r"(work.head), "=r"(work.begin), "=r"(work.end) : "r"(from + 16) : "memory");
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(work.partial) : "r"(from + 32) : "memory");
         __syncwarp();
+        if (elect()) bar_arrive(bar_taken + 8 * at);
+        ++turn;
+        if (uniform(work.row0) < 0) return false;
+        plan();
+        return true;
+    };
+    const auto work_done = [&] { total += n, turns += n > 0; };
+
+    if (warp == kLoadWarp) {
+        // ---- loads, and the order of the work: when a work's last loads are issued, the place of a block of the grid that has not
+        // started is taken over (cluster launch control), so that its loads and first products run beside the end of this one.
+        int asked = 0;
+        const auto publish = [&](int row0) {
+            const int at = turn & 1;
+            if (turn >= 2 && !bar_wait_warp(bar_taken + 8 * at, ((turn >> 1) - 1) & 1, a.limit)) {
+                failed = true;
+                return;
+            }
+            if (elect()) {
+                const uint32_t to = works + 48 * at;
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(work.sq.q0), "r"(work.sq.lq), "r"(work.sq.k0), "r"(work.sq.lk) : "memory");
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to + 16), "r"(row0), "r"(work.head), "r"(work.begin), "r"(work.end) : "memory");
+                asm volatile("st.shared.u32 [%0], %1;" ::"r"(to + 32), "r"(work.partial) : "memory");
+                bar_arrive(bar_work + 8 * at);
+            }
+            __syncwarp();
+            ++turn;
+        };
+        int issued = 0;  // tiles, of all works
+        while (!failed) {
+            if (work.row0 >= 0) {
+                publish(work.row0);
+                plan();
+                const Sequence sq = work.sq;
+                const int head = work.head, hk = KEYS ? head : head / a.group;
+                // -lse (base 2) and delta of the tile's queries, fetched one tile ahead; a row that is none has -lse = -inf: P = 0
+                float l[2], d[2];
+                const auto fetch = [&](int i) {
+                    if (!KEYS || i >= n) return;
+                    const int h = head * a.group + i / tiles, row = tile_row(i);
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const int q = row + 2 * lane + x;
+                        l[x] = -INFINITY, d[x] = 0.0f;
+                        if (q < work.end) {
+                            const int64_t at = (int64_t)h * a.r.total_q + sq.q0 + q;
+                            const float v = __ldg(a.lse + at), w = __ldcg(a.delta + at);  // (both on their way before either is looked at)
+                            if (v != -INFINITY) l[x] = kLift - v * kLog2e;
+                            d[x] = -kLower * w;
+                        }
+                    }
+                };
+                if (n > 0 && !failed) {
+                    if (turns > 0) {
+                        fetch(0);
+                        if (!bar_wait_warp(bar_fixed_free, (turns - 1) & 1, a.limit)) {
+                            failed = true;
+                            break;
+                        }
+                    }
+                    if (elect()) {
+                        bar_expect(bar_fixed, 2 * S::kFixed);
+                        const int h1 = head * (KEYS ? a.k_mul : a.q_mul), h2 = head * (KEYS ? a.v_mul : a.go_mul);
+                        const int row = (KEYS ? sq.k0 : sq.q0) + work.row0;
+                        for (int c = 0; c < kBlocks; ++c) {
+                            tma_load_3d(smem + c * (kRows * 128), &map_fixed1, 64 * c, h1, row, bar_fixed);
+                            tma_load_3d(smem + S::kFixed + c * (kRows * 128), &map_fixed2, 64 * c, h2, row, bar_fixed);
+                        }
+                    }
+                    if (turns == 0) {
+                        grid_wait();  // (the first stationary operands are on their way)
+                        fetch(0);
+                    }
+                    ++turns;
+                    for (int i = 0; i < n; ++i) {
+                        const int g = total + i, st = g % kStages;
+                        if (g >= kStages && !bar_wait_warp(bar_empty + 8 * st, (g / kStages - 1) & 1, a.limit)) {
+                            failed = true;
+                            break;
+                        }
+                        if (KEYS) {
+                            const uint32_t vec = smem + S::kVec + st * S::kVectors + 8 * lane;
+                            asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(vec), "f"(l[0]), "f"(l[1]) : "memory");
+                            asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(vec + 4 * kTile), "f"(d[0]), "f"(d[1]) : "memory");
+                            fetch(i + 1);
+                            __syncwarp();
+                        }
+                        if (elect()) {
+                            bar_expect(bar_full + 8 * st, 2 * S::kStream);
+                            const int h = KEYS ? head * a.group + i / tiles : hk;
+                            const int h1 = h * (KEYS ? a.q_mul : a.k_mul), h2 = h * (KEYS ? a.go_mul : a.v_mul);
+                            const int row = (KEYS ? sq.q0 : sq.k0) + tile_row(i);
+                            const uint32_t to = smem + S::kRing + st * 2 * S::kStream;
+                            for (int c = 0; c < kBlocks; ++c) {
+                                tma_load_3d(to + c * (kTile * 128), &map_stream1, 64 * c, h1, row, bar_full + 8 * st);
+                                tma_load_3d(to + S::kStream + c * (kTile * 128), &map_stream2, 64 * c, h2, row, bar_full + 8 * st);
+                            }
+                        }
+                        issued = g + 1;
+                    }
+                    total += n;
+                }
+            }
+            if (failed) break;
+            if (elect()) {
+                bar_expect(bar_asked, 16);
+                ask_block(answer, bar_asked);
+            }
+            __syncwarp();
+            if (!bar_wait_warp(bar_asked, asked & 1, a.limit)) {
+                bar_wait_warp(bar_asked, asked & 1, kDrain);
+                failed = true;
+                break;
+            }
+            ++asked;
+            const int number = uniform(asked_block(answer));
+            fence_async();  // (the next answer is written by another proxy than this one was read by)
+            __syncwarp();
+            if (number < 0) {
+                publish(-1);
+                break;
+            }
+            work = work_of<KEYS>(a, number, lane);
+        }
+        // nothing of this block's memory is given back while a copy is on its way, whoever gave up
+        if (turns > 0) bar_wait_warp(bar_fixed, (turns - 1) & 1, kDrain);
+        for (int i = max(0, issued - kStages); i < issued; ++i) bar_wait_warp(bar_full + 8 * (i % kStages), (i / kStages) & 1, kDrain);
     } else if (warp == kScoreWarp) {
         // ---- S and dP, issued by one thread, each once its columns are free
         constexpr uint32_t kDesc = mma_desc(!kHalf, kTile, false);
-        if (n > 0 && elect()) {
-            failed = !bar_wait(bar_fixed, 0, a.limit);
-            const uint64_t f1 = smem_desc(smem), f2 = smem_desc(smem + S::kFixed);
-            for (int i = 0; i < n && !failed; ++i) {
-                const int st = i % kStages, b = i % kBuffers;
-                const uint32_t before = (i / kBuffers - 1) & 1;  // the phase of the buffer's last use
-                const uint32_t s1 = smem + S::kRing + st * 2 * S::kStream;
-                const uint64_t m1 = smem_desc(s1), m2 = smem_desc(s1 + S::kStream);
-                if (!bar_wait(bar_clear + 8 * st, (i / kStages) & 1, a.limit) || (i >= kBuffers && !bar_wait(bar_free_s + 8 * b, before, a.limit))) {
-                    failed = true;
-                    break;
-                }
-                fence_after();
+        const uint64_t f1 = smem_desc(smem), f2 = smem_desc(smem + S::kFixed);
+        while (!failed && next_work()) {
+            if (n > 0 && elect()) {
+                failed = !bar_wait(bar_fixed, turns & 1, a.limit);
+                for (int i = 0; i < n && !failed; ++i) {
+                    const int g = total + i, st = g % kStages, b = g % kBuffers;
+                    const uint32_t before = (g / kBuffers - 1) & 1;  // the phase of the buffer's last use
+                    const uint32_t s1 = smem + S::kRing + st * 2 * S::kStream;
+                    const uint64_t m1 = smem_desc(s1), m2 = smem_desc(s1 + S::kStream);
+                    if (!bar_wait(bar_clear + 8 * st, (g / kStages) & 1, a.limit) || (g >= kBuffers && !bar_wait(bar_free_s + 8 * b, before, a.limit))) {
+                        failed = true;
+                        break;
+                    }
+                    fence_after();
 #pragma unroll
-                for (int k = 0; k < DP / 16; ++k)
-                    mma_ss(t_s + kTile * b, desc_at(f1, (k >> 2) * (kRows * 128) + (k & 3) * 32), desc_at(m1, (k >> 2) * (kTile * 128) + (k & 3) * 32),
-                           kDesc | a.negate, k > 0);
-                mma_commit(bar_s + 8 * b);
-                if (i >= kBuffers && !bar_wait(bar_free_dp + 8 * b, before, a.limit)) {
-                    failed = true;
-                    break;
-                }
-                fence_after();
+                    for (int k = 0; k < DP / 16; ++k)
+                        mma_ss(t_s + kTile * b, desc_at(f1, (k >> 2) * (kRows * 128) + (k & 3) * 32), desc_at(m1, (k >> 2) * (kTile * 128) + (k & 3) * 32),
+                               kDesc | a.negate, k > 0);
+                    mma_commit(bar_s + 8 * b);
+                    if (g >= kBuffers && !bar_wait(bar_free_dp + 8 * b, before, a.limit)) {
+                        failed = true;
+                        break;
+                    }
+                    fence_after();
 #pragma unroll
-                for (int k = 0; k < DP / 16; ++k)
-                    mma_ss(t_dp + kTile * b, desc_at(f2, (k >> 2) * (kRows * 128) + (k & 3) * 32), desc_at(m2, (k >> 2) * (kTile * 128) + (k & 3) * 32),
-                           kDesc, k > 0);
-                mma_commit(bar_dp + 8 * b);
+                    for (int k = 0; k < DP / 16; ++k)
+                        mma_ss(t_dp + kTile * b, desc_at(f2, (k >> 2) * (kRows * 128) + (k & 3) * 32), desc_at(m2, (k >> 2) * (kTile * 128) + (k & 3) * 32),
+                               kDesc, k > 0);
+                    mma_commit(bar_dp + 8 * b);
+                }
+                mma_commit(bar_fixed_free);
             }
+            __syncwarp();
+            failed = __any_sync(0xffffffffu, failed);
+            work_done();
+        }
+        if (elect()) {
             mma_commit(bar_end);  // the tensor memory is given back only when no product uses it any more
             bar_wait(bar_end, 0, kDrain);
         }
@@ -433,33 +536,41 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (warp == kSumWarp) {
         // ---- dV and dK, or M and dQ, issued by one thread
         constexpr uint32_t kDesc = mma_desc(!kHalf, DP, true);
-        if (n > 0 && elect()) {
-            for (int i = 0; i < n; ++i) {
-                const int st = i % kStages, b = i % kBuffers;
-                const uint32_t phase = (i / kBuffers) & 1;
-                const uint32_t s1 = smem + S::kRing + st * 2 * S::kStream;
-                const uint64_t m1 = smem_desc(s1, kTile * 128), m2 = smem_desc(s1 + S::kStream, kTile * 128);
-                if (!bar_wait(bar_clear + 8 * st, (i / kStages) & 1, a.limit) || !bar_wait(bar_p + 8 * b, phase, a.limit)) {
-                    failed = true;
-                    break;
-                }
-                fence_after();
+        while (!failed && next_work()) {
+            if (n > 0 && elect()) {
+                failed = turns > 0 && !bar_wait(bar_drained, (turns - 1) & 1, a.limit);
+                for (int i = 0; i < n && !failed; ++i) {
+                    const int g = total + i, st = g % kStages, b = g % kBuffers;
+                    const uint32_t phase = (g / kBuffers) & 1;
+                    const uint32_t s1 = smem + S::kRing + st * 2 * S::kStream;
+                    const uint64_t m1 = smem_desc(s1, kTile * 128), m2 = smem_desc(s1 + S::kStream, kTile * 128);
+                    if (!bar_wait(bar_clear + 8 * st, (g / kStages) & 1, a.limit) || !bar_wait(bar_p + 8 * b, phase, a.limit)) {
+                        failed = true;
+                        break;
+                    }
+                    fence_after();
 #pragma unroll
-                for (int k = 0; k < kTile / 16; ++k)
-                    mma_ts(t_out1, t_s + kTile * b + 8 * k, desc_at(KEYS ? m2 : m1, k * 2048), kDesc, i > 0 || k > 0);
-                mma_commit(bar_free_s + 8 * b);
-                if (!bar_wait(bar_ds + 8 * b, phase, a.limit)) {
-                    failed = true;
-                    break;
-                }
-                fence_after();
+                    for (int k = 0; k < kTile / 16; ++k)
+                        mma_ts(t_out1, t_s + kTile * b + 8 * k, desc_at(KEYS ? m2 : m1, k * 2048), kDesc, i > 0 || k > 0);
+                    mma_commit(bar_free_s + 8 * b);
+                    if (!bar_wait(bar_ds + 8 * b, phase, a.limit)) {
+                        failed = true;
+                        break;
+                    }
+                    fence_after();
 #pragma unroll
-                for (int k = 0; k < kTile / 16; ++k)
-                    mma_ts(t_out2, t_dp + kTile * b + 8 * k, desc_at(m1, k * 2048), kDesc, i > 0 || k > 0);
-                mma_commit(bar_free_dp + 8 * b);
-                mma_commit(bar_empty + 8 * st);
-                if (i == n - 1) mma_commit(bar_last);
+                    for (int k = 0; k < kTile / 16; ++k)
+                        mma_ts(t_out2, t_dp + kTile * b + 8 * k, desc_at(m1, k * 2048), kDesc, i > 0 || k > 0);
+                    mma_commit(bar_free_dp + 8 * b);
+                    mma_commit(bar_empty + 8 * st);
+                    if (i == n - 1) mma_commit(bar_last);
+                }
             }
+            __syncwarp();
+            failed = __any_sync(0xffffffffu, failed);
+            work_done();
+        }
+        if (elect()) {
             mma_commit(bar_end + 8);
             bar_wait(bar_end + 8, 0, kDrain);
         }
@@ -467,163 +578,174 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (warp == kClearWarp) {
         // ---- rows whose weight is zero for every row here are cleared before they enter a sum: zero times a NaN that lies there
         // would not be zero. Keys kernel: queries behind the last one; queries kernel: keys nobody sees.
-        const int first_seen = max(p_low - a.window + 1, 0);  // queries kernel: the first key in reach of some row here
-        for (int i = 0; i < n; ++i) {
-            const int st = i % kStages, row = tile_row(i);
-            if (!bar_wait_warp(bar_full + 8 * st, (i / kStages) & 1, a.limit)) {
-                failed = true;
-                break;
-            }
-            const int clear_low = KEYS ? 0 : min(max(first_seen - row, 0), kTile);
-            const int keep = KEYS ? 0 : min(max(a.sinks - row, 0), kTile);
-            const int clear_high = min(max((KEYS ? end : p_high + 1) - row, 0), kTile);
-            if (clear_low > keep || clear_high < kTile) {
-                for (int x = lane; x < (KEYS ? 2 : 1) * kTile * 8 * kBlocks; x += 32) {  // (stream 2 lies behind stream 1)
-                    const int at = (x >> 3) & (kTile - 1);
-                    if ((at < clear_low && at >= keep) || at >= clear_high)
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(smem + S::kRing + st * 2 * S::kStream + x * 16), "r"(0) : "memory");
+        while (!failed && next_work()) {
+            const int first_seen = max(p_low - a.window + 1, 0);  // queries kernel: the first key in reach of some row here
+            for (int i = 0; i < n; ++i) {
+                const int g = total + i, st = g % kStages, row = tile_row(i);
+                if (!bar_wait_warp(bar_full + 8 * st, (g / kStages) & 1, a.limit)) {
+                    failed = true;
+                    break;
                 }
-                fence_async();
+                const int clear_low = KEYS ? 0 : min(max(first_seen - row, 0), kTile);
+                const int keep = KEYS ? 0 : min(max(a.sinks - row, 0), kTile);
+                const int clear_high = min(max((KEYS ? work.end : p_high + 1) - row, 0), kTile);
+                if (clear_low > keep || clear_high < kTile) {
+                    for (int x = lane; x < (KEYS ? 2 : 1) * kTile * 8 * kBlocks; x += 32) {  // (stream 2 lies behind stream 1)
+                        const int at = (x >> 3) & (kTile - 1);
+                        if ((at < clear_low && at >= keep) || at >= clear_high)
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(smem + S::kRing + st * 2 * S::kStream + x * 16), "r"(0) : "memory");
+                    }
+                    fence_async();
+                    __syncwarp();
+                }
+                if (elect()) bar_arrive(bar_clear + 8 * st);
                 __syncwarp();
             }
-            if (elect()) bar_arrive(bar_clear + 8 * st);
-            __syncwarp();
+            work_done();
         }
     } else {
         // ---- P and dS: thread = stationary row; the two groups take the tiles in turn
         const int group = warp >> 2;
         const int r = threadIdx.x & (kRows - 1);
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;
-        const int64_t token = (int64_t)(KEYS ? sq.k0 : sq.q0) + row0 + r;
-        float own_l = -INFINITY, own_d = 0.0f;  // queries kernel: the row's -lse and -delta
-        if (!KEYS && r < rows) {
-            const int64_t at = (int64_t)head * a.r.total_q + token;
-            const float v = __ldg(a.lse + at);
-            if (v != -INFINITY) own_l = kLift - v * kLog2e;
-            own_d = -kLower * __ldcg(a.delta + at);
-        }
-        float e = 0.0f;  // queries kernel: the sum of the row's dS
-        for (int i = group; i < n; i += 2) {
-            const int b = i % kBuffers;
-            const uint32_t phase = (i / kBuffers) & 1;
-            const uint32_t ts = t_s + kTile * b + lanes, td = t_dp + kTile * b + lanes;
-            // (the second wait is over by then; it is there for the vectors, which ordinary stores wrote)
-            if (!bar_wait_warp(bar_s + 8 * b, phase, a.limit) || (KEYS && !bar_wait_warp(bar_full + 8 * (i % kStages), (i / kStages) & 1, a.limit))) {
-                failed = true;
-                break;
+        while (!failed && next_work()) {
+            const int row0 = work.row0;
+            const int64_t token = (int64_t)(KEYS ? work.sq.k0 : work.sq.q0) + row0 + r;
+            float own_l = -INFINITY, own_d = 0.0f;  // queries kernel: the row's -lse and -delta
+            if (!KEYS && r < rows) {
+                const int64_t at = (int64_t)work.head * a.r.total_q + token;
+                const float v = __ldg(a.lse + at);
+                if (v != -INFINITY) own_l = kLift - v * kLog2e;
+                own_d = -kLower * __ldcg(a.delta + at);
             }
-            fence_after();
-            uint32_t p[kTile];
-            tmem_load32(ts, p);
-            tmem_load32(ts + 32, p + 32);
-            const int row = tile_row(i);
-            uint64_t seen = ~0ull;
-            if (KEYS) {
-                // key j = row0 + r, query at position p = shift + row + c: seen iff p >= j and (p < j + window or j < sinks)
-                const int p0 = shift + row, j = row0 + r;  // (positions)
-                if (p0 < row0 + kRows - 1 || (p0 + kTile - 1 >= row0 + a.window && row0 + kRows > a.sinks)) {
-                    const int from = min(max(j - p0, 0), 64);
-                    const int upto = j < a.sinks ? 64 : min(max(j + a.window - p0, 0), 64);
-                    seen = (from < 64 ? ~0ull << from : 0ull) & (upto < 64 ? (1ull << upto) - 1 : ~0ull);
+            float e = 0.0f;  // queries kernel: the sum of the row's dS
+            for (int i = (group ^ total) & 1; i < n; i += 2) {
+                const int g = total + i, b = g % kBuffers;
+                const uint32_t phase = (g / kBuffers) & 1;
+                const uint32_t ts = t_s + kTile * b + lanes, td = t_dp + kTile * b + lanes;
+                // (the second wait is over by then; it is there for the vectors, which ordinary stores wrote)
+                if (!bar_wait_warp(bar_s + 8 * b, phase, a.limit) || (KEYS && !bar_wait_warp(bar_full + 8 * (g % kStages), (g / kStages) & 1, a.limit))) {
+                    failed = true;
+                    break;
                 }
-            } else {
-                // query at p, key j = row + c: seen iff j <= p and (j > p - window or j < sinks)
-                const int at = p_low + r;
-                if (row + kTile - 1 > p_low || (row <= p_low + kRows - 1 - a.window && row + kTile > a.sinks)) {
-                    const int upto = min(max(at + 1 - row, 0), 64), from = min(max(at - a.window + 1 - row, 0), 64);
-                    const int keep = min(max(a.sinks - row, 0), 64);
-                    const uint64_t near = from < 64 ? ~0ull << from : 0ull, kept = keep < 64 ? (1ull << keep) - 1 : ~0ull;
-                    seen = (near | kept) & (upto < 64 ? (1ull << upto) - 1 : ~0ull);
-                }
-            }
-            const uint32_t vec = smem + S::kVec + (i % kStages) * S::kVectors;
-            const bool masked = !__all_sync(0xffffffffu, seen == ~0ull);
-            wait_loads();
-            after_loads32(p), after_loads32(p + 32);
-            if (masked)
-                weights<T, KEYS, true>(p, ts, seen, vec, own_l, a.scale_log2);
-            else
-                weights<T, KEYS, false>(p, ts, seen, vec, own_l, a.scale_log2);
-            wait_stores();
-            fence_before();
-            bar_arrive(bar_p + 8 * b);
-            if (!bar_wait_warp(bar_dp + 8 * b, phase, a.limit)) {
-                failed = true;
-                break;
-            }
-            fence_after();
-            uint32_t d[kTile];
-            tmem_load32(td, d);
-            tmem_load32(td + 32, d + 32);
-            wait_loads();
-            after_loads32(d), after_loads32(d + 32);
-            if (masked)
-                e += weight_gradients<T, KEYS, true>(p, d, td, seen, vec + 4 * kTile, own_d);
-            else
-                e += weight_gradients<T, KEYS, false>(p, d, td, seen, vec + 4 * kTile, own_d);
-            wait_stores();
-            fence_before();
-            bar_arrive(bar_ds + 8 * b);
-        }
-        // ---- outputs: keys kernel: one group writes dV, the other dK; queries kernel: each half of dQ's columns
-        if (n > 0 && !failed) {
-            if (!KEYS) {  // the row's sum over the tiles of both groups
-                const uint32_t words = smem + S::kVec;
-                asm volatile("st.shared.f32 [%0], %1;" ::"r"(words + 4 * (kRows * group + r)), "f"(e) : "memory");
-                bar_arrive(bar_x);
-                failed = !bar_wait_warp(bar_x, 0, a.limit);
-                float e0, e1;
-                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(e0) : "r"(words + 4 * r) : "memory");
-                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(e1) : "r"(words + 4 * (kRows + r)) : "memory");
-                e = e0 + e1;
-                if (group == 0 && r < rows && !failed) a.delta_out[(int64_t)head * a.r.total_q + token] = e - own_d / kLower;
-            }
-            failed = !bar_wait_warp(bar_last, 0, a.limit) || failed;
-            fence_after();
-        }
-        const float less = -e * kLower;
-        const float factor = KEYS && group == 0 ? kLower : a.scale;
-        T* out = group == 1 && KEYS ? static_cast<T*>(a.out2) + token * a.out2_token + (int64_t)head * a.out2_head
-                                    : static_cast<T*>(a.out1) + token * a.out1_token + (int64_t)head * a.out1_head;
-        float* part = partial < 0 ? nullptr : a.partial + ((partial * 2 + group) * kRows + r) * DP;
-        const int c0 = KEYS ? 0 : group * (DP / 2), c1 = KEYS ? DP : c0 + DP / 2;
-#pragma unroll 1
-        for (int c = c0; c < c1; c += 32) {
-            uint32_t o[32];
-            if (n > 0 && !failed) {
-                tmem_load32((KEYS && group == 0 ? t_out1 : t_out2) + lanes + c, o);
-                if (!KEYS) {
-                    uint32_t m[32];
-                    tmem_load32(t_out1 + lanes + c, m);
-                    wait_loads();
-                    after_loads32(o), after_loads32(m);
-#pragma unroll
-                    for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(fmaf(less, __uint_as_float(m[x]), __uint_as_float(o[x])));
+                fence_after();
+                uint32_t p[kTile];
+                tmem_load32(ts, p);
+                tmem_load32(ts + 32, p + 32);
+                const int row = tile_row(i);
+                uint64_t seen = ~0ull;
+                if (KEYS) {
+                    // key j = row0 + r, query at position p = shift + row + c: seen iff p >= j and (p < j + window or j < sinks)
+                    const int p0 = shift + row, j = row0 + r;  // (positions)
+                    if (p0 < row0 + kRows - 1 || (p0 + kTile - 1 >= row0 + a.window && row0 + kRows > a.sinks)) {
+                        const int from = min(max(j - p0, 0), 64);
+                        const int upto = j < a.sinks ? 64 : min(max(j + a.window - p0, 0), 64);
+                        seen = (from < 64 ? ~0ull << from : 0ull) & (upto < 64 ? (1ull << upto) - 1 : ~0ull);
+                    }
                 } else {
-                    wait_loads();
-                    after_loads32(o);
+                    // query at p, key j = row + c: seen iff j <= p and (j > p - window or j < sinks)
+                    const int at = p_low + r;
+                    if (row + kTile - 1 > p_low || (row <= p_low + kRows - 1 - a.window && row + kTile > a.sinks)) {
+                        const int upto = min(max(at + 1 - row, 0), 64), from = min(max(at - a.window + 1 - row, 0), 64);
+                        const int keep = min(max(a.sinks - row, 0), 64);
+                        const uint64_t near = from < 64 ? ~0ull << from : 0ull, kept = keep < 64 ? (1ull << keep) - 1 : ~0ull;
+                        seen = (near | kept) & (upto < 64 ? (1ull << upto) - 1 : ~0ull);
+                    }
                 }
-            } else {
-#pragma unroll
-                for (int x = 0; x < 32; ++x) o[x] = 0u;
+                const uint32_t vec = smem + S::kVec + (g % kStages) * S::kVectors;
+                const bool masked = !__all_sync(0xffffffffu, seen == ~0ull);
+                wait_loads();
+                after_loads32(p), after_loads32(p + 32);
+                if (masked)
+                    weights<T, KEYS, true>(p, ts, seen, vec, own_l, a.scale_log2);
+                else
+                    weights<T, KEYS, false>(p, ts, seen, vec, own_l, a.scale_log2);
+                wait_stores();
+                fence_before();
+                bar_arrive(bar_p + 8 * b);
+                if (!bar_wait_warp(bar_dp + 8 * b, phase, a.limit)) {
+                    failed = true;
+                    break;
+                }
+                fence_after();
+                uint32_t d[kTile];
+                tmem_load32(td, d);
+                tmem_load32(td + 32, d + 32);
+                wait_loads();
+                after_loads32(d), after_loads32(d + 32);
+                if (masked)
+                    e += weight_gradients<T, KEYS, true>(p, d, td, seen, vec + 4 * kTile, own_d);
+                else
+                    e += weight_gradients<T, KEYS, false>(p, d, td, seen, vec + 4 * kTile, own_d);
+                wait_stores();
+                fence_before();
+                bar_arrive(bar_ds + 8 * b);
             }
-            if (failed) continue;
-            if (part != nullptr) {
+            // ---- outputs: keys kernel: one group writes dV, the other dK; queries kernel: each half of dQ's columns
+            if (n > 0 && !failed) {
+                if (!KEYS) {  // the row's sum over the tiles of both groups (two places in turn: a slow reader of the last work's)
+                    const uint32_t words = smem + S::kVec + (turns & 1) * (8 * kRows);
+                    asm volatile("st.shared.f32 [%0], %1;" ::"r"(words + 4 * (kRows * group + r)), "f"(e) : "memory");
+                    bar_arrive(bar_x);
+                    failed = !bar_wait_warp(bar_x, turns & 1, a.limit);
+                    float e0, e1;
+                    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(e0) : "r"(words + 4 * r) : "memory");
+                    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(e1) : "r"(words + 4 * (kRows + r)) : "memory");
+                    e = e0 + e1;
+                    if (group == 0 && r < rows && !failed) a.delta_out[(int64_t)work.head * a.r.total_q + token] = e - own_d / kLower;
+                }
+                failed = !bar_wait_warp(bar_last, turns & 1, a.limit) || failed;
+                fence_after();
+            }
+            if (failed) break;
+            const float less = -e * kLower;
+            const float factor = KEYS && group == 0 ? kLower : a.scale;
+            T* out = group == 1 && KEYS ? static_cast<T*>(a.out2) + token * a.out2_token + (int64_t)work.head * a.out2_head
+                                        : static_cast<T*>(a.out1) + token * a.out1_token + (int64_t)work.head * a.out1_head;
+            float* part = work.partial < 0 ? nullptr : a.partial + (((int64_t)work.partial * 2 + group) * kRows + r) * DP;
+            const int c0 = KEYS ? 0 : group * (DP / 2), c1 = KEYS ? DP : c0 + DP / 2;
+#pragma unroll 1
+            for (int c = c0; c < c1; c += 32) {
+                uint32_t o[32];
+                if (n > 0) {
+                    tmem_load32((KEYS && group == 0 ? t_out1 : t_out2) + lanes + c, o);
+                    if (!KEYS) {
+                        uint32_t m[32];
+                        tmem_load32(t_out1 + lanes + c, m);
+                        wait_loads();
+                        after_loads32(o), after_loads32(m);
 #pragma unroll
-                for (int x = 0; x < 32; x += 4) *reinterpret_cast<uint4*>(part + c + x) = make_uint4(o[x], o[x + 1], o[x + 2], o[x + 3]);
-            } else if (r < rows) {
+                        for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(fmaf(less, __uint_as_float(m[x]), __uint_as_float(o[x])));
+                    } else {
+                        wait_loads();
+                        after_loads32(o);
+                    }
+                    if (c + 32 == c1) {  // the next work's products may overwrite the sums
+                        fence_before();
+                        bar_arrive(bar_drained);
+                    }
+                } else {
 #pragma unroll
-                for (int x = 0; x < 32; x += 8) {
-                    if (c + x < a.dim) {
-                        uint4 w;
-                        w.x = pack2<T>(__uint_as_float(o[x]) * factor, __uint_as_float(o[x + 1]) * factor);
-                        w.y = pack2<T>(__uint_as_float(o[x + 2]) * factor, __uint_as_float(o[x + 3]) * factor);
-                        w.z = pack2<T>(__uint_as_float(o[x + 4]) * factor, __uint_as_float(o[x + 5]) * factor);
-                        w.w = pack2<T>(__uint_as_float(o[x + 6]) * factor, __uint_as_float(o[x + 7]) * factor);
-                        *reinterpret_cast<uint4*>(out + c + x) = w;
+                    for (int x = 0; x < 32; ++x) o[x] = 0u;
+                }
+                if (part != nullptr) {
+#pragma unroll
+                    for (int x = 0; x < 32; x += 4) *reinterpret_cast<uint4*>(part + c + x) = make_uint4(o[x], o[x + 1], o[x + 2], o[x + 3]);
+                } else if (r < rows) {
+#pragma unroll
+                    for (int x = 0; x < 32; x += 8) {
+                        if (c + x < a.dim) {
+                            uint4 w;
+                            w.x = pack2<T>(__uint_as_float(o[x]) * factor, __uint_as_float(o[x + 1]) * factor);
+                            w.y = pack2<T>(__uint_as_float(o[x + 2]) * factor, __uint_as_float(o[x + 3]) * factor);
+                            w.z = pack2<T>(__uint_as_float(o[x + 4]) * factor, __uint_as_float(o[x + 5]) * factor);
+                            w.w = pack2<T>(__uint_as_float(o[x + 6]) * factor, __uint_as_float(o[x + 7]) * factor);
+                            *reinterpret_cast<uint4*>(out + c + x) = w;
+                        }
                     }
                 }
             }
+            work_done();
         }
         fence_before();
     }
