@@ -120,25 +120,34 @@ __device__ __forceinline__ RaggedBlock far_block(const Ragged& r, int number, in
     return RaggedBlock{number >= start ? lo : -1, number - start};
 }
 
-// delta = rowsum(dO * O): 16 lanes per row, 8 values each.
+// delta = rowsum(dO * O): 16 lanes take four consecutive tokens of a head, 8 values of each row at a time, all eight loads on their
+// way together. (Bound by memory, 2 * headDim * 2 bytes per row and head.)
+constexpr int kDeltaRows = 4;
 template <typename T>
 __global__ void __launch_bounds__(256) delta_kernel(AttentionArgs a, float* __restrict__ delta) {
     grid_release();
     const int64_t g = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> 4;
-    const int part = threadIdx.x & 15;
-    float sum = 0.0f;
-    const bool live = g < (int64_t)a.total_q * a.q_heads;
-    const int64_t t = live ? g / a.q_heads : 0, h = live ? g % a.q_heads : 0;
-    if (live && 8 * part < a.dim) {
-        const uint4 x = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.o.p) + t * a.o.token + h * a.o.head + 8 * part);
-        const uint4 y = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.d_o.p) + t * a.d_o.token + h * a.d_o.head + 8 * part);
-        const T *xv = reinterpret_cast<const T*>(&x), *yv = reinterpret_cast<const T*>(&y);
+    const int part = threadIdx.x & 15, h = (int)(g % a.q_heads);
+    const int64_t t0 = g / a.q_heads * kDeltaRows;
+    uint4 x[kDeltaRows], y[kDeltaRows];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum = fmaf(to_float(xv[i]), to_float(yv[i]), sum);
+    for (int i = 0; i < kDeltaRows; ++i) {
+        x[i] = y[i] = make_uint4(0, 0, 0, 0);
+        if (t0 + i < a.total_q && 8 * part < a.dim) {
+            x[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.o.p) + (t0 + i) * a.o.token + h * a.o.head + 8 * part);
+            y[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.d_o.p) + (t0 + i) * a.d_o.token + h * a.d_o.head + 8 * part);
+        }
     }
 #pragma unroll
-    for (int d = 8; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    if (live && part == 0) delta[h * a.total_q + t] = sum;
+    for (int i = 0; i < kDeltaRows; ++i) {
+        const T *xv = reinterpret_cast<const T*>(&x[i]), *yv = reinterpret_cast<const T*>(&y[i]);
+        float sum = 0.0f;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) sum = fmaf(to_float(xv[c]), to_float(yv[c]), sum);
+#pragma unroll
+        for (int d = 8; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        if (part == 0 && t0 + i < a.total_q) delta[(int64_t)h * a.total_q + t0 + i] = sum;
+    }
 }
 
 // Four values of the tile's columns: from shared memory (keys kernel), or the row's own.
@@ -839,7 +848,8 @@ cudaError_t launch(cudaStream_t s, const AttentionArgs& a, void* buffer) {
     p.chunk = far_chunk(a), p.far_tiles = far_tiles(a), p.far_slots = p.far_tiles > 0 ? far_slots(a) : 0;
     p.partial = reinterpret_cast<float*>(b + align256(size_t(a.q_heads) * a.total_q * 4));
     p.limit = window_wait_limit(a), p.fault = a.wait.fault_word;
-    delta_kernel<T><<<(unsigned)(((int64_t)a.total_q * a.q_heads + 15) / 16), 256, 0, s>>>(a, delta);
+    const int64_t delta_groups = ((int64_t)a.total_q + kDeltaRows - 1) / kDeltaRows * a.q_heads;
+    delta_kernel<T><<<(unsigned)((delta_groups + 15) / 16), 256, 0, s>>>(a, delta);
     cudaError_t e = cudaGetLastError();
     static SharedMemoryOnce once_keys, once_queries;
     if (e == cudaSuccess) e = once_keys.allow(reinterpret_cast<const void*>(window_backward_kernel<T, DP, true>), S::kTotal);
