@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(256)
 template <typename T, int V>
 struct Rows {
     static constexpr int kBytes = sizeof(Pack<T, V>);      // 16 or 32, per thread and row
-    static constexpr int kAhead = kBytes == 16 ? 16 : 8, kGroup = 4;
+    static constexpr int kAhead = 8, kGroup = 4;
     static constexpr int kShared = kAhead * kBytes * 256;  // of a block
     uint32_t ring;
     const T* from;
@@ -290,7 +290,13 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
             for (int x = 0; x < Rows<Y, V>::kGroup; ++x) {
                 const unsigned key = __shfl_sync(0xffffffffu, token.x, (j + x) & 31), t = __shfl_sync(0xffffffffu, token.y, (j + x) & 31);
-                if (j + x < n && key < (unsigned)a.rows) rows.fetch(j + x, x, t);
+                const unsigned last = __shfl_sync(0xffffffffu, token.x, (j + x - 1) & 31);
+                if (j + x < n && key < (unsigned)a.rows) {
+                    rows.fetch(j + x, x, t);
+                    // (a row of the table that will be read when its sum is done)
+                    if (V > 1 && beta != 0.0f && (j + x == 0 || key != last) && first + lane * V < a.width)
+                        asm volatile("prefetch.global.L2 [%0];" ::"l"(table + (int64_t)key * a.ld_e + first + lane * V));
+                }
             }
             rows.commit();
         };
