@@ -4,13 +4,14 @@
 // Lookup: one pass; a warp moves a piece of one row with 16-byte loads and stores. Bound by memory (count * width read,
 // unless rows repeat, and written).
 //
-// Gradient, four launches, each prepared while the one before it runs (programmatic dependent launch):
+// Gradient, up to four launches, each prepared while the one before it runs (programmatic dependent launch):
 //   1. S^T in CSR form is the tokens sorted by id: a stable radix sort of (id, position) pairs. Up to 131072 tokens one cluster
-//      of 8 thread blocks sorts them in two passes or three (ids below 2^18: two 9-bit digits), its digit counts exchanged over
-//      distributed shared memory, its barriers the cluster's; more tokens take the multi-launch sort of transpose.cu.
+//      of 16 thread blocks sorts them in two passes or three (ids below 2^18: two 9-bit digits), its digit counts exchanged over
+//      distributed shared memory, its barriers the cluster's; up to 2048 one block does, as one more block of the next launch. More
+//      tokens, or a device that holds no such cluster, take the multi-launch sort of transpose.cu.
 //   2. Beside the sort, the rows no token names are written (beta = 0: zeros, most of the traffic of a large table). A block
 //      finds those of its rows by marking the ids that are its own in shared memory, so it need not wait for the sort. (As
-//      further blocks of the sort's own launch they came up in clusters of 8, 16 of which the GPU holds: 116 us against 65.)
+//      further blocks of the sort's own launch they came up in clusters, few of which the GPU holds at a time: 116 us against 65.)
 //   3. The sorted tokens are cut into chunks of equal size whatever the ids are, so a token that fills half the batch costs no
 //      more than any other; a warp owns one chunk and a slab of columns, adds in fp32 and writes every sum that lies inside
 //      its chunk. A sum that crosses chunks is left as one partial per chunk.
@@ -18,6 +19,8 @@
 // No atomics: the order of every addition follows from ids and sizes. Bound by memory: count * width read, rows * width written.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <atomic>
 
 #include "internal.h"
 #include "launch.h"
@@ -385,10 +388,11 @@ __global__ void __launch_bounds__(kJoinThreads)
 
 // ----------------------------------------------------------------------------- sort, and the rows without a token
 
-constexpr int kSortCluster = 8;
+constexpr int kSortCluster = 16;  // (8, the most that every device must hold, took 36 us against 24 for 65536 tokens)
 constexpr int kSortThreads = 1024;
-constexpr int kSortRounds = 16;  // items per thread, at most
-constexpr int kFewRounds = 2;    // the same, of the kernel for few tokens (registers and predicated code for 16 cost it 3 us)
+constexpr int kSortRounds = 8;  // items per thread, at most
+constexpr int kFewRounds = 2;   // the same, of the kernel for few tokens (registers and predicated code for more cost it)
+constexpr int64_t kSortAlone = kSortThreads * kFewRounds;  // tokens that one block sorts
 constexpr int64_t kSortMost = (int64_t)kSortCluster * kSortThreads * kSortRounds;
 constexpr int kMostDigits = 512;
 
@@ -680,8 +684,7 @@ int gradient_chunk(int64_t count, int64_t width) {
 }
 
 struct GradientLayout {
-    bool one_cluster;
-    TransposePlan sort;  // more tokens than one cluster sorts
+    TransposePlan sort;  // for tokens that one cluster does not sort
     int chunk;
     int64_t chunks;
     size_t off_raw, off_sorted[2], off_partial, bytes;
@@ -689,17 +692,16 @@ struct GradientLayout {
 
 GradientLayout gradient_layout(int64_t count, int64_t rows, int64_t width) {
     GradientLayout l = {};
-    l.one_cluster = count <= kSortMost;
     l.chunk = gradient_chunk(count, width);
     l.chunks = (count + l.chunk - 1) / l.chunk;
     size_t off = 0;
-    if (!l.one_cluster) {
+    if (count > kSortAlone) {  // (room for it whatever the device holds: the size is asked for without one)
         l.sort = transpose_plan(rows, rows + 1, count, 0);
         off = l.sort.bytes;
         l.off_raw = off;
         off += align256(size_t(count) * 4);
     }
-    for (int i = 0; i < (l.one_cluster ? 2 : 1); ++i) {
+    for (int i = 0; i < (count <= kSortMost ? 2 : 1); ++i) {
         l.off_sorted[i] = off;
         off += align256(size_t(count) * 8);
     }
@@ -719,6 +721,38 @@ __global__ void __launch_bounds__(256)
     if (t < count) sorted[t] = make_uint2((unsigned)keys[t], perm[t]);
 }
 
+cudaLaunchConfig_t cluster_config(cudaStream_t s, unsigned blocks, cudaLaunchAttribute& attr) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(blocks);
+    cfg.blockDim = dim3(kSortThreads);
+    cfg.stream = s;
+    attr = {};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = blocks, attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cfg;
+}
+
+// Whether the current device holds a cluster of kSortCluster blocks (a part of a partitioned one may not). Asked once per device.
+bool sort_cluster_fits() {
+    static std::atomic<int> known[64];  // 0: not asked, 1: no, 2: yes
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess) return false;
+    if (device < 64 && known[device].load(std::memory_order_relaxed) != 0) return known[device].load(std::memory_order_relaxed) == 2;
+    cudaLaunchAttribute attr;
+    const cudaLaunchConfig_t cfg = cluster_config(nullptr, kSortCluster, attr);
+    const auto allow = [&](auto kernel) {
+        int clusters = 0;
+        return cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+               cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) == cudaSuccess && clusters > 0;
+    };
+    const bool fits = allow(embedding_sort_kernel<kFewRounds>) && allow(embedding_sort_kernel<kSortRounds>);
+    if (!fits) cudaGetLastError();
+    if (device < 64) known[device].store(fits ? 2 : 1, std::memory_order_relaxed);
+    return fits;
+}
+
 template <typename Y, typename E, int V>
 cudaError_t launch_gradient(cudaStream_t s, const EmbeddingArgs& a, char* b) {
     const GradientLayout l = gradient_layout(a.count, a.rows, a.width);
@@ -734,24 +768,17 @@ cudaError_t launch_gradient(cudaStream_t s, const EmbeddingArgs& a, char* b) {
     const bool fill = a.beta.dev != nullptr || a.beta.host != 1.0f;
     int last = (so.passes - 1) & 1;
     // few tokens: one block sorts them in two rounds, as a further block of the other launch where there is one
-    so.sorters = a.count == 0 || !l.one_cluster ? 0 : a.count > kFewRounds * kSortThreads ? kSortCluster : 1;
+    so.sorters = a.count == 0 ? 0 : a.count <= kSortAlone ? 1 : a.count <= kSortMost && sort_cluster_fits() ? kSortCluster : 0;
     const bool together = fill && so.sorters == 1;
     if (so.sorters > 0 && !together) {
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3((unsigned)so.sorters);
-        cfg.blockDim = dim3(kSortThreads);
-        cfg.stream = s;
-        cudaLaunchAttribute attr = {};
-        attr.id = cudaLaunchAttributeClusterDimension;
-        attr.val.clusterDim.x = (unsigned)so.sorters, attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-        cfg.attrs = &attr;
-        cfg.numAttrs = 1;
+        cudaLaunchAttribute attr;
+        const cudaLaunchConfig_t cfg = cluster_config(s, (unsigned)so.sorters, attr);
         const bool few = a.count <= (int64_t)so.sorters * kSortThreads * kFewRounds;
         const cudaError_t e = few ? cudaLaunchKernelEx(&cfg, embedding_sort_kernel<kFewRounds>, static_cast<const SortArgs>(so))
                                   : cudaLaunchKernelEx(&cfg, embedding_sort_kernel<kSortRounds>, static_cast<const SortArgs>(so));
         if (e != cudaSuccess) return e;
     }
-    if (!l.one_cluster) {
+    if (a.count > 0 && so.sorters == 0) {
         int* raw = reinterpret_cast<int*>(b + l.off_raw);
         embedding_keys_kernel<<<(unsigned)((a.count + 255) / 256), 256, 0, s>>>(so, raw);
         const cudaError_t e = sort_keys(s, a.rows, a.count, raw, l.sort, b);
