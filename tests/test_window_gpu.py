@@ -263,6 +263,22 @@ def test_many_first_tokens_of_a_long_sequence(handle, device, sinks):
     check(handle, q, k, v, lengths, lengths, 100, sinks, dout=g)
 
 
+@pytest.mark.parametrize("dtype,heads", [(torch.bfloat16, (16, 4, 128)), (torch.float16, (18, 6, 64)), (torch.bfloat16, (12, 12, 40))], ids=str)
+def test_more_work_than_blocks_run_at_once(handle, device, dtype, heads):
+    """Every thread block takes over others' places: long work next to short, sequences without queries or keys, queries that see
+    nothing, in changing order; the order in which blocks take over is no part of the result."""
+    hq, hk, d = heads
+    lengths = [(0, 7), (1, 1), (300, 300), (0, 0), (65, 20), (40, 0), (1400, 1400), (257, 400), (5, 0), (128, 128), (1, 900), (640, 64)]
+    lengths = lengths * 2 + lengths[::-1] * 2
+    lq, lk = [a for a, _ in lengths], [b for _, b in lengths]
+    gen = torch.Generator(device=device).manual_seed(53)
+    q, k, v, g = (normal((n, h, d), dtype, device, gen) for n, h in ((sum(lq), hq), (sum(lk), hk), (sum(lk), hk), (sum(lq), hq)))
+    first = check(handle, q, k, v, lq, lk, 200, 3, dout=g)
+    again = check(handle, q, k, v, lq, lk, 200, 3, dout=g)
+    for a, b in zip(first[:2] + tuple(first[2].values()), again[:2] + tuple(again[2].values())):
+        assert torch.equal(a, b)
+
+
 def test_offsets_past_32_bits(handle, device):
     """2.4e9 values per tensor of queries: the last sequence lies behind 2^31 of them."""
     gen = torch.Generator(device=device).manual_seed(54)
