@@ -4,7 +4,7 @@
 // Lookup: one pass; a warp moves a piece of one row with 16-byte loads and stores. Bound by memory (count * width read,
 // unless rows repeat, and written).
 //
-// Gradient, up to four launches, each prepared while the one before it runs (programmatic dependent launch):
+// Gradient, two or three launches, each prepared while the one before it runs (programmatic dependent launch):
 //   1. S^T in CSR form is the tokens sorted by id: a stable radix sort of (id, position) pairs. Up to 131072 tokens one cluster
 //      of 16 thread blocks sorts them in two passes or three (ids below 2^18: two 9-bit digits), its digit counts exchanged over
 //      distributed shared memory, its barriers the cluster's; up to 2048 one block does, as one more block of the next launch. More
@@ -14,9 +14,9 @@
 //      further blocks of the sort's own launch they came up in clusters, few of which the GPU holds at a time: 116 us against 65.)
 //   3. The sorted tokens are cut into chunks of equal size whatever the ids are, so a token that fills half the batch costs no
 //      more than any other; a warp owns one chunk and a slab of columns, adds in fp32 and writes every sum that lies inside
-//      its chunk. A sum that crosses chunks is left as one partial per chunk.
-//   4. Those partials are put together in chunk order.
-// No atomics: the order of every addition follows from ids and sizes. Bound by memory: count * width read, rows * width written.
+//      its chunk. A sum that crosses chunks is left as one partial per chunk; the warp that finds all of a sum's partials there
+//      (a counter per sum) adds them, in chunk order.
+// The order of every addition follows from ids and sizes alone. Bound by memory: count * width read, rows * width written.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(256)
 // ----------------------------------------------------------------------------- gradient
 
 // The rows of a warp's chunk on their way. Vectors: a ring of asynchronous copies in shared memory, a thread reads back what it
-// copied itself; the copies of 16 (8) rows are in flight whatever the warp is doing. (Loads into registers, as many ahead,
+// copied itself; the copies of 8 rows are in flight whatever the warp is doing. (Loads into registers, as many ahead,
 // waited for the newest of them at every row: 52 us against 25 for 16384 rows of 2048 bf16 values.)
 template <typename T, int V>
 struct Rows {
@@ -238,6 +238,7 @@ struct GradientArgs {
     int chunk, slabs;
     const uint2* sorted;  // (row, token) by row, then token; row = rows: none
     float* partial;       // [chunk][2][width]: a sum that came in open, a sum that goes out open
+    unsigned* arrived;    // [chunk][slab]: partials that are there of the sum that goes out of a chunk; zero before the launch
 };
 
 // dE[r, slab] = beta * dE[r, slab] + alpha * sum
@@ -260,22 +261,74 @@ __device__ __forceinline__ void finish_row(E* table, const GradientArgs& a, int6
     store_columns<E, V>(row, first, a.width, lane, out);
 }
 
+// Called by the warp that has written chunk c's partial of a sum over several chunks. The one that comes last of them puts the
+// partials together, in chunk order whoever it is.
+template <typename E, int V>
+__device__ __forceinline__ void join_partials(E* table, const GradientArgs& a, int64_t c, bool came_in, int slab, int row, int64_t first, int lane,
+                                              float alpha, float beta) {
+    constexpr int kPer = Columns<V>::kPer, kDepth = 4;
+    const auto starts_with = [&](int64_t d) { return d >= 0 && d < a.chunks && (int)__ldcg(&a.sorted[d * a.chunk].x) == row; };
+    // the run of chunks around c that start with the row (32 of them are looked at in one step)
+    int64_t begin = c, last = c;
+    if (came_in)
+        for (int n = 32; n == 32; begin -= n) n = __popc(__ballot_sync(0xffffffffu, starts_with(begin - 1 - lane)));
+    for (int n = 32; n == 32; last += n) n = __popc(__ballot_sync(0xffffffffu, starts_with(last + 1 + lane)));
+    // the sum began in the chunk before the first of them, unless it began right with it
+    if (came_in && begin > 0 && (int)__ldcg(&a.sorted[begin * a.chunk - 1].x) == row) --begin;
+    __threadfence();
+    __syncwarp();
+    unsigned before = 0;
+    if (lane == 0) before = atomicAdd(a.arrived + begin * a.slabs + slab, 1u);
+    before = __shfl_sync(0xffffffffu, before, 0);
+    if (before != (unsigned)(last - begin)) return;
+    __threadfence();
+    const auto load = [&](int64_t d, float* v) {
+        const float* from = a.partial + (2 * d + (d == begin)) * a.width + first;
+#pragma unroll
+        for (int i = 0; i < kPer; i += V > 1 ? 4 : 1) {
+            const int64_t x = Columns<V>::at(lane, i);
+            if (V > 1) {
+                const float4 f = first + x < a.width ? __ldcg(reinterpret_cast<const float4*>(from + x)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                v[i] = f.x, v[(i + 1) % kPer] = f.y, v[(i + 2) % kPer] = f.z, v[(i + 3) % kPer] = f.w;
+            } else {
+                v[i] = first + x < a.width ? __ldcg(from + x) : 0.0f;
+            }
+        }
+    };
+    float sum[kPer];
+    load(begin, sum);
+    for (int64_t d = begin + 1; d <= last; d += kDepth) {
+        float v[kDepth][kPer];
+#pragma unroll
+        for (int j = 0; j < kDepth; ++j) {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) v[j][i] = 0.0f;
+            if (d + j <= last) load(d + j, v[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < kDepth; ++j)
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) sum[i] += v[j][i];
+    }
+    finish_row<E, V>(table, a, row, first, lane, alpha, beta, sum);
+}
+
 // One warp per (chunk of sorted tokens, slab of columns).
 template <typename Y, typename E, int V>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 4)  // (64 registers: 389 us against 401 with 76, two passes of 65536 tokens)
     embedding_sum_kernel(GradientArgs a, const Y* __restrict__ dy, E* __restrict__ table, ScalarArg<float> alpha_arg,
                          ScalarArg<float> beta_arg) {
     constexpr int kPer = Columns<V>::kPer, kSlab = Columns<V>::kSlab;
     const int64_t warp = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> 5;
     const int lane = threadIdx.x & 31;
     const float alpha = alpha_arg.get(), beta = beta_arg.get();
-    grid_release();
     if (warp >= a.chunks * a.slabs) {
         grid_wait();
         return;
     }
     const int64_t c = warp / a.slabs;
-    const int64_t first = (warp - c * a.slabs) * kSlab;
+    const int slab = (int)(warp - c * a.slabs);
+    const int64_t first = (int64_t)slab * kSlab;
     const int64_t k0 = c * a.chunk, k1 = min(k0 + a.chunk, a.count);
     grid_wait();  // the sort
     float sum[kPer];
@@ -283,6 +336,7 @@ __global__ void __launch_bounds__(256)
     for (int i = 0; i < kPer; ++i) sum[i] = 0.0f;
     int row = (int)__ldcg(&a.sorted[k0].x);
     bool open = k0 > 0 && (int)__ldcg(&a.sorted[k0 - 1].x) == row;  // the first sum began in an earlier chunk
+    int came_in = -1;                                               // its row, once its partial is written
     extern __shared__ __align__(16) uint8_t smem_raw[];
     Rows<Y, V> rows(smem_raw, dy, a.ld_y, first, a.width, lane);
     for (int64_t k = k0; k < k1; k += 32) {
@@ -312,10 +366,12 @@ __global__ void __launch_bounds__(256)
                 const int key = (int)__shfl_sync(0xffffffffu, token.x, (j0 + x) & 31);
                 if (j0 + x < n) {
                     if (key != row) {
-                        if (open)
+                        if (open) {
                             store_columns<float, V>(a.partial + (2 * c) * a.width, first, a.width, lane, sum);
-                        else
+                            came_in = row;
+                        } else {
                             finish_row<E, V>(table, a, row, first, lane, alpha, beta, sum);
+                        }
                         open = false;
                         row = key;
 #pragma unroll
@@ -328,61 +384,22 @@ __global__ void __launch_bounds__(256)
         }
         rows.drain();
     }
-    if (row >= a.rows) return;
-    const bool goes_on = k1 < a.count && (int)__ldcg(&a.sorted[k1].x) == row;
-    if (open)
-        store_columns<float, V>(a.partial + (2 * c) * a.width, first, a.width, lane, sum);
-    else if (goes_on)
-        store_columns<float, V>(a.partial + (2 * c + 1) * a.width, first, a.width, lane, sum);
-    else
-        finish_row<E, V>(table, a, row, first, lane, alpha, beta, sum);
-}
-
-// One block per chunk: if a sum starts in this chunk and goes on, its partials are added in chunk order; a warp takes a slab of
-// columns at a time, eight partials on their way. (Few partials each, mostly: small blocks, of which many run at once.)
-constexpr int kJoinThreads = 256;
-
-template <typename E, int V>
-__global__ void __launch_bounds__(kJoinThreads)
-    embedding_join_kernel(GradientArgs a, E* __restrict__ table, ScalarArg<float> alpha_arg, ScalarArg<float> beta_arg) {
-    constexpr int kPer = Columns<V>::kPer, kSlab = Columns<V>::kSlab, kDepth = 8;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t c = blockIdx.x;
-    const int64_t k0 = c * a.chunk, k1 = k0 + a.chunk;
-    grid_wait();  // the sums
-    if (c + 1 >= a.chunks) return;
-    const unsigned row = __ldcg(&a.sorted[k1 - 1].x);
-    if (row >= (unsigned)a.rows || __ldcg(&a.sorted[k1].x) != row) return;  // nothing goes on
-    if (k0 > 0 && __ldcg(&a.sorted[k0 - 1].x) == row) return;               // it started earlier
-    // its last chunk: the rows at the chunks' starts ascend, 32 of them are looked at in one step
-    int64_t last = c + 1, beyond = a.chunks;
-    while (beyond - last > 1) {
-        const int64_t step = (beyond - last + 31) / 32, d = last + step * lane;
-        const unsigned same = __ballot_sync(0xffffffffu, d < beyond && __ldcg(&a.sorted[d * a.chunk].x) == row);
-        last += step * (31 - __clz(same));
-        beyond = min(last + step, beyond);
-    }
-    const float alpha = alpha_arg.get(), beta = beta_arg.get();
-    for (int slab = warp; slab < a.slabs; slab += kJoinThreads / 32) {
-        const int64_t first = (int64_t)slab * kSlab;
-        float sum[kPer];
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) sum[i] = 0.0f;
-        load_columns<float, V>(a.partial + (2 * c + 1) * a.width, first, a.width, lane, sum);
-        for (int64_t d = c + 1; d <= last; d += kDepth) {
-            float v[kDepth][kPer];
-#pragma unroll
-            for (int j = 0; j < kDepth; ++j) {
-#pragma unroll
-                for (int i = 0; i < kPer; ++i) v[j][i] = 0.0f;
-                if (d + j <= last) load_columns<float, V>(a.partial + (2 * (d + j)) * a.width, first, a.width, lane, v[j]);
-            }
-#pragma unroll
-            for (int j = 0; j < kDepth; ++j)
-#pragma unroll
-                for (int i = 0; i < kPer; ++i) sum[i] += v[j][i];
+    bool goes_on = false;
+    if (row < a.rows) {
+        goes_on = k1 < a.count && (int)__ldcg(&a.sorted[k1].x) == row;
+        if (open) {
+            store_columns<float, V>(a.partial + (2 * c) * a.width, first, a.width, lane, sum);
+            came_in = row;
+            goes_on = false;  // (the same sum)
+        } else if (goes_on) {
+            store_columns<float, V>(a.partial + (2 * c + 1) * a.width, first, a.width, lane, sum);
+        } else {
+            finish_row<E, V>(table, a, row, first, lane, alpha, beta, sum);
         }
-        finish_row<E, V>(table, a, row, first, lane, alpha, beta, sum);
+    }
+    for (int part = 0; part < 2; ++part) {
+        if (part == 0 ? came_in < 0 : !goes_on) continue;
+        join_partials<E, V>(table, a, c, part == 0, slab, part == 0 ? came_in : row, first, lane, alpha, beta);
     }
 }
 
@@ -404,6 +421,8 @@ struct SortArgs {
     uint2* sorted[2];   // (key, token); the passes write them in turn
     int passes, bits;   // digits of `bits` bits, at most 9
     int sorters;        // thread blocks that sort (one cluster)
+    unsigned* arrived;  // set to zero on the way, `counters` of them
+    int64_t counters;
     // rows without a token
     void* table;
     int64_t ld, width;
@@ -458,6 +477,7 @@ __device__ __forceinline__ void sort_block(const SortArgs& a, SortShared& s, int
     const int rounds = (int)((a.count + (int64_t)a.sorters * kSortThreads - 1) / ((int64_t)a.sorters * kSortThreads));
     const int64_t begin = ((int64_t)rank * 32 + warp) * rounds * 32 + lane;
     const int digits = 1 << a.bits;
+    for (int64_t i = rank * kSortThreads + (int)threadIdx.x; i < a.counters; i += (int64_t)a.sorters * kSortThreads) a.arrived[i] = 0u;
     for (int pass = 0; pass < a.passes; ++pass) {
         const int shift = pass * a.bits, to = pass & 1;
         const uint2* in = to ? a.sorted[0] : a.sorted[1];
@@ -687,7 +707,7 @@ struct GradientLayout {
     TransposePlan sort;  // for tokens that one cluster does not sort
     int chunk;
     int64_t chunks;
-    size_t off_raw, off_sorted[2], off_partial, bytes;
+    size_t off_raw, off_sorted[2], off_partial, off_arrived, bytes;
 };
 
 GradientLayout gradient_layout(int64_t count, int64_t rows, int64_t width) {
@@ -707,6 +727,8 @@ GradientLayout gradient_layout(int64_t count, int64_t rows, int64_t width) {
     }
     l.off_partial = off;
     off += align256(size_t(l.chunks) * 2 * size_t(width) * 4);
+    l.off_arrived = off;
+    off += align256(size_t(l.chunks) * ((width + 127) / 128) * 4);  // (a slab is 128 columns at least)
     l.bytes = off + 256;
     return l;
 }
@@ -714,6 +736,7 @@ GradientLayout gradient_layout(int64_t count, int64_t rows, int64_t width) {
 __global__ void __launch_bounds__(256) embedding_keys_kernel(const SortArgs a, int* __restrict__ keys) {
     const int64_t t = blockIdx.x * (int64_t)blockDim.x + threadIdx.x;
     if (t < a.count) keys[t] = key_of(a, t);
+    for (int64_t i = t; i < a.counters; i += (int64_t)gridDim.x * blockDim.x) a.arrived[i] = 0u;
 }
 __global__ void __launch_bounds__(256)
     embedding_pairs_kernel(int64_t count, const int* __restrict__ keys, const unsigned* __restrict__ perm, uint2* __restrict__ sorted) {
@@ -761,6 +784,8 @@ cudaError_t launch_gradient(cudaStream_t s, const EmbeddingArgs& a, char* b) {
     so.count = a.count, so.rows = a.rows, so.ids = a.ids, so.wide = a.wide_ids, so.base = a.base;
     so.table = a.table, so.ld = a.ld_table, so.width = a.width;
     for (int i = 0; i < 2; ++i) so.sorted[i] = reinterpret_cast<uint2*>(b + l.off_sorted[i]);
+    const int slabs = (int)((a.width + Columns<V>::kSlab - 1) / Columns<V>::kSlab);
+    so.arrived = reinterpret_cast<unsigned*>(b + l.off_arrived), so.counters = l.chunks * slabs;
     int need = 1;  // bits of a key, `rows` included
     while (need < 31 && (int64_t(1) << need) <= a.rows) ++need;
     so.passes = (need + 8) / 9;
@@ -802,7 +827,7 @@ cudaError_t launch_gradient(cudaStream_t s, const EmbeddingArgs& a, char* b) {
     g.chunk = l.chunk, g.chunks = l.chunks;
     g.sorted = so.sorted[last];
     g.partial = reinterpret_cast<float*>(b + l.off_partial);
-    g.slabs = (int)((a.width + Columns<V>::kSlab - 1) / Columns<V>::kSlab);
+    g.slabs = slabs, g.arrived = so.arrived;
     const unsigned blocks = warp_blocks(g.chunks * g.slabs);
     if (blocks == 0) return cudaErrorInvalidValue;
     constexpr int kShared = Rows<Y, V>::kShared;
@@ -810,8 +835,6 @@ cudaError_t launch_gradient(cudaStream_t s, const EmbeddingArgs& a, char* b) {
     static SharedMemoryOnce once;
     if (kShared > 48 * 1024) e = once.allow(reinterpret_cast<const void*>(embedding_sum_kernel<Y, E, V>), kShared);
     if (e == cudaSuccess) e = launch_behind(s, true, embedding_sum_kernel<Y, E, V>, blocks, 256, kShared, g, static_cast<const Y*>(a.tokens), static_cast<E*>(a.table), a.alpha, a.beta);
-    if (e == cudaSuccess && g.chunks > 1)
-        e = launch_behind(s, true, embedding_join_kernel<E, V>, (unsigned)(g.chunks - 1), kJoinThreads, 0, g, static_cast<E*>(a.table), a.alpha, a.beta);
     return e;
 }
 
