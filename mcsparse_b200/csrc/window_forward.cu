@@ -3,14 +3,15 @@
 // One piece of work is 256 consecutive queries of a sequence and one query head: two tiles of 128 rows that share every
 // key tile of 64. A thread block (one per SM) takes over the place of another block of the grid when its loads are out, so that the
 // loads and first scores of the next work run beside the end of this one (blocks of one work each: 174 us against 159 for 16384
-// tokens in 5 sequences, 16/2 heads of 128, window 1024; 1981 against 1874 for 32768 tokens, 32/8 heads, window 4096). S = Q K^T and O += P V are tcgen05.mma with S, P and O in tensor memory (P overwrites its S, half as
-// wide); 128 threads per row tile, one row each, take maximum, exponentials and sum in registers. S has two buffers per row
-// tile: the next scores are there when a tile's weights are done, so the chain scores -> weights -> O -> next scores of a
-// single buffer (3300 clocks per 128 keys of both row tiles) is cut. Key tiles outside window and first tokens are never
-// loaded; a tile needs its mask only at an edge of the pattern.
+// tokens in 5 sequences, 16/2 heads of 128, window 1024; 1981 against 1874 for 32768 tokens, 32/8 heads, window 4096). S = Q K^T and
+// O += P V are tcgen05.mma with S, P and O in tensor memory (P overwrites its S, half as wide); 128 threads per row tile, one row
+// each, take maximum, exponentials and sum in registers. S has two buffers per row tile: the next scores are there when a tile's
+// weights are done, so the chain scores -> weights -> O -> next scores of a single buffer is cut. Key tiles outside window and
+// first tokens are never loaded; a tile needs its mask only at an edge of the pattern.
 //
-// Bounds at headDim 128, clocks per 128 keys and both row tiles: products 2560 (Q K^T with 64 keys reads 6 KB of shared memory
-// per 32 clocks of arithmetic and takes 48; P V reads P from tensor memory: 64), exponentials 2048 (16 per clock).
+// Bounds at headDim 128, clocks per 64 keys and both row tiles: products 1280 (Q K^T with 64 keys reads 6 KB of shared memory
+// per 32 clocks of arithmetic and takes 48; P V reads P from tensor memory: 64), exponentials 1024 (16 per clock). Measured on
+// 32768 tokens: 1680, at the 1585 MHz that the power limit leaves. Weights handed over by halves of a tile: no faster.
 #include <type_traits>
 
 #include "tensor_core.h"
