@@ -135,6 +135,22 @@ def test_gradient_long_batches(handle, device, count):
     assert torch.equal(table, again), "equal inputs, equal bits"
 
 
+@pytest.mark.parametrize("width", [24, 33, 264])
+@pytest.mark.parametrize("run", [1, 7, 8, 9, 16, 63, 64, 65, 512, 2048, 2049, 6000, 30000])
+def test_gradient_of_runs_of_one_length(handle, device, run, width):
+    """Every id occurs `run` times, so that sums begin and end on, before and behind the places where the work is cut."""
+    gen = torch.Generator(device=device).manual_seed(run)
+    rows = max(30000 // run, 1)
+    ids = torch.arange(rows, device=device).repeat_interleave(run)
+    ids = ids[torch.randperm(len(ids), generator=gen, device=device)] if run % 2 else ids
+    dy = torch.empty(len(ids), width, dtype=torch.bfloat16, device=device).normal_(generator=gen)
+    for beta in (0.0, 1.0):
+        table = torch.empty(rows + 3, width, device=device).normal_(generator=gen)
+        want = ref.gradient(ids, dy, rows + 3, 1.0, beta, table)
+        run_gradient(handle, ids, dy, table, beta=beta)
+        ref.close(table, want, f"beta {beta}")
+
+
 def test_gradient_strides_and_untouched_rows(handle, device):
     gen = torch.Generator(device=device).manual_seed(3)
     for pad, offset in ((8, 8), (3, 1)):
