@@ -19,17 +19,16 @@ namespace tc {
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 
-// True in one lane of a converged warp, always the same one. (With `lane == 0` in its place the compiler cannot tell that one
-// lane alone issues: every tcgen05.mma then sat in a loop over lanes, 95 to 210 clocks each against 64 of work.)
+// True in one lane of a converged warp, always the same one. (With `lane == 0` in its place a tcgen05.mma of 64 clocks of work
+// took 95 to 210 clocks in a row of them.)
 __device__ __forceinline__ bool elect() {
     uint32_t one = 0;
     asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n @p mov.u32 %0, 1;\n}" : "+r"(one));
     return one != 0;
 }
 
-// A value that is the same in all lanes of a converged warp, in a form that lets the compiler know it: tcgen05.mma takes its
-// operands from uniform registers, and values it cannot prove uniform (loaded ones, and counters of loops whose ends depend on
-// them) were moved there anew for every instruction, 75 to 100 clocks each.
+// A value that is the same in all lanes of a converged warp, taken over the warp. Loaded values, and loop bounds that depend on
+// them, pass through it before they reach the operands of a tcgen05.mma: without it each such instruction took 75 to 100 clocks more.
 __device__ __forceinline__ int uniform(int x) { return __reduce_max_sync(0xffffffffu, x); }
 __device__ __forceinline__ uint32_t uniform(uint32_t x) { return __reduce_max_sync(0xffffffffu, x); }
 
