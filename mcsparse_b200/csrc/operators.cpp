@@ -49,8 +49,12 @@ St embedding_check(mcsparseHandle_t h, int64_t count, mcsparseIndexType_t indexT
     return OK;
 }
 
-St embedding_indices(const void* indices, int64_t count, mcsparseIndexType_t type, mcsparseIndexBase_t base) {
-    if (indices == nullptr && count > 0) return BAD_POINTER;
+// A descriptor's values may have been taken away (mcsparseDnMatSetValues) after it was made.
+bool absent(const mcsparseDnMatDescr* m) { return m->values == nullptr && m->row_num > 0 && m->col_num > 0; }
+
+St embedding_arrays(const void* indices, int64_t count, mcsparseIndexType_t type, mcsparseIndexBase_t base, const mcsparseDnMatDescr* table,
+                    const mcsparseDnMatDescr* tokens) {
+    if ((indices == nullptr && count > 0) || absent(table) || absent(tokens)) return BAD_POINTER;
     if (base != MCSPARSE_INDEX_BASE_ZERO && base != MCSPARSE_INDEX_BASE_ONE) return BAD_VALUE;
     return misaligned(indices, type == MCSPARSE_INDEX_64I ? 8 : 4) ? BAD_VALUE : OK;
 }
@@ -159,7 +163,7 @@ mcsparseStatus_t mcsparseB200EmbeddingLookup(mcsparseHandle_t handle, const void
     St st = embedding_check(handle, count, indexType, matE, matY);
     if (st != OK) return pub(st);
     if (alpha == nullptr) return pub(BAD_POINTER);
-    if ((st = embedding_indices(indices, count, indexType, idxBase)) != OK) return pub(st);
+    if ((st = embedding_arrays(indices, count, indexType, idxBase, matE, matY)) != OK) return pub(st);
     DeviceGuard guard(handle->device);
     EmbeddingArgs a = embedding_args(count, indices, indexType, idxBase, matE, matY);
     a.alpha = scalar(handle, alpha);
@@ -183,7 +187,7 @@ mcsparseStatus_t mcsparseB200EmbeddingGradient(mcsparseHandle_t handle, const vo
     St st = embedding_check(handle, count, indexType, matDE, matDY);
     if (st != OK) return pub(st);
     if (alpha == nullptr || beta == nullptr || externalBuffer == nullptr) return pub(BAD_POINTER);
-    if ((st = embedding_indices(indices, count, indexType, idxBase)) != OK) return pub(st);
+    if ((st = embedding_arrays(indices, count, indexType, idxBase, matDE, matDY)) != OK) return pub(st);
     DeviceGuard guard(handle->device);
     EmbeddingArgs a = embedding_args(count, indices, indexType, idxBase, matDE, matDY);
     a.alpha = scalar(handle, alpha);

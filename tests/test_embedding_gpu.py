@@ -301,3 +301,28 @@ def test_refusals(handle, device):
         mc.embedding_lookup(handle, ids.float(), m_e, m_y)
     with pytest.raises(ValueError):
         mc.embedding_gradient(handle, ids, m_y, m_e, torch.empty(8, dtype=torch.uint8, device=device))
+
+
+def test_matrices_without_values_are_refused(handle, device):
+    """mcsparseDnMatSetValues may take a descriptor's values away: refused on the host, as the library's other products do."""
+    E, Y = torch.full((10, 16), 7.0, device=device), torch.full((4, 16), 7.0, device=device)
+    ids = torch.zeros(4, dtype=torch.int64, device=device)
+    m_e, m_y = mat(E), mat(Y)
+    buf = torch.empty(mc.embedding_gradient_buffer_size(handle, ids, m_y, m_e), dtype=torch.uint8, device=device)
+    for m in (m_e, m_y):
+        capi.check(lib.mcsparseDnMatSetValues(m.d, None))
+        for call in (lambda: mc.embedding_lookup(handle, ids, m_e, m_y), lambda: mc.embedding_gradient(handle, ids, m_y, m_e, buf)):
+            with pytest.raises(mc.McsparseError) as e:
+                call()
+            assert e.value.status == capi.MCSPARSE_STATUS_INVALID_VALUE
+        capi.check(lib.mcsparseDnMatSetValues(m.d, m.values.data_ptr()))
+    torch.cuda.synchronize()
+    assert bool((E == 7.0).all()) and bool((Y == 7.0).all())
+    # none are missing where there are none
+    capi.check(lib.mcsparseDnMatSetValues(m_y.d, None))
+    empty = mc.DnMat(Y, 0, 16, 16)
+    capi.check(lib.mcsparseDnMatSetValues(empty.d, None))
+    mc.embedding_lookup(handle, ids[:0], m_e, empty)
+    mc.embedding_gradient(handle, ids[:0], empty, m_e, buf, beta=1.0)
+    torch.cuda.synchronize()
+    assert bool((E == 7.0).all())
