@@ -337,7 +337,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     // tensor memory: the buffers of S and dP, 64 columns each, then the sums (dV and dK, or M and dQ)
     const uint32_t t_s = tmem, t_dp = tmem + kBuffers * kTile, t_out1 = tmem + 2 * kBuffers * kTile, t_out2 = t_out1 + DP;
     bool failed = false;
-    if (warp != kLoadWarp) grid_wait();  // (before any wait that is timed)
+    // (before any wait that is timed; the load warp has loads to issue first, and waits in publish() if it gets there without any)
+    if (warp != kLoadWarp) grid_wait();
 
     // All warps run through the same work, each with running counts of the barriers' phases: `total` tiles, `turns` works with tiles.
     int turn = 0, total = 0, turns = 0;
@@ -391,6 +392,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         int asked = 0;
         const auto publish = [&](int row0) {
             const int at = turn & 1;
+            // (the other warps take nothing before the launch ahead is done; works without tiles come here without having waited)
+            if (turn >= 2 && turns == 0) grid_wait();
             if (turn >= 2 && !bar_wait_warp(bar_taken + 8 * at, ((turn >> 1) - 1) & 1, a.limit)) {
                 failed = true;
                 return;

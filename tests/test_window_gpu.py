@@ -615,3 +615,36 @@ def test_refusals(handle, device):
         mc.window_attention(handle, w, q, k, k, out, k_offsets=off)
     with pytest.raises(ValueError):
         mc.window_attention_backward(handle, w, q, k, k, out, None, q, q, k, k, torch.empty(1 << 20, dtype=torch.uint8, device=device))
+
+
+def test_a_short_wait_limit_does_not_count_the_launch_ahead(device):
+    """Backward: the keys' launch comes up while the queries' launch still runs on one SM for milliseconds. Its blocks start with
+    keys that no query sees, which need no loads; waiting for the launch ahead must not use up the limit of their own waits."""
+    handle = mc.Handle()
+    d, unseen, long_keys, rows = 64, 148 * 8 * 128, 1 << 20, 128
+    n = unseen + long_keys
+    w = mc.Window(1 << 40, 0, 1, 1, d, torch.bfloat16)
+    gen = torch.Generator(device=device).manual_seed(61)
+    q, g = (normal((rows, 1, d), torch.bfloat16, device, gen) for _ in range(2))
+    k, v = (normal((n, 1, d), torch.bfloat16, device, gen) for _ in range(2))
+    qo = torch.tensor([0, 0, rows], dtype=torch.int32, device=device)
+    ko = torch.tensor([0, unseen, n], dtype=torch.int32, device=device)
+    out, lse = torch.empty_like(q), torch.empty(1, rows, device=device)
+    buf = torch.empty(mc.window_attention_backward_buffer_size(handle, w, 2, rows, n), dtype=torch.uint8, device=device)
+    mc.window_attention(handle, w, q, k, v, out, lse, q_offsets=qo, k_offsets=ko)
+    results = []
+    for limit in (40_000_000, 60_000):  # 64 times that: over a second, and 2 ms
+        grads = [torch.full_like(x, 7.0) for x in (q, k, v)]
+        torch.cuda.synchronize()
+        capi.check(lib.mcsparseB200SetDeviceWaitLimit(handle.h, limit, 0))
+        mc.window_attention_backward(handle, w, q, k, v, out, lse, g, *grads, buf, q_offsets=qo, k_offsets=ko)
+        torch.cuda.synchronize()
+        capi.check(lib.mcsparseB200SetDeviceWaitLimit(handle.h, 40_000_000, 0))
+        mc.window_attention(handle, w, q, k, v, out, lse, q_offsets=qo, k_offsets=ko)  # raises if a block gave up
+        results.append(grads)
+    for name, x, y in zip(("dq", "dk", "dv"), *results):
+        assert torch.equal(x, y), name
+    for x in results[1][1:]:
+        assert not bool(x[:unseen].any()), "keys that no query sees get zeros"
+        assert bool(x[unseen:].isfinite().all()) and bool(x[unseen:].any())
+    handle.close()
