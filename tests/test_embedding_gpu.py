@@ -326,3 +326,31 @@ def test_matrices_without_values_are_refused(handle, device):
     mc.embedding_gradient(handle, ids[:0], empty, m_e, buf, beta=1.0)
     torch.cuda.synchronize()
     assert bool((E == 7.0).all())
+
+
+def gradient_time(handle, device, count, width, hot):
+    """Median milliseconds of a gradient (beta = 1) of `count` tokens, a share `hot` of them with one id, the others spread."""
+    rows = 50000
+    gen = torch.Generator(device=device).manual_seed(count)
+    ids = torch.randint(0, rows, (count,), device=device, generator=gen)
+    ids[torch.rand(count, device=device, generator=gen) < hot] = 7
+    dy, table = torch.ones(count, width, dtype=torch.bfloat16, device=device), torch.zeros(rows, width, device=device)
+    m_y, m_e = mat(dy), mat(table)
+    buf = torch.empty(mc.embedding_gradient_buffer_size(handle, ids, m_y, m_e), dtype=torch.uint8, device=device)
+    times = []
+    for _ in range(7):
+        start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        torch.cuda.synchronize()
+        start.record()
+        mc.embedding_gradient(handle, ids, m_y, m_e, buf, beta=1.0)
+        end.record()
+        torch.cuda.synchronize()
+        times.append(start.elapsed_time(end))
+    return sorted(times)[3]
+
+
+def test_time_of_a_run_grows_with_its_length(handle, device):
+    """Eight times as many tokens of one id cost about eight times as much (with chunks that look for each other's ends one after
+    the other: 21 times)."""
+    short, long = (gradient_time(handle, device, n, 512, 1.0) for n in (1 << 19, 1 << 22))
+    assert long < 13 * short, f"{short} ms and {long} ms"
