@@ -354,3 +354,35 @@ def test_time_of_a_run_grows_with_its_length(handle, device):
     the other: 21 times)."""
     short, long = (gradient_time(handle, device, n, 512, 1.0) for n in (1 << 19, 1 << 22))
     assert long < 13 * short, f"{short} ms and {long} ms"
+
+
+@pytest.mark.parametrize("types,width", [((torch.float32, torch.bfloat16), 8), ((torch.float32, torch.float32), 140), ((torch.float32, torch.bfloat16), 264),
+                                         ((torch.float32, torch.float16), 131)], ids=str)
+def test_gradient_of_runs_over_many_chunks(handle, device, types, width):
+    """Sums over 1 to 2250 chunks of 8 tokens, at the numbers of chunks where their groups change, and beginning and ending anywhere in
+    a chunk. Whole numbers whose sums stay below 2^24: every order of additions gives the same bits, and a chunk that is
+    missing or counted twice shows."""
+    gen = torch.Generator(device=device).manual_seed(width)
+    parts = [1, 2, 63, 64, 65, 66, 80, 81, 255, 256, 257, 258, 271, 272, 273, 1024, 1025]
+    runs = [8 * n + e for n in parts for e in (-3, 0, 5)]
+    te, ty = types
+    batches = [[]]
+    for n in runs + [18000]:
+        if sum(batches[-1]) + n > 18000:
+            batches.append([])
+        batches[-1].append(n)
+    for lengths in batches:
+        ids = torch.repeat_interleave(torch.arange(len(lengths), device=device), torch.tensor(lengths, device=device))
+        ids = ids[torch.randperm(len(ids), generator=gen, device=device)]
+        assert len(ids) * -(-width // 256) // (148 * 16) < 16, "chunks of 8 tokens"
+        dy = torch.randint(-8, 9, (len(ids), width), device=device, generator=gen).to(ty)
+        table = torch.randint(-8, 9, (len(lengths), width), device=device, generator=gen).to(te)
+        want = table.double().index_add(0, ids, 2.0 * dy.double())
+        run_gradient(handle, ids, dy, table, alpha=2.0, beta=1.0)
+        assert torch.equal(table.double(), want)
+
+
+def test_one_id_in_all_tokens_costs_little_more_than_spread_ids(handle, device):
+    """(One warp for all the partial sums of a row: 11 times as much.)"""
+    spread, one = (gradient_time(handle, device, 1 << 22, 512, hot) for hot in (0.0, 1.0))
+    assert one < 3 * spread, f"{spread} ms and {one} ms"
