@@ -750,7 +750,7 @@ GradientLayout gradient_layout(int64_t count, int64_t rows, int64_t width) {
     l.chunks = (count + l.chunk - 1) / l.chunk;
     size_t off = 0;
     if (count > kSortAlone) {  // (room for it whatever the device holds: the size is asked for without one)
-        l.sort = transpose_plan(rows, rows + 1, count, 0);
+        l.sort = sort_plan(rows + 1, count);
         off = l.sort.bytes;
         l.off_raw = off;
         off += align256(size_t(count) * 4);
@@ -840,7 +840,7 @@ cudaError_t launch_gradient(cudaStream_t s, const EmbeddingArgs& a, char* b) {
     if (a.count > 0 && so.sorters == 0) {
         int* raw = reinterpret_cast<int*>(b + l.off_raw);
         embedding_keys_kernel<<<(unsigned)((a.count + 255) / 256), 256, 0, s>>>(so, raw);
-        const cudaError_t e = sort_keys(s, a.rows, a.count, raw, l.sort, b);
+        const cudaError_t e = sort_keys(s, a.count, raw, l.sort, b);
         if (e != cudaSuccess) return e;
         const int slot = l.sort.final_slot();
         last = 0;

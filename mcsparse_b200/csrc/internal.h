@@ -339,11 +339,10 @@ cudaError_t transpose_structure(cudaStream_t s, int64_t m, int64_t n, int64_t nn
 template <typename I>
 cudaError_t coo_sort_structure(cudaStream_t s, int64_t key_range, int64_t nnz, int base, const I* key_idx,
                                const I* other_idx, const TransposePlan& plan, void* buf);
-// The same sort alone: 0-based keys in [0, key_range] sorted with their positions (keys[final_slot()], perm[final_slot()]),
-// and the first place of every key in [0, key_range) at off_ptr (key_range + 1 entries; the last one is where the keys
-// equal to key_range start). The plan is transpose_plan(any, key_range + 1, count, any).
-cudaError_t sort_keys(cudaStream_t s, int64_t key_range, int64_t count, const int32_t* keys, const TransposePlan& plan,
-                      void* buf);
+// The same sort alone: 0-based keys in [0, key_range) sorted with their positions (keys[final_slot()], perm[final_slot()]). Its
+// plan has no room for offsets: its size depends on count alone.
+TransposePlan sort_plan(int64_t key_range, int64_t count);
+cudaError_t sort_keys(cudaStream_t s, int64_t count, const int32_t* keys, const TransposePlan& plan, void* buf);
 // Array-of-pairs COO indices (row0, col0, row1, col1, ...; 8-byte aligned) -> two arrays.
 cudaError_t split_index_pairs(cudaStream_t s, int64_t nnz, const int32_t* pairs, int32_t* rows, int32_t* cols);
 // *host_flag = 1 if idx[0 .. count) is not ascending (one kernel, a 4-byte copy, a stream synchronisation).

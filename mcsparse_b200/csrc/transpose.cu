@@ -277,18 +277,18 @@ cudaError_t exclusive_scan_u32(cudaStream_t s, unsigned* data, long long count, 
     return cudaGetLastError();
 }
 
-TransposePlan transpose_plan(int64_t m, int64_t n, int64_t nnz, size_t value_size) {
-    (void)m;
+// `keys`: how many different ones there may be; `offsets`: row offsets to make room for.
+static TransposePlan plan_of(int64_t keys, int64_t nnz, size_t value_size, int64_t offsets) {
     TransposePlan p;
     int bits = 1;
-    while (bits < 31 && (int64_t(1) << bits) < n) ++bits;
+    while (bits < 31 && (int64_t(1) << bits) < keys) ++bits;
     p.passes = (bits + 7) / 8;
     p.tiles = (nnz + kSortTile - 1) / kSortTile;
     p.hist_count = 256 * p.tiles;
     p.scan_chunks = (p.hist_count + kScanChunk - 1) / kScanChunk;
     size_t off = 0;
     p.off_ptr = off;
-    off += align256(size_t(n + 1) * 4);
+    off += align256(size_t(offsets) * 4);
     for (int i = 0; i < 2; ++i) {
         p.off_keys[i] = off;
         off += align256(size_t(nnz) * 4);
@@ -306,6 +306,13 @@ TransposePlan transpose_plan(int64_t m, int64_t n, int64_t nnz, size_t value_siz
     p.bytes = off;
     return p;
 }
+
+TransposePlan transpose_plan(int64_t m, int64_t n, int64_t nnz, size_t value_size) {
+    (void)m;
+    return plan_of(n, nnz, value_size, n + 1);
+}
+
+TransposePlan sort_plan(int64_t key_range, int64_t count) { return plan_of(key_range, count, 0, 0); }
 
 // Stable sort of the positions 0 .. nnz-1 by key (key - base in [0, 2^(8 passes))): leaves the sorted
 // 0-based keys in keys[final_slot()] and the permutation in perm[final_slot()].
@@ -357,12 +364,8 @@ cudaError_t coo_sort_structure(cudaStream_t s, int64_t key_range, int64_t nnz, i
     return e;
 }
 
-cudaError_t sort_keys(cudaStream_t s, int64_t key_range, int64_t count, const int32_t* keys, const TransposePlan& p, void* buf) {
-    char* b = static_cast<char*>(buf);
-    const cudaError_t e = radix_sort_positions(s, count, 0, keys, p, buf);
-    if (e != cudaSuccess) return e;
-    return coo_row_offsets(s, key_range, count, 0, reinterpret_cast<const int*>(b + p.off_keys[p.final_slot()]),
-                           reinterpret_cast<int32_t*>(b + p.off_ptr));
+cudaError_t sort_keys(cudaStream_t s, int64_t count, const int32_t* keys, const TransposePlan& p, void* buf) {
+    return radix_sort_positions(s, count, 0, keys, p, buf);
 }
 
 __device__ int g_unsorted_flag;  // result word of indices_unsorted (one check at a time per process)

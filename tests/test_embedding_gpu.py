@@ -386,3 +386,29 @@ def test_one_id_in_all_tokens_costs_little_more_than_spread_ids(handle, device):
     """(One warp for all the partial sums of a row: 11 times as much.)"""
     spread, one = (gradient_time(handle, device, 1 << 22, 512, hot) for hot in (0.0, 1.0))
     assert one < 3 * spread, f"{spread} ms and {one} ms"
+
+
+@pytest.mark.parametrize("count", [100, 5000, 140001])
+def test_gradient_buffer_does_not_grow_with_the_table(handle, device, count):
+    """The sort needs room for the tokens, not for the rows (it once reserved a word for each of them, a gigabyte at 2^28)."""
+    ids = torch.zeros(count, dtype=torch.int32, device=device)
+    dy, table = torch.empty(count, 2, device=device), torch.empty(1, 2, device=device)  # (sizes alone are looked at)
+    sizes = [mc.embedding_gradient_buffer_size(handle, ids, mat(dy), mc.DnMat(table, rows, 2, 2)) for rows in (10, 50000, 1 << 28)]
+    assert sizes[0] == sizes[1] == sizes[2], sizes
+
+
+@pytest.mark.parametrize("kind", ["one", "outside", "edges", "skewed"])
+@pytest.mark.parametrize("index,base", [(torch.int32, 1), (torch.int64, 0)], ids=str)
+@pytest.mark.parametrize("rows", [200, 70000, 1 << 26])
+def test_gradient_of_more_tokens_than_one_cluster_sorts(handle, device, kind, index, base, rows):
+    """140001 tokens, ids of one to four digits, and those outside the table, whose key is the number of rows."""
+    count = 140001
+    gen = torch.Generator(device=device).manual_seed(rows)
+    ids = ids_for(count, rows, kind, device, seed=3, index=index, base=base)
+    dy = torch.randint(-4, 5, (count, 8), device=device, generator=gen).bfloat16()  # whole numbers: any order of additions is exact
+    table = torch.zeros(rows, 8, device=device)
+    run_gradient(handle, ids, dy, table, beta=1.0, base=base)
+    i = ids.long() - base
+    ok = (i >= 0) & (i < rows)
+    want = torch.zeros(rows, 8, device=device).index_add_(0, i[ok], dy[ok].float())
+    assert torch.equal(table, want)
