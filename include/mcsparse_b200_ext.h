@@ -310,7 +310,8 @@ typedef struct mcsparseB200Heads {
  * are rounded to the inputs' type for the product with V, and O is rounded once. Asynchronous, no buffer, no allocation. The
  * tensor-core kernels' waits are bounded by 64 times the handle's device wait limit (mcsparseB200SetDeviceWaitLimit): a block
  * that gives up leaves its rows unwritten, and the next forward or backward call on the handle returns
- * MCSPARSE_STATUS_EXECUTION_FAILED once.
+ * MCSPARSE_STATUS_EXECUTION_FAILED once, before doing anything else (mcsparseSpMV and its kin report their own waits alone;
+ * the single-token and the embedding calls have no such waits and report none).
  */
 mcsparseStatus_t mcsparseB200WindowAttention(mcsparseHandle_t handle, mcsparseB200WindowDescr_t descr, int64_t batch,
                                              const int32_t* qOffsets, const int32_t* kOffsets, int64_t totalQ,

@@ -174,7 +174,7 @@ WaitCfg wait_cfg(const mcsparseContext* h) {
 }
 
 bool take_device_fault(mcsparseContext* h) {
-    return api::take_device_fault(h, "an earlier call on this handle gave up a bounded device-side wait; its result is incomplete");
+    return api::take_device_fault(h->fault_word_host, "an earlier SpMV on this handle gave up a bounded device-side wait; its result is incomplete");
 }
 
 struct PushArgs {

@@ -102,11 +102,11 @@ inline bool value_type_known(macaDataType t) {
     }
 }
 
-// A kernel of an earlier call on this handle gave up a bounded wait: reported once, by the next compute call, as an execution
-// failure (the word lives in pinned host memory the kernels can write, so reading it needs no synchronisation).
-inline bool take_device_fault(mcsparseContext* h, const char* what) {
-    if (h->fault_word_host == nullptr || *reinterpret_cast<volatile int*>(h->fault_word_host) == 0) return false;
-    *reinterpret_cast<volatile int*>(h->fault_word_host) = 0;
+// A kernel of an earlier call on a handle gave up a bounded wait: reported once, by the next compute call of its kind, as an
+// execution failure (the word lives in pinned host memory the kernels can write, so reading it needs no synchronisation).
+inline bool take_device_fault(int* word, const char* what) {
+    if (word == nullptr || *reinterpret_cast<volatile int*>(word) == 0) return false;
+    *reinterpret_cast<volatile int*>(word) = 0;
     log_error(what);
     return true;
 }

@@ -20,15 +20,19 @@ mcsparseStatus_t mcsparseCreate(mcsparseHandle_t* handle) {
     if (ctx == nullptr) return MCSPARSE_STATUS_ALLOC_FAILED;
     ctx->device = dev;
     cudaDeviceGetAttribute(&ctx->sm_count, cudaDevAttrMultiProcessorCount, dev);
-    // One word of pinned host memory that kernels can write: a tile kernel that gives up its bounded
-    // wait says so here, and the next compute call reports it without a synchronisation. Without it
-    // (allocation refused) such a failure is still recorded in the work buffer's status word.
+    // Two words of pinned host memory that kernels can write: a tile kernel (or an attention kernel) that gives up its bounded
+    // wait says so there, and the next compute call of its kind reports it without a synchronisation. Without them
+    // (allocation refused) a tile's failure is still recorded in the work buffer's status word.
     void* word = nullptr;
-    if (cudaHostAlloc(&word, sizeof(int), cudaHostAllocMapped) == cudaSuccess) {
+    if (cudaHostAlloc(&word, 2 * sizeof(int), cudaHostAllocMapped) == cudaSuccess) {
         ctx->fault_word_host = static_cast<int*>(word);
-        *ctx->fault_word_host = 0;
+        ctx->attention_fault_host = ctx->fault_word_host + 1;
+        *ctx->fault_word_host = *ctx->attention_fault_host = 0;
         void* dev_view = nullptr;
-        if (cudaHostGetDevicePointer(&dev_view, word, 0) == cudaSuccess) ctx->fault_word_dev = static_cast<int*>(dev_view);
+        if (cudaHostGetDevicePointer(&dev_view, word, 0) == cudaSuccess) {
+            ctx->fault_word_dev = static_cast<int*>(dev_view);
+            ctx->attention_fault_dev = ctx->fault_word_dev + 1;
+        }
     } else {
         cudaGetLastError();
     }

@@ -40,6 +40,10 @@ struct mcsparseContext {
     int withhold_copies = 0;           // diagnostics: issue no bulk copies, so that every wait runs out
     int* fault_word_host = nullptr;
     int* fault_word_dev = nullptr;
+    // The same for the attention kernels, which the next attention call reports: its own word, so that neither kind of call
+    // takes what the other kind's next call is to report.
+    int* attention_fault_host = nullptr;
+    int* attention_fault_dev = nullptr;
     // L2 residency of x (see XResidency in api.cpp): the device's largest persisting carve-out, read once, and
     // whether this handle has already asked for it.
     long long max_persisting_l2 = -1;

@@ -23,7 +23,7 @@ ScalarArg<float> scalar(const mcsparseContext* h, const void* p) {
 }
 
 bool gave_up(mcsparseContext* h) {
-    return take_device_fault(h, "an earlier call on this handle gave up a bounded device-side wait; its result is incomplete");
+    return take_device_fault(h->attention_fault_host, "an earlier attention call on this handle gave up a bounded device-side wait; its result is incomplete");
 }
 
 // ----------------------------------------------------------------------------- embedding
@@ -118,7 +118,7 @@ St attention_sizes(mcsparseHandle_t h, const mcsparseB200WindowDescr* d, int64_t
     a->scale = d->scale, a->type = d->valueType;
     a->sm_count = h->sm_count > 0 ? h->sm_count : 148;
     a->wait.limit_cycles = h->wait_cycles;
-    a->wait.fault_word = h->fault_word_dev;
+    a->wait.fault_word = h->attention_fault_dev;
     return OK;
 }
 

@@ -648,3 +648,43 @@ def test_a_short_wait_limit_does_not_count_the_launch_ahead(device):
         assert not bool(x[:unseen].any()), "keys that no query sees get zeros"
         assert bool(x[unseen:].isfinite().all()) and bool(x[unseen:].any())
     handle.close()
+
+
+def test_each_kind_of_call_reports_its_own_waits(device):
+    """An attention call that gave up is not reported by mcsparseSpMV, nor the other way round; both are reported once."""
+    handle = mc.Handle()
+    gen = torch.Generator(device=device).manual_seed(67)
+    n, w = 300, mc.Window(50, 1, 2, 2, 64, torch.bfloat16)
+    q, k, v = (normal((n, 2, 64), torch.bfloat16, device, gen) for _ in range(3))
+    out, one = torch.empty_like(q), torch.empty(1, 2, 64, dtype=torch.bfloat16, device=device)
+    room = torch.empty(mc.window_attention_decode_buffer_size(handle, w, 1, 1, n), dtype=torch.uint8, device=device)
+    length = torch.tensor([n], dtype=torch.int32, device=device)
+    rows = 20000  # a diagonal of ones and one below it
+    ptr = (2 * torch.arange(rows + 1, device=device)).int()
+    col = (torch.arange(2 * rows, device=device) // 2 - (torch.arange(2 * rows, device=device) % 2)).clamp_min(0).int()
+    A = mc.CsrMatrix(rows, rows, ptr, col, torch.ones(2 * rows, device=device))
+    x, y = mc.DnVec(torch.ones(rows, device=device)), mc.DnVec(torch.zeros(rows, device=device))
+    buf = torch.empty(max(mc.spmv_buffer_size(handle, A, x, y), 16), dtype=torch.uint8, device=device)
+
+    def limit(clocks, withhold):
+        torch.cuda.synchronize()
+        capi.check(lib.mcsparseB200SetDeviceWaitLimit(handle.h, clocks, withhold))
+
+    attention = lambda: mc.window_attention(handle, w, q, k, v, out)
+    spmv = lambda: mc.spmv(handle, A, x, y, buf)
+    others = lambda: mc.window_attention_decode(handle, w, q[-1:], k[None], v[None], length, one, buffer=room)
+    attention(), spmv(), others()
+    for fails, clocks, withhold, fine in ((attention, 1, 0, spmv), (spmv, 100_000, 1, attention)):
+        limit(clocks, withhold)
+        fails()
+        limit(40_000_000, 0)
+        fine(), others()
+        with pytest.raises(mc.McsparseError) as e:
+            fails()
+        assert e.value.status == capi.MCSPARSE_STATUS_EXECUTION_FAILED
+        fails(), fine()
+    torch.cuda.synchronize()
+    assert bool((y.values == 2).all())
+    want = ref.attention(q, k, v, 50, 1, w.scale)
+    ref.close(out, want["out"], "out")
+    handle.close()
