@@ -322,7 +322,9 @@ mcsparseStatus_t mcsparseB200WindowAttention(mcsparseHandle_t handle, mcsparseB2
  * mcsparseB200WindowAttentionBackward: gradients of the same product. o and lse: what the forward call wrote; dO: the gradient
  * of O; dQ, dK, dV are written (rows in no sequence are left as they were; keys that no query sees get zeros; shared key
  * heads get the sum over their query heads). No atomics: equal inputs give equal bits. A dO that is not finite may reach
- * every gradient of its sequence. externalBuffer: the bytes that _bufferSize reports, free again when the call's work is done.
+ * every gradient of its sequence. Scores, dP and all sums are fp32; with 16-bit inputs the tensor-core kernels round P and
+ * dS = P * (dP - rowsum(dO * O)) to the inputs' type for the products with dO, K and Q, and every gradient once. In fp16 a dS below
+ * 2^-14 loses bits: scale a small dO. externalBuffer: the bytes that _bufferSize reports, free again when the call's work is done.
  */
 mcsparseStatus_t mcsparseB200WindowAttentionBackward_bufferSize(mcsparseHandle_t handle, mcsparseB200WindowDescr_t descr,
                                                                 int64_t batch, int64_t totalQ, int64_t totalK,
@@ -340,7 +342,8 @@ mcsparseStatus_t mcsparseB200WindowAttentionBackward(
  * (h, d) at values[page * pageStride + token * tokenStride + h * headStride + d]. lengths: device int32; a length is taken
  * as at most maxPages * pageSize, 0 (or less) gives zeros and lse = -inf. Tokens of a page number outside [0, numPages) are
  * not seen; pages that lie wholly outside the window and the sinks are not read, their numbers neither.
- * q, o: batch x qHeads x headDim (a token per sequence). lse: batch x qHeads floats, may be NULL.
+ * q, o: batch x qHeads x headDim (a token per sequence). lse: batch x qHeads floats, may be NULL. Roundings as in the forward
+ * call: 16-bit weights for the product with V, everything else fp32, O rounded once.
  */
 typedef struct mcsparseB200Cache {
     void* values;

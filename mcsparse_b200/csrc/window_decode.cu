@@ -22,7 +22,9 @@ constexpr int kKeys = 16;    // keys of a tile
 constexpr int kHeads = 16;   // query heads of a block
 constexpr int kCluster = 8;  // most blocks of one sequence and key head that join without the work buffer
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kSlack = 8.0f;  // a row's reference follows its maximum in steps of at least 2^8 (weights stay below 256)
+// A row's reference follows its maximum in steps of at least 2^8, so that weights stay below 256, far from fp16's 65504. The product
+// with V takes them rounded to the inputs' type (one 16-bit type for both operands), the row's sum in fp32.
+constexpr float kSlack = 8.0f;
 
 template <int DP>
 struct Ring {
@@ -372,8 +374,9 @@ int64_t decode_items(const DecodeArgs& a) {
 }
 
 // Parts per sequence and key head. A part costs its keys and about 250 more (its start, its first loads, the join: fitted to
-// 64 sequences x 8 key heads x 4100 keys, where 1, 2, 3 parts took 196, 206, 217 us); two blocks run per SM, so the launch costs
-// its whole rounds of blocks. At least 64 keys (a tile per warp) each. Up to 8 parts join as a cluster; more take the work buffer
+// 64 sequences x 8 key heads x 4100 keys, where 1, 2, 3 parts took 196, 206, 217 us); with headDim above 64, which it was fitted
+// for, two blocks run per SM, so the launch costs its whole rounds of blocks (headDim up to 64: three fit, and the count of rounds
+// is too high). At least 64 keys (a tile per warp) each. Up to 8 parts join as a cluster; more take the work buffer
 // and a second launch (200 keys' worth) and only come into question when an eighth is still long.
 int decode_splits(const DecodeArgs& a) {
     const int64_t room = a.max_pages * a.page_size, items = decode_items(a);

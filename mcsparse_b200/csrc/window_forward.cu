@@ -31,7 +31,9 @@ constexpr int kLoadWarp = kSoftmaxWarps, kScoreWarp = kSoftmaxWarps + 1, kValueW
 constexpr int kThreads = 32 * (kSoftmaxWarps + 4);
 constexpr float kLog2e = 1.4426950408889634f;
 // The running reference of a row's exponentials is only moved when its maximum has grown past it by more than 2^8: until
-// then the weights are at most 256 (exact in fp32 sums, far from fp16's 65504) and O needs no rescaling.
+// then the weights are at most 256, far from fp16's 65504, and O needs no rescaling. A weight enters the product with V rounded
+// to the inputs' type (the tensor cores take both operands of one 16-bit type), and the row's sum as it is in fp32: O differs from
+// the exact one by the half step of each weight, by the fp32 sums, and by its own rounding, of which the first is the largest part.
 constexpr float kSlack = 8.0f;
 
 template <int DP>
