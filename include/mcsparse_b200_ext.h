@@ -324,7 +324,7 @@ mcsparseStatus_t mcsparseB200WindowAttention(mcsparseHandle_t handle, mcsparseB2
  * heads get the sum over their query heads). No atomics: equal inputs give equal bits. A dO that is not finite may reach
  * every gradient of its sequence. Scores, dP and all sums are fp32; with 16-bit inputs the tensor-core kernels round P and
  * dS = P * (dP - rowsum(dO * O)) to the inputs' type for the products with dO, K and Q, and every gradient once. In fp16 a dS below
- * 2^-14 loses bits: scale a small dO. externalBuffer: the bytes that _bufferSize reports, free again when the call's work is done.
+ * 2^-14 loses bits and one above 65504 is infinite: dO has to be scaled between them. externalBuffer: the bytes that _bufferSize reports, free again when the call's work is done.
  */
 mcsparseStatus_t mcsparseB200WindowAttentionBackward_bufferSize(mcsparseHandle_t handle, mcsparseB200WindowDescr_t descr,
                                                                 int64_t batch, int64_t totalQ, int64_t totalK,

@@ -688,3 +688,42 @@ def test_each_kind_of_call_reports_its_own_waits(device):
     want = ref.attention(q, k, v, 50, 1, w.scale)
     ref.close(out, want["out"], "out")
     handle.close()
+
+
+def decode_parts(handle, batch, hq, hk, d, dtype, window, sinks, per, page):
+    """Parts of a sequence, by the room that their sums take in the work buffer (0: at most 8, which take none)."""
+    size = mc.window_attention_decode_buffer_size(handle, mc.Window(window, sinks, hq, hk, d, dtype), batch, per, page)
+    tiles = -(-(hq // hk) // 16)
+    return (size - 256) // (batch * hk * tiles * 16 * ((64 if d <= 64 else 128) + 2) * 4)
+
+
+@pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 128), (torch.float16, 64), (torch.bfloat16, 40), (torch.float16, 72)], ids=str)
+@pytest.mark.parametrize("page", [0, 16, 37])
+@pytest.mark.parametrize("heads,lengths,window,sinks,parts", [
+    ((16, 16), [8192], 1 << 40, 0, 16),             # the fewest visible keys that take the work buffer
+    ((32, 8), [9001, 0, 3, 700, 8193], 8500, 5, 8),  # (five sequences: a cluster each)
+    ((32, 8), [9001], 8500, 5, 32),
+    ((18, 1), [30011, 1], 20000, 130, 64),          # two tiles of query heads
+    ((4, 1), [65536], 1 << 40, 0, 64),
+], ids=str)
+def test_decode_over_many_parts(handle, device, dtype, d, page, heads, lengths, window, sinks, parts):
+    """Long visible caches: the parts of a sequence are joined through the work buffer. What no query sees is NaN."""
+    gen = torch.Generator(device=device).manual_seed(71)
+    q, k, v, table = decode_case(device, dtype, lengths, page, *heads, d, gen, window, sinks)
+    per = 1 if table is None else table.shape[1]
+    got = decode_parts(handle, len(lengths), *heads, d, dtype, window, sinks, per, k.shape[1])
+    assert (got if parts > 8 else max(got, 8)) == parts
+    seen = torch.zeros(k.shape[:2], dtype=torch.bool, device=device)
+    for b, n in enumerate(lengths):
+        j = torch.arange(n, device=device)
+        j = j[(j > n - 1 - window) | (j < sinks)]
+        seen[torch.full_like(j, b) if table is None else table[b].long()[j // k.shape[1]], j % k.shape[1]] = True
+    k[~seen] = float("nan")
+    v[~seen] = float("inf")
+    out, lse = decode_check(handle, q, k, v, table, lengths, window, sinks)
+    again = decode_check(handle, q, k, v, table, lengths, window, sinks)
+    assert torch.equal(out, again[0]) and torch.equal(lse, again[1]), "equal inputs, equal bits"
+    if page:  # pages outside the cache are not seen, whichever part they fall to
+        table[0, ::3] = -1
+        table[0, 1::9] = k.shape[0]
+        decode_check(handle, q, k, v, table, lengths, window, sinks)
