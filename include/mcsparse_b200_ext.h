@@ -184,7 +184,7 @@ mcsparseStatus_t mcsparseB200SpMVPushMulticast(mcsparseHandle_t handle, mcsparse
  * i.e. until every peer's rows of that step are in this GPU's memory. Epochs must grow from step to step
  * (compared modulo 2^32). The wait is bounded (fifty times the handle's device wait limit, about a second):
  * when it runs out the kernel sets bit 0 of the status word and the handle's fault word and returns, and the
- * next compute call on the handle reports MCSPARSE_STATUS_EXECUTION_FAILED. The waiting kernels of the ranks
+ * next such call or SpMV on the handle reports MCSPARSE_STATUS_EXECUTION_FAILED. The waiting kernels of the ranks
  * run on different GPUs; never run two ranks of one job on the same GPU. No reference counterpart.
  */
 #define MCSPARSE_B200_PEER_FLAG_INTS 16

@@ -35,7 +35,7 @@ struct mcsparseContext {
     cudaStream_t capture_stream = nullptr;  // origin stream while the step is captured as a graph
     // Bounded device-side waits: how long a thread block waits for the bulk copies of its tile (SM clocks),
     // and a word in pinned, device-mapped host memory that a kernel sets when it gave a tile up. The next
-    // compute call on the handle reads the word on the host (no synchronisation) and reports it.
+    // SpMV or peer-flag call on the handle reads the word on the host (no synchronisation) and reports it.
     long long wait_cycles = 40000000;  // about 20 ms of SM clocks
     int withhold_copies = 0;           // diagnostics: issue no bulk copies, so that every wait runs out
     int* fault_word_host = nullptr;
