@@ -442,7 +442,7 @@ __global__ void __launch_bounds__(256, 4)  // (64 registers: 389 us against 401 
 constexpr int kSortCluster = 16;  // (8, the most that every device must hold, took 36 us against 24 for 65536 tokens)
 constexpr int kSortThreads = 1024;
 constexpr int kSortRounds = 8;  // items per thread, at most
-constexpr int kFewRounds = 2;   // the same, of the kernel for few tokens (registers and predicated code for more cost it)
+constexpr int kFewRounds = 2;   // the same, of the kernel for few tokens (room for more costs it registers and time)
 constexpr int64_t kSortAlone = kSortThreads * kFewRounds;  // tokens that one block sorts
 constexpr int64_t kSortMost = (int64_t)kSortCluster * kSortThreads * kSortRounds;
 constexpr int kMostDigits = 512;
@@ -490,8 +490,8 @@ struct SortShared {
     unsigned part[32];
 };
 
-// Lanes with the same digit as the calling one (a lane that is not live: nobody's). One vote per bit: __match_any_sync visits the
-// distinct digits one after the other, up to 32 of them (four times as long on ids as text has them).
+// Lanes with the same digit as the calling one (a lane that is not live: nobody's). One vote per bit:
+// __match_any_sync took four times as long on ids as text has them.
 __device__ __forceinline__ unsigned same_digit(unsigned d, bool live, int bits) {
     unsigned peers = __ballot_sync(0xffffffffu, live);
 #pragma unroll
